@@ -82,7 +82,7 @@ def draw(rng):
     direction = rng.choice(["forward", "train", "train"])
     if op == "norm":
         size = _size(rng, 16, 16384)
-        case = _norm("", direction, min(_log_uniform(rng, 1, 65536), (2 ** 28 - 1) // size), size, rng.choice(["bf16", "bf16", "fp16", "fp32"]))
+        case = _norm("", direction, min(_log_uniform(rng, 1, 65536), (2 ** 28 - 2 ** 17) // size), size, rng.choice(["bf16", "bf16", "fp16", "fp32"]))
         if case["dtype"] == "fp32":
             case["rows"] = max(1, case["rows"] // 2)
     elif op == "router":
