@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define STK_AMD_ABI_VERSION 21
+#define STK_AMD_ABI_VERSION 22
 
 /* status codes */
 #define STK_OK 0
@@ -605,6 +605,89 @@ int stk_dsd_scatter_few_as_cut(int64_t m, int64_t k, int64_t n, const void* data
                                int64_t out_stride_m, int64_t nnz, int blocking, int dtype, int index_dtype, void* workspace,
                                int64_t workspace_bytes, const uint8_t* plan, int64_t dsd_workspace_bytes, stk_stream_t stream);
 int stk_dsd_cuts(int64_t m, int64_t n, int64_t nnz, int64_t workspace_bytes);
+
+/*
+ * Layer norm of rows and its gradients; no counterpart in the reference (the step in front of a routed layer).
+ *   y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(variance + eps),  the variance over `size`, without correction
+ * x and out are [rows, size] with x_stride, out_stride elements between rows (a stride of 0: one row for all); any size of at
+ * least 1, any alignment.  dtype STK_F16 / STK_BF16 / STK_F32; weight and bias [size] (or NULL) of param_dtype, which is dtype or
+ * STK_F32.  mean and rstd, fp32 [rows] (or both NULL), receive the statistics, which the backward pass takes.  Statistics and sums
+ * are fp32, every result is rounded once.
+ * Backward: dx [rows, size] (or NULL), dweight and dbias [size] of param_dtype (or NULL), every element of which is written (zeros
+ * where rows is 0).  The sums over the rows are added up in an order that depends on the sizes alone: the same bits every time.
+ * workspace: stk_layer_norm_backward_workspace_bytes(rows, size) bytes, 16-byte aligned, needed with dweight or dbias; nothing in it
+ * is read before it is written.
+ */
+int stk_layer_norm(const void* x, int64_t rows, int64_t size, int64_t x_stride, const void* weight, const void* bias, float eps,
+                   void* out, int64_t out_stride, float* mean, float* rstd, int dtype, int param_dtype, stk_stream_t stream);
+size_t stk_layer_norm_backward_workspace_bytes(int64_t rows, int64_t size);
+int stk_layer_norm_backward(const void* grad, int64_t grad_stride, const void* x, int64_t x_stride, const float* mean, const float* rstd,
+                            const void* weight, int64_t rows, int64_t size, void* dx, int64_t dx_stride, void* dweight, void* dbias,
+                            int dtype, int param_dtype, void* workspace, size_t workspace_bytes, stk_stream_t stream);
+
+/*
+ * A router's choice: the top_k largest of a token's scores in descending order, ties to the lower expert, and their weights
+ *   weights[t][j] = p[chosen[t][j]],  p = softmax(scores[t])          normalize: divided by their sum over j
+ * chosen [tokens, top_k] (int32) is what stk_route takes as top_experts, weights [tokens, top_k] (fp32) what stk_padded_scatter takes.
+ * scores [tokens, experts] with `stride` elements between rows; dtype STK_F16 / STK_BF16 / STK_F32; at most 1024 experts, the top
+ * 64.  A score of -infinity masks an expert: its weight is 0, and in a row with fewer than top_k others the masked ones of lowest
+ * number fill the places; a row of nothing else gets weights of 0.  A NaN ranks above every number, and a row with a NaN or
+ * +infinity gets weights of NaN.
+ * Backward: the gradient with respect to the scores, every element of it, given that of the weights (grad [tokens, top_k], fp32);
+ * with normalize the scores are not read and may be NULL.  No counterpart in the reference (see stk_route).
+ */
+int stk_top_experts(const void* scores, int64_t tokens, int64_t experts, int64_t stride, int top_k, int normalize,
+                    int32_t* chosen, float* weights, int dtype, stk_stream_t stream);
+int stk_top_experts_backward(const void* scores, int64_t stride, const int32_t* chosen, const float* weights, const float* grad,
+                             int64_t tokens, int64_t experts, int top_k, int normalize,
+                             void* dscores, int64_t dscores_stride, int dtype, stk_stream_t stream);
+
+/*
+ * Weights of 4 bits with a scale, and optionally an offset, for every group_size inputs of an output:
+ *   w[e][i][o] = scale[e][i / group_size][o] * (code[e][i][o] - 8)       without offsets
+ *              = scale * code + offset[e][i / group_size][o]             with
+ * codes 0 .. 15 (one a byte, [experts, inputs, outputs]), scales and offsets of STK_F16 / STK_BF16 [experts, groups, outputs], groups =
+ * ceil(inputs / group_size); group_size 32, 64 or a multiple of 128 (one group: any such multiple that is not below inputs).
+ * stk_quantize_4bit makes them from weights w (element strides; of w_dtype, the scales' type or STK_F32): scale = round(max |w| / 7), or
+ * with offsets scale = round((max - min) / 15) and offset = round(min), then the nearest codes.
+ * stk_pack_4bit lays them out for the products, once: stk_4bit_packed_bytes bytes, 16-byte aligned, of codes and stk_4bit_scales
+ * 16-bit elements of scales and of offsets, whose order is the library's own.  stk_dequantize_4bit writes the weights
+ * [experts, inputs, outputs] that a packed form stands for, each rounded once.  No counterpart in the reference.
+ */
+int64_t stk_4bit_packed_bytes(int64_t experts, int64_t inputs, int64_t outputs);
+int64_t stk_4bit_scales(int64_t experts, int64_t inputs, int64_t outputs, int64_t group_size);
+int stk_quantize_4bit(const void* w, int64_t stride_e, int64_t stride_i, int64_t stride_o, int64_t experts, int64_t inputs, int64_t outputs,
+                      int64_t group_size, uint8_t* codes, void* scales, void* offsets, int w_dtype, int dtype, stk_stream_t stream);
+int stk_pack_4bit(const uint8_t* codes, const void* scales, const void* offsets, int64_t experts, int64_t inputs, int64_t outputs,
+                  int64_t group_size, void* packed, void* packed_scales, void* packed_offsets, stk_stream_t stream);
+int stk_dequantize_4bit(const void* packed, const void* scales, const void* offsets, int64_t experts, int64_t inputs, int64_t outputs,
+                        int64_t group_size, void* out, int dtype, stk_stream_t stream);
+
+/*
+ * Products with packed weights (those of stk_pack_4bit; offsets NULL: none).  x is 16-bit rows of `inputs` values of the scales' type,
+ * x_stride elements apart, at any alignment; activation one of STK_ACT_NONE .. STK_ACT_SILU.  Sums are fp32 and rounded once, behind the activation.
+ *   stk_matmul_4bit           out[r] = act(x[r] w), r < rows
+ *   stk_gather_matmul_4bit    out[p] = act(x[indices[p] / top_k] w[e]), p < tokens * top_k, e the expert of the sorted position p:
+ *                             the first one with bins[e] > p.  indices and bins are stk_route's.
+ *   stk_matmul_4bit_scatter   out[t] = sum over j < top_k, in that order, of weights[s] * (x[p] w[e]), s = t * top_k + j = indices[p]
+ *                             (weights NULL: ones; x has a row for each sorted position).  The sums stay fp32 up to the one
+ *                             rounding.
+ * A row of x with an infinity or a NaN gives NaN throughout its result.  Weights of experts without rows are not read.  workspace: the
+ * stk_matmul_4bit*_workspace_bytes, 16-byte aligned, nothing in it is read before it is written (0: may be NULL).
+ */
+size_t stk_matmul_4bit_workspace_bytes(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs);
+int stk_matmul_4bit(const void* x, int64_t rows, int64_t x_stride, const void* packed, const void* scales, const void* offsets,
+                    int64_t inputs, int64_t outputs, int64_t group_size, void* out, int64_t out_stride, int activation, int dtype,
+                    void* workspace, size_t workspace_bytes, stk_stream_t stream);
+int stk_gather_matmul_4bit(const void* x, int64_t tokens, int64_t x_stride, const int32_t* indices, const int32_t* bins, int top_k,
+                           const void* packed, const void* scales, const void* offsets, int64_t experts, int64_t inputs, int64_t outputs,
+                           int64_t group_size, void* out, int64_t out_stride, int activation, int dtype,
+                           void* workspace, size_t workspace_bytes, stk_stream_t stream);
+size_t stk_matmul_4bit_scatter_workspace_bytes(int64_t slots, int64_t experts, int64_t inputs, int64_t outputs);
+int stk_matmul_4bit_scatter(const void* x, int64_t x_stride, const int32_t* indices, const int32_t* bins, int top_k, int64_t tokens,
+                            const float* weights, const void* packed, const void* scales, const void* offsets, int64_t experts,
+                            int64_t inputs, int64_t outputs, int64_t group_size, void* out, int64_t out_stride, int dtype,
+                            void* workspace, size_t workspace_bytes, stk_stream_t stream);
 
 #ifdef __cplusplus
 }

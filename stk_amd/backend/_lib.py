@@ -12,12 +12,12 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "libstk_amd.so")
 NATIVE_PATH = os.path.join(os.path.dirname(_HERE), "_native.so")
 
-ABI_VERSION = 21
+ABI_VERSION = 22
 STK_OK, STK_ERR_DIMS, STK_ERR_UNSUPPORTED, STK_ERR_HIP, STK_ERR_WORKSPACE = 0, 1, 2, 3, 4
 STK_F16, STK_BF16, STK_F32 = 0, 1, 2
 STK_I16, STK_I32 = 0, 1
 
-_p, _i64, _int, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
+_p, _i64, _int, _sz, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/stk_amd.h one to one
 SIGNATURES = {
@@ -69,6 +69,21 @@ SIGNATURES = {
     "stk_dsd_cuts": (_int, [_i64, _i64, _i64, _i64]),
     "stk_dsd_scatter_few": (_int, [_i64, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _int, _i64, _p, _i64, _i64, _int, _int, _int, _p, _i64, _p]),
     "stk_dsd_scatter_few_as_cut": (_int, [_i64, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _int, _i64, _p, _i64, _i64, _int, _int, _int, _p, _i64, _p, _i64, _p]),
+    "stk_layer_norm": (_int, [_p, _i64, _i64, _i64, _p, _p, _f32, _p, _i64, _p, _p, _int, _int, _p]),
+    "stk_layer_norm_backward_workspace_bytes": (_sz, [_i64, _i64]),
+    "stk_layer_norm_backward": (_int, [_p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _p, _i64, _p, _p, _int, _int, _p, _sz, _p]),
+    "stk_top_experts": (_int, [_p, _i64, _i64, _i64, _int, _int, _p, _p, _int, _p]),
+    "stk_top_experts_backward": (_int, [_p, _i64, _p, _p, _p, _i64, _i64, _int, _int, _p, _i64, _int, _p]),
+    "stk_4bit_packed_bytes": (_i64, [_i64, _i64, _i64]),
+    "stk_4bit_scales": (_i64, [_i64, _i64, _i64, _i64]),
+    "stk_quantize_4bit": (_int, [_p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _int, _int, _p]),
+    "stk_pack_4bit": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p]),
+    "stk_dequantize_4bit": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _int, _p]),
+    "stk_matmul_4bit_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "stk_matmul_4bit": (_int, [_p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _int, _int, _p, _sz, _p]),
+    "stk_gather_matmul_4bit": (_int, [_p, _i64, _i64, _p, _p, _int, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _int, _int, _p, _sz, _p]),
+    "stk_matmul_4bit_scatter_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "stk_matmul_4bit_scatter": (_int, [_p, _i64, _p, _p, _int, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _int, _p, _sz, _p]),
     "stk_dsd_scatter": (_int, [_i64, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _i64, _int, _int, _int, _p, _p, _i64, _p]),
 }
 

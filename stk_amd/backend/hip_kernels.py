@@ -501,3 +501,60 @@ def dsd_scatter_few(shape, data, offsets, column_indices, rhs, row_slots, slot_r
         return None
     plan = fusion_plan(offsets, column_indices, offsets_t, column_indices_t, 128) if dsd_workspace else None
     return _lib.native().dsd_scatter_few(m, k, data, offsets, column_indices, rhs, row_slots, slot_rows, top_k, weights, plan, dsd_workspace)
+
+
+# ---------------------------------------------------------------- around the products of a routed layer (no counterpart in the reference)
+def layer_norm(x, weight=None, bias=None, eps=1e-5, with_statistics=False):
+    """(result, statistics) of stk_layer_norm over the last dimension; statistics fp32 [2, rows]: mean and 1 / deviation, or None."""
+    return _lib.native().layer_norm(x, weight, bias, eps, with_statistics)
+
+
+def layer_norm_backward(grad, x, statistics, weight, bias, want_x=True, want_weight=True, want_bias=True):
+    """(dx, dweight, dbias) of stk_layer_norm_backward, None for what is not asked for or has no parameter."""
+    return _lib.native().layer_norm_backward(grad, x, statistics, weight, bias, want_x, want_weight, want_bias)
+
+
+def top_experts(scores, top_k, normalize=False):
+    """(chosen int32, weights fp32) of stk_top_experts."""
+    return _lib.native().top_experts(scores, top_k, normalize)
+
+
+def top_experts_backward(scores, chosen, weights, grad, normalize=False):
+    """Gradient with respect to the scores (stk_top_experts_backward)."""
+    return _lib.native().top_experts_backward(scores, chosen, weights, grad, normalize)
+
+
+def quantize_4bit(w, group_size, with_offsets, dtype):
+    """(codes, scales, offsets or None) of weights [experts, inputs, outputs] (stk_quantize_4bit)."""
+    return _lib.native().quantize_4bit(w, group_size, with_offsets, dtype)
+
+
+def pack_4bit(codes, scales, group_size, offsets=None):
+    """(codes, scales, offsets) in the layout of the products (stk_pack_4bit)."""
+    return _lib.native().pack_4bit(codes, scales, group_size, offsets)
+
+
+def dequantize_4bit(packed, scales, offsets, inputs, outputs, group_size):
+    """[experts, inputs, outputs] (stk_dequantize_4bit)."""
+    return _lib.native().dequantize_4bit(packed, scales, offsets, inputs, outputs, group_size)
+
+
+def matmul_4bit(x, packed, scales, offsets, inputs, outputs, group_size, activation=None):
+    """act(x @ w) (stk_matmul_4bit)."""
+    return _lib.native().matmul_4bit(x, packed, scales, offsets, inputs, outputs, group_size, _forward_activation(activation))
+
+
+def gather_matmul_4bit(x, indices, bins, top_k, packed, scales, offsets, inputs, outputs, group_size, activation=None):
+    """act(x[indices // top_k] @ w of the expert), a row for each sorted slot (stk_gather_matmul_4bit)."""
+    return _lib.native().gather_matmul_4bit(x, indices, bins, top_k, packed, scales, offsets, inputs, outputs, group_size, _forward_activation(activation))
+
+
+def matmul_4bit_scatter(x, indices, bins, top_k, packed, scales, offsets, inputs, outputs, group_size, weights=None):
+    """The tokens' weighted sums of x @ w of the expert (stk_matmul_4bit_scatter)."""
+    return _lib.native().matmul_4bit_scatter(x, indices, bins, top_k, packed, scales, offsets, inputs, outputs, group_size, weights)
+
+
+def _forward_activation(activation):
+    if activation not in ACTIVATIONS or ACTIVATIONS[activation] > ACTIVATIONS["silu"]:
+        raise ValueError(f"unknown activation {activation!r}; one of {sorted(k for k, v in ACTIVATIONS.items() if k and v <= ACTIVATIONS['silu'])}")
+    return ACTIVATIONS[activation]

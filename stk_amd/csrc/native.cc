@@ -603,6 +603,247 @@ OptTensor dsd_scatter_few(int64_t m, int64_t k, const Tensor& data, const Tensor
   return out;
 }
 
+// ------------------------------------------------------------------------------------------------ layer norm
+// x [..., size] as rows of `size` values at one distance from each other: in place where the leading dimensions allow that,
+// copied to row-major otherwise.
+struct Rows {
+  Tensor t;
+  int64_t rows, size, stride;
+  explicit Rows(const Tensor& x) : t(x.detach()), rows(1), size(x.size(-1)), stride(0) {
+    for (int64_t d = 0; d < t.dim() - 1; d++) rows *= t.size(d);
+    bool in_place = size <= 1 || t.stride(-1) == 1;
+    stride = size;
+    int64_t step = -1, inside = 1;   // the distance between rows, and the rows spanned by the dimensions behind d
+    for (int64_t d = t.dim() - 2; d >= 0 && in_place; d--) {
+      if (t.size(d) == 1) continue;
+      if (step < 0) step = t.stride(d);
+      else in_place = t.stride(d) == step * inside;
+      inside *= t.size(d);
+    }
+    if (step >= 0) stride = step;
+    if (rows > 0 && !in_place) t = t.contiguous(), stride = size;
+  }
+};
+// A parameter of a layer norm: one value per feature, of the rows' type or float32.
+OptTensor norm_parameter(const OptTensor& p_, const Tensor& x, const char* what) {
+  if (!p_) return {};
+  need_gpu(*p_);
+  const OptTensor p = p_->detach().contiguous();
+  require(p->dim() == 1 && p->numel() == x.size(-1), "layer_norm: weight and bias have one value per feature");
+  require(p->device() == x.device(), "layer_norm: the rows and their parameters are on one device");
+  if (p->scalar_type() != x.scalar_type() && p->scalar_type() != at::kFloat)
+    raise(PyExc_NotImplementedError, std::string("stk_amd: layer_norm's ") + what + " has the rows' type or float32, got " + c10::toString(p->scalar_type()));
+  return p;
+}
+int norm_parameter_dtype(const OptTensor& weight, const OptTensor& bias, const Tensor& x) {
+  require(!weight || !bias || weight->scalar_type() == bias->scalar_type(), "layer_norm: weight and bias have one type");
+  return weight ? value_dtype(*weight) : bias ? value_dtype(*bias) : value_dtype(x);
+}
+// The result and, with_statistics, mean and 1 / deviation of the rows.
+std::tuple<Tensor, OptTensor> layer_norm(const Tensor& x_, const OptTensor& weight_, const OptTensor& bias_, double eps, bool with_statistics) {
+  need_gpu(x_);
+  require(x_.dim() >= 1 && x_.size(-1) >= 1, "layer_norm: rows of at least one value");
+  value_dtype(x_);
+  const c10::DeviceGuard guard(x_.device());
+  const OptTensor weight = norm_parameter(weight_, x_, "weight"), bias = norm_parameter(bias_, x_, "bias");
+  const int param = norm_parameter_dtype(weight, bias, x_);
+  const Rows x(x_);
+  Tensor out = at::empty(x_.sizes(), x_.options());
+  OptTensor statistics;
+  if (with_statistics) statistics = at::empty({2, x.rows}, x_.options().dtype(at::kFloat));
+  float* mean = ptr<float>(statistics);
+  check(stk_layer_norm(ptr<void>(x.t), x.rows, x.size, x.stride, ptr<void>(weight), ptr<void>(bias), (float)eps, ptr<void>(out), x.size, mean,
+                       mean ? mean + x.rows : nullptr, value_dtype(x_), param, stream_of(x_)));
+  return {out, statistics};
+}
+// The gradients that are asked for.
+std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_backward(const Tensor& grad_, const Tensor& x_, const Tensor& statistics, const OptTensor& weight_,
+                                                                const OptTensor& bias_, bool want_x, bool want_weight, bool want_bias) {
+  need_gpu(grad_), need_gpu(x_);
+  require(grad_.sizes() == x_.sizes() && grad_.scalar_type() == x_.scalar_type(), "layer_norm: the gradient is laid out like the result");
+  const c10::DeviceGuard guard(x_.device());
+  const OptTensor weight = norm_parameter(weight_, x_, "weight"), bias = norm_parameter(bias_, x_, "bias");
+  const int param = norm_parameter_dtype(weight, bias, x_);
+  const Rows x(x_), grad(grad_);
+  OptTensor dx, dweight, dbias, workspace;
+  if (want_x) dx = at::empty(x_.sizes(), x_.options());
+  if (want_weight && weight) dweight = at::empty_like(*weight);
+  if (want_bias && bias) dbias = at::empty_like(*bias);
+  size_t bytes = 0;
+  if (dweight || dbias) {
+    bytes = stk_layer_norm_backward_workspace_bytes(x.rows, x.size);
+    workspace = at::empty({(int64_t)bytes}, x_.options().dtype(at::kByte));
+  }
+  check(stk_layer_norm_backward(ptr<void>(grad.t), grad.stride, ptr<void>(x.t), x.stride, ptr<float>(statistics), ptr<float>(statistics) + x.rows, ptr<void>(weight),
+                                x.rows, x.size, ptr<void>(dx), x.size, ptr<void>(dweight), ptr<void>(dbias), value_dtype(x_), param, ptr<void>(workspace), bytes,
+                                stream_of(x_)));
+  return {dx, dweight, dbias};
+}
+
+// ------------------------------------------------------------------------------------------------ router
+// Scores as rows: one dimension of tokens in front of that of the experts.
+Tensor score_rows(const Tensor& scores) {
+  require(scores.dim() == 2, "top_experts: scores are [tokens, experts]");
+  const Tensor s = scores.detach();
+  return s.size(1) <= 1 || s.stride(1) == 1 ? s : s.contiguous();
+}
+// chosen and weights
+std::tuple<Tensor, Tensor> top_experts(const Tensor& scores_, int64_t top_k, bool normalize) {
+  need_gpu(scores_);
+  const int dtype = value_dtype(scores_);
+  const c10::DeviceGuard guard(scores_.device());
+  const Tensor scores = score_rows(scores_);
+  const int64_t tokens = scores.size(0), experts = scores.size(1);
+  require(top_k >= 1 && top_k <= experts, "top_experts: top_k of 1 up to the number of experts");
+  Tensor chosen = at::empty({tokens, top_k}, scores.options().dtype(at::kInt)), weights = at::empty({tokens, top_k}, scores.options().dtype(at::kFloat));
+  check(stk_top_experts(ptr<void>(scores), tokens, experts, scores.stride(0), (int)std::min<int64_t>(top_k, INT32_MAX), normalize, ptr<int32_t>(chosen),
+                        ptr<float>(weights), dtype, stream_of(scores)));
+  return {chosen, weights};
+}
+Tensor top_experts_backward(const Tensor& scores_, const Tensor& chosen, const Tensor& weights, const Tensor& grad_, bool normalize) {
+  need_gpu(grad_);
+  const c10::DeviceGuard guard(scores_.device());
+  const Tensor scores = score_rows(scores_), grad = grad_.detach().to(at::kFloat).contiguous();
+  require(grad.sizes() == weights.sizes(), "top_experts: one gradient per weight");
+  Tensor out = at::empty(scores.sizes(), scores.options());
+  check(stk_top_experts_backward(ptr<void>(scores), scores.stride(0), ptr<int32_t>(chosen), ptr<float>(weights), ptr<float>(grad), scores.size(0),
+                                 scores.size(1), (int)weights.size(1), normalize, ptr<void>(out), out.size(1), value_dtype(scores), stream_of(scores)));
+  return out;
+}
+
+// ------------------------------------------------------------------------------------------------ 4-bit weights
+// codes [experts, inputs, outputs] and scales, offsets [experts, groups, outputs] of weights [experts, inputs, outputs]
+std::tuple<Tensor, Tensor, OptTensor> quantize_4bit(const Tensor& w_, int64_t group, bool with_offsets, at::ScalarType dtype) {
+  need_gpu(w_);
+  const Tensor w = w_.detach();
+  require(w.dim() == 3 && group >= 1, "quantize_4bit: weights are [inputs, outputs] or [experts, inputs, outputs], in groups of inputs");
+  const c10::DeviceGuard guard(w.device());
+  const int64_t experts = w.size(0), inputs = w.size(1), outputs = w.size(2), groups = (inputs + group - 1) / group;
+  Tensor codes = at::empty({experts, inputs, outputs}, w.options().dtype(at::kByte)), scales = at::empty({experts, groups, outputs}, w.options().dtype(dtype));
+  OptTensor offsets;
+  if (with_offsets) offsets = at::empty_like(scales);
+  check(stk_quantize_4bit(ptr<void>(w), w.stride(0), w.stride(1), w.stride(2), experts, inputs, outputs, group, ptr<uint8_t>(codes), ptr<void>(scales),
+                          ptr<void>(offsets), value_dtype(w), value_dtype(scales), stream_of(w)));
+  return {codes, scales, offsets};
+}
+// The packed codes, scales and offsets; codes [experts, inputs, outputs], scales and offsets [experts, groups, outputs].
+std::tuple<Tensor, Tensor, OptTensor> pack_4bit(const Tensor& codes_, const Tensor& scales_, int64_t group, const OptTensor& offsets_) {
+  need_gpu(codes_), need_gpu(scales_);
+  require(codes_.dim() == 3 && scales_.dim() == 3 && group >= 1, "pack_4bit: codes [experts, inputs, outputs], scales [experts, groups, outputs]");
+  if (codes_.scalar_type() != at::kByte) raise(PyExc_NotImplementedError, std::string("stk_amd: 4-bit codes are uint8, one a byte, got ") + c10::toString(codes_.scalar_type()));
+  const c10::DeviceGuard guard(codes_.device());
+  const int64_t experts = codes_.size(0), inputs = codes_.size(1), outputs = codes_.size(2), groups = (inputs + group - 1) / group;
+  require(scales_.size(0) == experts && scales_.size(1) == groups && scales_.size(2) == outputs && scales_.device() == codes_.device(),
+          "pack_4bit: one scale per group of inputs and output");
+  if (scales_.scalar_type() != at::kHalf && scales_.scalar_type() != at::kBFloat16)
+    raise(PyExc_NotImplementedError, std::string("stk_amd: 4-bit weights have scales of float16 or bfloat16, got ") + c10::toString(scales_.scalar_type()));
+  const Tensor codes = codes_.contiguous(), scales = scales_.detach().contiguous();
+  OptTensor offsets, packed_offsets;
+  if (offsets_) {
+    need_gpu(*offsets_);
+    require(offsets_->sizes() == scales.sizes() && offsets_->scalar_type() == scales.scalar_type() && offsets_->device() == scales.device(),
+            "pack_4bit: offsets are laid out like the scales");
+    offsets = offsets_->detach().contiguous();
+  }
+  const int64_t along = (inputs + 127) / 128, down = (outputs + 15) / 16;
+  Tensor packed = at::empty({experts, down, along, stk_4bit_packed_bytes(1, 1, 1)}, codes.options());
+  Tensor packed_scales = at::empty({experts, down, groups, 16}, scales.options());
+  if (offsets) packed_offsets = at::empty_like(packed_scales);
+  check(stk_pack_4bit(ptr<uint8_t>(codes), ptr<void>(scales), ptr<void>(offsets), experts, inputs, outputs, group, ptr<void>(packed), ptr<void>(packed_scales),
+                      ptr<void>(packed_offsets), stream_of(codes)));
+  return {packed, packed_scales, packed_offsets};
+}
+// Packed weights as the calls take them: what pack_4bit made, in its shapes.
+struct Packed {
+  int64_t experts, inputs, outputs, group;
+  Packed(const Tensor& packed, const Tensor& scales, const OptTensor& offsets, int64_t inputs_, int64_t outputs_, int64_t group_)
+      : experts(0), inputs(inputs_), outputs(outputs_), group(group_) {
+    need_gpu(packed), need_gpu(scales);
+    require(packed.dim() == 4 && packed.scalar_type() == at::kByte && packed.is_contiguous() && scales.is_contiguous() && inputs > 0 && outputs > 0 && group > 0,
+            "packed 4-bit weights come from pack_4bit");
+    experts = packed.size(0);
+    require(packed.numel() == stk_4bit_packed_bytes(experts, inputs, outputs) && scales.numel() == stk_4bit_scales(experts, inputs, outputs, group) &&
+                scales.device() == packed.device() &&
+                (!offsets || (offsets->numel() == scales.numel() && offsets->is_contiguous() && offsets->scalar_type() == scales.scalar_type() &&
+                              offsets->device() == packed.device())),
+            "packed 4-bit weights come from pack_4bit");
+  }
+};
+#define PACKED_ARGS const Tensor &packed, const Tensor &scales, const OptTensor &offsets, int64_t inputs, int64_t outputs, int64_t group
+Tensor dequantize_4bit(PACKED_ARGS) {
+  const Packed w(packed, scales, offsets, inputs, outputs, group);
+  const c10::DeviceGuard guard(packed.device());
+  Tensor out = at::empty({w.experts, inputs, outputs}, scales.options());
+  check(stk_dequantize_4bit(ptr<void>(packed), ptr<void>(scales), ptr<void>(offsets), w.experts, inputs, outputs, group, ptr<void>(out), value_dtype(scales),
+                            stream_of(packed)));
+  return out;
+}
+// Rows of the products: `inputs` values of the scales' type, next to each other.
+Tensor rows4(const Tensor& x_, const Tensor& scales, int64_t inputs) {
+  need_gpu(x_);
+  require(x_.dim() == 2 && x_.size(1) == inputs, "incompatible dimensions");
+  require(x_.device() == scales.device(), "operands are on one device");
+  if (x_.scalar_type() != scales.scalar_type())
+    raise(PyExc_NotImplementedError, std::string("stk_amd: rows and scales of 4-bit weights have one type, got ") + c10::toString(x_.scalar_type()) + " and " +
+                                         c10::toString(scales.scalar_type()));
+  const Tensor x = x_.detach();
+  return inputs == 1 || x.stride(1) == 1 ? x : x.contiguous();
+}
+OptTensor workspace4(size_t bytes, const Tensor& like) {
+  if (bytes == 0) return {};
+  return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+}
+Tensor matmul_4bit(const Tensor& x_, PACKED_ARGS, int activation) {
+  const Packed w(packed, scales, offsets, inputs, outputs, group);
+  require(w.experts == 1, "matmul_4bit: the weights of one matrix");
+  const c10::DeviceGuard guard(packed.device());
+  const Tensor x = rows4(x_, scales, inputs);
+  const int64_t rows = x.size(0);
+  Tensor out = at::empty({rows, outputs}, x.options());
+  const size_t bytes = stk_matmul_4bit_workspace_bytes(rows, 1, inputs, outputs);
+  const OptTensor ws = workspace4(bytes, x);
+  check(stk_matmul_4bit(ptr<void>(x), rows, x.stride(0), ptr<void>(packed), ptr<void>(scales), ptr<void>(offsets), inputs, outputs, group, ptr<void>(out), outputs,
+                        activation, value_dtype(x), ptr<void>(ws), bytes, stream_of(x)));
+  return out;
+}
+void check_routing(const Tensor& indices, const Tensor& bins, const Packed& w, const Tensor& scales) {
+  need_gpu(indices), need_gpu(bins);
+  for (const Tensor* t : {&indices, &bins})
+    require(t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == scales.device(), "the routing's arrays come from route");
+  require(bins.numel() == w.experts, "one bin for each expert's weights");
+}
+Tensor gather_matmul_4bit(const Tensor& x_, const Tensor& indices, const Tensor& bins, int top_k, PACKED_ARGS, int activation) {
+  const Packed w(packed, scales, offsets, inputs, outputs, group);
+  check_routing(indices, bins, w, scales);
+  const c10::DeviceGuard guard(packed.device());
+  const Tensor x = rows4(x_, scales, inputs);
+  const int64_t slots = indices.numel();
+  require(top_k >= 1 && x.size(0) * top_k == slots, "one row per token");
+  Tensor out = at::empty({slots, outputs}, x.options());
+  const size_t bytes = stk_matmul_4bit_workspace_bytes(slots, w.experts, inputs, outputs);
+  const OptTensor ws = workspace4(bytes, x);
+  check(stk_gather_matmul_4bit(ptr<void>(x), x.size(0), x.stride(0), ptr<int32_t>(indices), ptr<int32_t>(bins), top_k, ptr<void>(packed), ptr<void>(scales),
+                               ptr<void>(offsets), w.experts, inputs, outputs, group, ptr<void>(out), outputs, activation, value_dtype(x), ptr<void>(ws), bytes,
+                               stream_of(x)));
+  return out;
+}
+Tensor matmul_4bit_scatter(const Tensor& x_, const Tensor& indices, const Tensor& bins, int top_k, PACKED_ARGS, const OptTensor& weights) {
+  const Packed w(packed, scales, offsets, inputs, outputs, group);
+  check_routing(indices, bins, w, scales);
+  const c10::DeviceGuard guard(packed.device());
+  const Tensor x = rows4(x_, scales, inputs);
+  const int64_t slots = indices.numel();
+  require(top_k >= 1 && slots % top_k == 0 && x.size(0) == slots, "one row per slot");
+  const OptTensor by_slot = weights32(weights, slots);
+  Tensor out = at::empty({slots / top_k, outputs}, x.options());
+  const size_t bytes = stk_matmul_4bit_scatter_workspace_bytes(slots, w.experts, inputs, outputs);
+  const OptTensor ws = workspace4(bytes, x);
+  check(stk_matmul_4bit_scatter(ptr<void>(x), x.stride(0), ptr<int32_t>(indices), ptr<int32_t>(bins), top_k, slots / top_k, ptr<float>(by_slot), ptr<void>(packed),
+                                ptr<void>(scales), ptr<void>(offsets), w.experts, inputs, outputs, group, ptr<void>(out), outputs, value_dtype(x), ptr<void>(ws), bytes,
+                                stream_of(x)));
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -631,4 +872,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dsd_scatter_few_case", &dsd_scatter_few_case);
   m.def("dsd_scatter_few", &dsd_scatter_few, py::call_guard<py::gil_scoped_release>());
   m.def("dsd_scatter", &dsd_scatter, py::call_guard<py::gil_scoped_release>());
+  m.def("layer_norm", &layer_norm, py::call_guard<py::gil_scoped_release>());
+  m.def("layer_norm_backward", &layer_norm_backward, py::call_guard<py::gil_scoped_release>());
+  m.def("top_experts", &top_experts, py::call_guard<py::gil_scoped_release>());
+  m.def("top_experts_backward", &top_experts_backward, py::call_guard<py::gil_scoped_release>());
+  m.def("quantize_4bit", &quantize_4bit, py::call_guard<py::gil_scoped_release>());
+  m.def("pack_4bit", &pack_4bit, py::call_guard<py::gil_scoped_release>());
+  m.def("dequantize_4bit", &dequantize_4bit, py::call_guard<py::gil_scoped_release>());
+  m.def("matmul_4bit", &matmul_4bit, py::call_guard<py::gil_scoped_release>());
+  m.def("gather_matmul_4bit", &gather_matmul_4bit, py::call_guard<py::gil_scoped_release>());
+  m.def("matmul_4bit_scatter", &matmul_4bit_scatter, py::call_guard<py::gil_scoped_release>());
 }

@@ -1,0 +1,27 @@
+// Weights of 4 bits and a scale (and offset) for every group of inputs, as stk_pack_4bit lays them out.
+//
+// A piece is 16 outputs x 128 inputs, 1024 bytes, the A operand of four v_mfma_f32_16x16x32: lane l of a wavefront finds its 32
+// codes - output l % 16, of every 32 inputs the eight from 8 (l / 16) on - in the 16 bytes from 16 l on, one dword for each step of
+// 32 inputs.  Bits [4p, 4p + 4) of a dword are the code of input 2p of the eight, the same bits 16 higher that of input 2p + 1, so that
+// one shift and one and-or make a pair of 16-bit values of each.  Pieces follow each other along the inputs, then along the outputs, then
+// expert by expert.  Scales (16-bit): [expert][16 outputs][group][16], so that the four outputs a lane accumulates are 8 bytes.
+// Inputs beyond the last hold code 8, outputs beyond the last scale 0.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace stk {
+
+constexpr int kPieceInputs = 128, kPieceOutputs = 16, kPieceBytes = 1024;
+
+__host__ __device__ inline int64_t pieces_in(int64_t inputs) { return (inputs + kPieceInputs - 1) / kPieceInputs; }
+__host__ __device__ inline int64_t pieces_out(int64_t outputs) { return (outputs + kPieceOutputs - 1) / kPieceOutputs; }
+__host__ __device__ inline int64_t groups_of(int64_t inputs, int64_t group) { return (inputs + group - 1) / group; }
+
+// Byte of a piece and shift in it where the code of output o % 16 and input i % 128 is.
+__host__ __device__ inline void code_at(int o, int i, int* byte, int* shift) {
+  const int lane = (o & 15) + 16 * ((i >> 3) & 3), dword = (i >> 5) & 3, j = i & 7, bit = 4 * (j >> 1) + 16 * (j & 1);
+  *byte = 16 * lane + 4 * dword + bit / 8, *shift = bit % 8;
+}
+
+}  // namespace stk

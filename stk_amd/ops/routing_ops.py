@@ -7,6 +7,7 @@ and the two copies are HIP kernels; `Route.padded_bins` feeds stk.ops.dmoe_topol
 from collections import namedtuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from stk_amd.backend import autocast, hip_kernels
 from stk_amd.backend.autograd import applies
@@ -35,6 +36,36 @@ def route(top_experts, num_experts, blocking, padded_rows=None):
 def route_capacity(slots, num_experts, blocking):
     """Largest padded layout `slots` slots over `num_experts` experts can need (a multiple of blocking)."""
     return (slots + num_experts * (blocking - 1)) // blocking * blocking
+
+
+class _TopExperts(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, scores, top_k, normalize):
+        chosen, weights = hip_kernels.top_experts(scores, top_k, normalize)
+        ctx.save_for_backward(scores, chosen, weights)
+        ctx.normalize = normalize
+        ctx.mark_non_differentiable(chosen)
+        return chosen, weights
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _, grad):
+        scores, chosen, weights = ctx.saved_tensors
+        return hip_kernels.top_experts_backward(scores, chosen, weights, grad, ctx.normalize), None, None
+
+
+def top_experts(scores, top_k, normalize=False):
+    """A router's choice given scores [tokens, experts] on the GPU: (experts, weights), both [tokens, top_k].
+
+    experts  int32, the top_k experts of the highest scores in descending order, ties to the lower number: what route takes
+    weights  fp32, their softmax over all experts, or with normalize over the chosen ones: what padded_scatter takes;
+             differentiable with respect to the scores
+
+    scores float16, bfloat16 or float32, at most 1024 experts, the top 64.  A score of -infinity masks an expert (its weight is 0, in a
+    row of nothing else every weight is); a NaN or +infinity makes the weights of its row NaN."""
+    if not applies(scores):
+        return hip_kernels.top_experts(scores, top_k, normalize)
+    return _TopExperts.apply(scores, top_k, normalize)
 
 
 class _PaddedGather(torch.autograd.Function):
