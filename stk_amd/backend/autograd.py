@@ -147,6 +147,12 @@ def applies(*tensors):
     return _wants_grad(*tensors) or forward_ad._current_level >= 0 or _transforms_active() or _is_tracing()
 
 
+def seen_by_python_only():
+    """Whether only a function of torch's Python interface will do: for the cases above in which nothing needs a gradient.  Functions
+    of the native boundary (csrc/native.cc) stand in the graph like these, at a third of the host time, but are not recorded."""
+    return forward_ad._current_level >= 0 or _transforms_active() or _is_tracing()
+
+
 class DSD(torch.autograd.Function):
 
     @staticmethod

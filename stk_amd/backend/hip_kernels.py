@@ -509,6 +509,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, with_statistics=False):
     return _lib.native().layer_norm(x, weight, bias, eps, with_statistics)
 
 
+def layer_norm_graph(x, weight=None, bias=None, eps=1e-5):
+    """The result of layer_norm, in torch's graph where a gradient is wanted."""
+    return _lib.native().layer_norm_graph(x, weight, bias, eps)
+
+
 def layer_norm_backward(grad, x, statistics, weight, bias, want_x=True, want_weight=True, want_bias=True):
     """(dx, dweight, dbias) of stk_layer_norm_backward, None for what is not asked for or has no parameter."""
     return _lib.native().layer_norm_backward(grad, x, statistics, weight, bias, want_x, want_weight, want_bias)
@@ -517,6 +522,11 @@ def layer_norm_backward(grad, x, statistics, weight, bias, want_x=True, want_wei
 def top_experts(scores, top_k, normalize=False):
     """(chosen int32, weights fp32) of stk_top_experts."""
     return _lib.native().top_experts(scores, top_k, normalize)
+
+
+def top_experts_graph(scores, top_k, normalize=False):
+    """The results of top_experts, in torch's graph where a gradient is wanted."""
+    return _lib.native().top_experts_graph(scores, top_k, normalize)
 
 
 def top_experts_backward(scores, chosen, weights, grad, normalize=False):

@@ -7,6 +7,8 @@
 // state is kept between calls but one pinned word per host thread and device (Mailbox).
 #include <torch/extension.h>
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 
@@ -680,6 +682,42 @@ std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_backward(const Tensor& gr
   return {dx, dweight, dbias};
 }
 
+// Outputs of a backward pass that has no gradient of its own: asked for with create_graph they say so when they are differentiated.
+torch::autograd::variable_list once_differentiable(torch::autograd::variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::variable_list inputs;
+  for (const Tensor& t : grads) inputs.push_back(t.defined() ? t.detach().requires_grad_(true) : t);
+  const auto error = std::make_shared<torch::autograd::DelayedError>(std::string("stk_amd: ") + what + " can be differentiated once", (int64_t)inputs.size());
+  return error->apply(std::move(inputs));
+}
+
+// Autograd in native code: through a Python function a forward and backward pass cost 30 us more on the host than these, longer than
+// the kernels of a layer norm of 16384 x 1024 values take.
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+    auto [out, statistics] = layer_norm(x, weight, bias, eps, true);
+    ctx->save_for_backward({x, weight ? *weight : Tensor(), bias ? *bias : Tensor(), *statistics});
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto given = [&](size_t i) { return saved[i].defined() ? OptTensor(saved[i]) : OptTensor(); };
+    // (parameters that are not there have no edge)
+    size_t edge = 0;
+    const bool want_x = ctx->needs_input_grad(edge++), want_weight = saved[1].defined() && ctx->needs_input_grad(edge++);
+    const bool want_bias = saved[2].defined() && ctx->needs_input_grad(edge++);
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto [dx, dweight, dbias] = layer_norm_backward(grads[0], saved[0], saved[3], given(1), given(2), want_x, want_weight, want_bias);
+    return once_differentiable({dx.value_or(Tensor()), dweight.value_or(Tensor()), dbias.value_or(Tensor()), Tensor()}, "layer_norm");
+  }
+};
+bool wants_gradient(const OptTensor& t) { return t && t->requires_grad(); }
+// layer_norm with its place in the graph where a gradient is wanted.
+Tensor layer_norm_graph(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  if (at::GradMode::is_enabled() && (x.requires_grad() || wants_gradient(weight) || wants_gradient(bias))) return LayerNorm::apply(x, weight, bias, eps);
+  return std::get<0>(layer_norm(x, weight, bias, eps, false));
+}
+
 // ------------------------------------------------------------------------------------------------ router
 // Scores as rows: one dimension of tokens in front of that of the experts.
 Tensor score_rows(const Tensor& scores) {
@@ -709,6 +747,26 @@ Tensor top_experts_backward(const Tensor& scores_, const Tensor& chosen, const T
   check(stk_top_experts_backward(ptr<void>(scores), scores.stride(0), ptr<int32_t>(chosen), ptr<float>(weights), ptr<float>(grad), scores.size(0),
                                  scores.size(1), (int)weights.size(1), normalize, ptr<void>(out), out.size(1), value_dtype(scores), stream_of(scores)));
   return out;
+}
+
+struct TopExperts : torch::autograd::Function<TopExperts> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& scores, int64_t top_k, bool normalize) {
+    auto [chosen, weights] = top_experts(scores, top_k, normalize);
+    ctx->save_for_backward({scores, chosen, weights});
+    ctx->saved_data["normalize"] = normalize;
+    ctx->mark_non_differentiable({chosen});
+    return {chosen, weights};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    if (!grads[1].defined()) return {Tensor(), Tensor(), Tensor()};
+    return once_differentiable({top_experts_backward(saved[0], saved[1], saved[2], grads[1], ctx->saved_data["normalize"].toBool()), Tensor(), Tensor()}, "top_experts");
+  }
+};
+std::tuple<Tensor, Tensor> top_experts_graph(const Tensor& scores, int64_t top_k, bool normalize) {
+  if (!at::GradMode::is_enabled() || !scores.requires_grad()) return top_experts(scores, top_k, normalize);
+  const auto out = TopExperts::apply(scores, top_k, normalize);
+  return {out[0], out[1]};
 }
 
 // ------------------------------------------------------------------------------------------------ 4-bit weights
@@ -873,8 +931,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dsd_scatter_few", &dsd_scatter_few, py::call_guard<py::gil_scoped_release>());
   m.def("dsd_scatter", &dsd_scatter, py::call_guard<py::gil_scoped_release>());
   m.def("layer_norm", &layer_norm, py::call_guard<py::gil_scoped_release>());
+  m.def("layer_norm_graph", &layer_norm_graph, py::call_guard<py::gil_scoped_release>());
   m.def("layer_norm_backward", &layer_norm_backward, py::call_guard<py::gil_scoped_release>());
   m.def("top_experts", &top_experts, py::call_guard<py::gil_scoped_release>());
+  m.def("top_experts_graph", &top_experts_graph, py::call_guard<py::gil_scoped_release>());
   m.def("top_experts_backward", &top_experts_backward, py::call_guard<py::gil_scoped_release>());
   m.def("quantize_4bit", &quantize_4bit, py::call_guard<py::gil_scoped_release>());
   m.def("pack_4bit", &pack_4bit, py::call_guard<py::gil_scoped_release>());

@@ -4,10 +4,12 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from stk_amd.backend import hip_kernels
-from stk_amd.backend.autograd import applies
+from stk_amd.backend.autograd import seen_by_python_only
 
 
 class _LayerNorm(torch.autograd.Function):
+    """What forward-mode differentiation and transforms refuse and torch.jit.trace records; otherwise the native function runs."""
+
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         out, statistics = hip_kernels.layer_norm(x, weight, bias, eps, with_statistics=True)
@@ -28,6 +30,6 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     are fp32 and every result is rounded once, to the type of what it belongs to.  The gradients of x, weight and bias
     have the same bits every time.  x may have any strides (rows that are not one distance apart, or whose values are not next to each
     other, are copied first); the result is contiguous."""
-    if not applies(x, weight, bias):
-        return hip_kernels.layer_norm(x, weight, bias, eps)[0]
-    return _LayerNorm.apply(x, weight, bias, eps)
+    if seen_by_python_only():
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return hip_kernels.layer_norm_graph(x, weight, bias, eps)

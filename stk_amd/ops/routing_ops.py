@@ -10,7 +10,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from stk_amd.backend import autocast, hip_kernels
-from stk_amd.backend.autograd import applies
+from stk_amd.backend.autograd import applies, seen_by_python_only
 from stk_amd.matrix import Matrix
 
 Route = namedtuple("Route", "indices bin_ids bins padded_bins slot_rows row_slots top_k blocking")
@@ -39,6 +39,8 @@ def route_capacity(slots, num_experts, blocking):
 
 
 class _TopExperts(torch.autograd.Function):
+    """What forward-mode differentiation and transforms refuse and torch.jit.trace records; otherwise the native function runs."""
+
     @staticmethod
     def forward(ctx, scores, top_k, normalize):
         chosen, weights = hip_kernels.top_experts(scores, top_k, normalize)
@@ -63,9 +65,9 @@ def top_experts(scores, top_k, normalize=False):
 
     scores float16, bfloat16 or float32, at most 1024 experts, the top 64.  A score of -infinity masks an expert (its weight is 0, in a
     row of nothing else every weight is); a NaN or +infinity makes the weights of its row NaN."""
-    if not applies(scores):
-        return hip_kernels.top_experts(scores, top_k, normalize)
-    return _TopExperts.apply(scores, top_k, normalize)
+    if seen_by_python_only():
+        return _TopExperts.apply(scores, top_k, normalize)
+    return hip_kernels.top_experts_graph(scores, top_k, normalize)
 
 
 class _PaddedGather(torch.autograd.Function):

@@ -266,3 +266,10 @@ def test_statistics_are_those_of_the_rows():
     _, _, r = L.layer_norm(U.np32(x))
     np.testing.assert_allclose(_n64(statistics[0]), U.np32(x).astype(np.float64).mean(axis=1), rtol=0, atol=20 * 2.0 ** -24 * float(x.float().abs().max()))
     np.testing.assert_allclose(_n64(statistics[1]), r[:, 0], rtol=40 * 2.0 ** -24)
+
+
+def test_a_traced_call_computes_its_result_again():
+    x, w, b, _ = (t.to(DEV) for t in _inputs(5, 64, torch.float32, torch.float32, 18))
+    traced = torch.jit.trace(lambda v: stk.ops.layer_norm(v, w, b), (x,), check_trace=False)
+    other = x.flip(0) * 2
+    assert torch.equal(traced(other), stk.ops.layer_norm(other, w, b))

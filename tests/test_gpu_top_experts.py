@@ -194,3 +194,9 @@ def test_refusals():
         first.sum().backward()
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda s: stk.ops.top_experts(s, 2)[1])(x.view(2, 2, 8))
+
+
+def test_a_traced_call_computes_its_result_again():
+    x = torch.randn(6, 12, generator=torch.Generator().manual_seed(1)).to(DEV)
+    traced = torch.jit.trace(lambda v: stk.ops.top_experts(v, 2)[1], (x,), check_trace=False)
+    assert torch.equal(traced(x.flip(0)), stk.ops.top_experts(x.flip(0), 2)[1])
