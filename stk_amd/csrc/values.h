@@ -30,6 +30,7 @@ template <> struct Value<STK_F32> {
 typedef uint32_t Quad __attribute__((ext_vector_type(4)));
 typedef uint32_t QuadAt2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t QuadAt4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t PairAt2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef float Pair __attribute__((ext_vector_type(2)));
 typedef _Float16 HalfPair __attribute__((ext_vector_type(2)));
 template <int DTYPE> struct Eight { Quad q[DTYPE == STK_F32 ? 2 : 1]; };

@@ -5,6 +5,7 @@
 #include "common.h"
 #include "gemm_core.h"
 #include "values.h"
+#include "wave_scan.h"
 #include "weights4.h"
 
 namespace stk {
@@ -117,47 +118,260 @@ struct Product4 {
   int activation;
 };
 
-__device__ __forceinline__ int expert_of(const int32_t* bins, int experts, int64_t row) {
-  int lo = 0, hi = experts - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (bins[mid] > row) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
+// ---------------------------------------------------------------- products
+// A code becomes the 16-bit number 16 + code: its four bits at the top of the mantissa of a number between 16 and 32.  A group's
+// products are then sums over x (16 + code), and the sums over x that are too much, -24 x (the code's zero at 8) or -16 x (with
+// offsets), are what the accumulator starts from: a product of x with a constant operand, shared by all outputs.  The group's scale
+// multiplies the fp32 sum.  That makes 8 instructions for eight weights and one for a group's four outputs, below half of
+// what a stream of weights at memory speed leaves time for.
+template <bool BF16> struct Codes;
+template <> struct Codes<true> {
+  static constexpr uint32_t mask = 0x00780078u, magic = 0x41804180u, minus24 = 0xc1c0c1c0u, minus16 = 0xc180c180u;
+  static __device__ __forceinline__ uint32_t placed(uint32_t w, int p) { return p == 0 ? w << 3 : w >> (4 * p - 3); }
+};
+template <> struct Codes<false> {
+  static constexpr uint32_t mask = 0x03c003c0u, magic = 0x4c004c00u, minus24 = 0xce00ce00u, minus16 = 0xcc00cc00u;
+  static __device__ __forceinline__ uint32_t placed(uint32_t w, int p) { return p == 0 ? w << 6 : p == 1 ? w << 2 : w >> (4 * p - 6); }
+};
+template <bool BF16>
+__device__ __forceinline__ u32x4 numbers(uint32_t w) {
+  typedef Codes<BF16> C;
+  u32x4 v;
+#pragma unroll
+  for (int p = 0; p < 4; p++) v[p] = (C::placed(w, p) & C::mask) | C::magic;
+  return v;
+}
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+template <bool BF16>
+__device__ __forceinline__ f32x4_t mfma_16x16x32(u32x4 a, u32x4 b, f32x4_t c) {
+  if constexpr (BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// A thread per row and output.
-template <int DTYPE>
-__global__ __launch_bounds__(256) void product_kernel(Product4 p) {
-  typedef typename Value<DTYPE>::stored T;
-  const int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (o >= p.outputs) return;
-  for (int64_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
-    const int64_t slot = p.indices ? p.indices[row] : row, e = p.bins ? expert_of(p.bins, (int)p.experts, row) : 0;
-    if (slot < 0 || slot >= p.rows) continue;
-    const T* x = static_cast<const T*>(p.x) + (p.top_k > 0 ? slot / p.top_k : row) * p.x_stride;
-    float sum = 0.f;
-    for (int64_t i = 0; i < p.inputs; i++)
-      sum += Value<DTYPE>::widen(x[i]) * weight_of<DTYPE>(p.packed, static_cast<const T*>(p.scales), static_cast<const T*>(p.offsets), e, i, o,
-                                                          pieces_in(p.inputs), pieces_out(p.outputs), p.group, groups_of(p.inputs, p.group));
-    if (p.sums) p.sums[slot * p.outputs + o] = sum;
-    else static_cast<T*>(p.out)[row * p.out_stride + o] = Value<DTYPE>::round(activated(sum, p.activation));
+// Which rows a tile of up to R rows of one expert is: tiles are numbered expert by expert, an expert of c rows has ceil(c / R).
+struct RowTile {
+  int expert, first, rows;   // (rows 0: no such tile)
+};
+template <int R>
+__device__ __forceinline__ RowTile row_tile(const Product4& p, int tile, int lane) {
+  if (!p.bins) {
+    const int64_t first = (int64_t)tile * R, left = p.rows - first;
+    return {0, (int)first, left <= 0 ? 0 : left < R ? (int)left : R};
+  }
+  int before = 0;
+  for (int e0 = 0; e0 < p.experts; e0 += kWave) {
+    const int e = e0 + lane;
+    const bool is = e < p.experts;
+    // (bins that do not ascend or leave the rows are kept inside them)
+    const int hi = is ? min(max(p.bins[e], 0), (int)p.rows) : 0, lo = is && e > 0 ? min(max(p.bins[e - 1], 0), (int)p.rows) : 0;
+    const int count = hi > lo ? hi - lo : 0, tiles = (count + R - 1) / R, upto = before + wave_inclusive_scan(tiles, lane);
+    const uint64_t mine = __ballot(upto > tile);
+    if (mine) {
+      const int at = __builtin_ctzll(mine);
+      const int inside = tile - __builtin_amdgcn_readlane(upto - tiles, at), c = __builtin_amdgcn_readlane(count, at);
+      return {e0 + at, __builtin_amdgcn_readlane(lo, at) + inside * R, min(c - inside * R, R)};
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return {0, 0, 0};
+}
+
+// Eight values of a row from input i on, zeros beyond the last input.
+__device__ __forceinline__ u32x4 row_values(const uint16_t* row, int i, int inputs) {
+  if (i + 8 <= inputs) return __builtin_bit_cast(u32x4, *reinterpret_cast<const QuadAt2*>(row + i));
+  u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const uint32_t one = i + j < inputs ? row[i + j] : 0u;
+    v[j / 2] |= one << (16 * (j & 1));
+  }
+  return v;
+}
+
+// KW wavefronts share the inputs of NW x NT x 16 outputs and 16 MT rows of one expert, a piece of weights at a time; their sums meet
+// in LDS.  SUB: groups of a piece whose sums are scaled apart (1, or 4: groups of 32 or 64).
+template <bool BF16, bool AFFINE, int SUB, int KW, int NW, int NT, int MT>
+__global__ __launch_bounds__(64 * KW * NW) void stream_kernel(Product4 p) {
+  constexpr int kAtOnce = NT * MT == 1 ? 4 : NT * MT == 2 ? 2 : 1;   // pieces whose loads are in flight together
+  extern __shared__ f32x4_t shared[];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), kw = wave % KW, nw = wave / KW;
+  const RowTile t = row_tile<16 * MT>(p, blockIdx.y, lane);
+  if (t.rows == 0) return;
+  const int along = (int)pieces_in(p.inputs), down = (int)pieces_out(p.outputs), groups = (int)groups_of(p.inputs, p.group);
+  const int row = lane & 15, quarter = lane >> 4;
+  const uint16_t* x[MT];
+  bool has[MT];
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    const int r = 16 * m + row;
+    has[m] = r < t.rows;
+    int64_t from = t.first + (has[m] ? r : 0);
+    if (p.top_k > 0) {
+      const int slot = p.indices[from];
+      has[m] = has[m] && (unsigned)slot < (unsigned)p.rows;
+      from = has[m] ? slot / p.top_k : 0;
+    }
+    x[m] = static_cast<const uint16_t*>(p.x) + from * p.x_stride;
+  }
+  int tile[NT];   // (the last tiles of a workgroup may lie beyond the outputs: computed again and not stored)
+  const u32x4* weights[NT];
+  const uint16_t *scales[NT], *offsets[NT];
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    tile[n] = ((int)blockIdx.x * NW + nw) * NT + n;
+    const int64_t at = (int64_t)t.expert * down + min(tile[n], down - 1);
+    weights[n] = reinterpret_cast<const u32x4*>(p.packed + at * along * kPieceBytes) + lane;
+    scales[n] = static_cast<const uint16_t*>(p.scales) + at * groups * 16 + 4 * quarter;
+    offsets[n] = static_cast<const uint16_t*>(p.offsets) + at * groups * 16 + 4 * quarter;
+  }
+  const int share = (along + KW - 1) / KW, begin = min(kw * share, along), end = min(begin + share, along);
+  const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+  f32x4_t total[NT][MT];
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int m = 0; m < MT; m++) total[n][m] = zero;
+  constexpr uint32_t minus = AFFINE ? Codes<BF16>::minus16 : Codes<BF16>::minus24;
+  const u32x4 constant = {minus, minus, minus, minus};
+  const int per_group = (int)(p.group / kPieceInputs), steps = (int)(p.group / 32);   // pieces of a group, or steps of one
+  for (int piece = begin; piece < end; piece += kAtOnce) {
+    u32x4 w[kAtOnce][NT], v[kAtOnce][MT][4];
+    u32x2 s[kAtOnce][NT][SUB], o[kAtOnce][NT][AFFINE ? SUB : 1];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; u++) {
+      const int at = min(piece + u, end - 1);
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        w[u][n] = __builtin_nontemporal_load(weights[n] + (int64_t)at * 64);
+#pragma unroll
+        for (int g = 0; g < SUB; g++) {
+          const int group = min(SUB == 1 ? at / per_group : (4 * at + g) / steps, groups - 1);
+          s[u][n][g] = *reinterpret_cast<const u32x2*>(scales[n] + group * 16);
+          if constexpr (AFFINE) o[u][n][g] = *reinterpret_cast<const u32x2*>(offsets[n] + group * 16);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int d = 0; d < 4; d++) {
+          v[u][m][d] = u32x4{0u, 0u, 0u, 0u};
+          if (has[m] && piece + u < end) v[u][m][d] = row_values(x[m], at * kPieceInputs + 32 * d + 8 * quarter, (int)p.inputs);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; u++)
+#pragma unroll
+      for (int g = 0; g < SUB; g++) {
+        f32x4_t start[MT];
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+          start[m] = zero;
+#pragma unroll
+          for (int d = 4 / SUB * g; d < 4 / SUB * (g + 1); d++) start[m] = mfma_16x16x32<BF16>(constant, v[u][m][d], start[m]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const f32x2_t s0 = unpack2<BF16>(s[u][n][g].x), s1 = unpack2<BF16>(s[u][n][g].y);
+          const f32x4_t scale = {s0.x, s0.y, s1.x, s1.y};
+          f32x4_t sum[MT];
+#pragma unroll
+          for (int m = 0; m < MT; m++) sum[m] = start[m];
+#pragma unroll
+          for (int d = 4 / SUB * g; d < 4 / SUB * (g + 1); d++) {
+            const u32x4 a = numbers<BF16>(w[u][n][d]);
+#pragma unroll
+            for (int m = 0; m < MT; m++) sum[m] = mfma_16x16x32<BF16>(a, v[u][m][d], sum[m]);
+          }
+#pragma unroll
+          for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) total[n][m][i] = fmaf(scale[i], sum[m][i], total[n][m][i]);
+          if constexpr (AFFINE) {
+            const f32x2_t o0 = unpack2<BF16>(o[u][n][g].x), o1 = unpack2<BF16>(o[u][n][g].y);
+            const f32x4_t offset = {o0.x, o0.y, o1.x, o1.y};
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) total[n][m][i] = fmaf(offset[i], start[m][i] * -0.0625f, total[n][m][i]);   // start = -16 sum(x)
+          }
+        }
+      }
+  }
+  if constexpr (KW > 1) {
+    if (kw > 0) {
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int m = 0; m < MT; m++) shared[(((kw - 1) * NW + nw) * NT * MT + n * MT + m) * 64 + lane] = total[n][m];
+    }
+    __syncthreads();
+    if (kw > 0) return;
+    for (int k = 0; k < KW - 1; k++)
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int m = 0; m < MT; m++) total[n][m] += shared[((k * NW + nw) * NT * MT + n * MT + m) * 64 + lane];
+  }
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    if (16 * m + row >= t.rows) continue;
+    int64_t to = t.first + 16 * m + row;
+    if (p.sums) {
+      to = p.indices[to];
+      if (to < 0 || to >= p.rows) continue;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      const int64_t first = (int64_t)tile[n] * 16 + 4 * quarter;
+      if (first >= p.outputs) continue;
+      const int here = (int)min(p.outputs - first, (int64_t)4);
+      if (p.sums) {
+        float* at = p.sums + to * p.outputs + first;
+        if (here == 4) *reinterpret_cast<QuadAt4*>(at) = __builtin_bit_cast(Quad, total[n][m]);
+        else
+          for (int i = 0; i < here; i++) at[i] = total[n][m][i];
+        continue;
+      }
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) y[i] = activated(total[n][m][i], p.activation);
+      const uint32_t two[2] = {pack2<BF16>(y[0], y[1]), pack2<BF16>(y[2], y[3])};
+      uint16_t* at = static_cast<uint16_t*>(p.out) + to * p.out_stride + first;
+      if (here == 4) *reinterpret_cast<PairAt2*>(at) = PairAt2{two[0], two[1]};
+      else
+        for (int i = 0; i < here; i++) at[i] = (uint16_t)(two[i / 2] >> (16 * (i & 1)));
+    }
   }
 }
 
-// out[t] = sum over the choices j of a token, in their order, of (weights[s]) sums[s], s = t top_k + j; rounded once.
-template <int DTYPE>
+// out[t] = sum over the choices j of a token, in their order, of (weights[s]) sums[s], s = t top_k + j; rounded once.  A thread per
+// token and four outputs.
+template <bool BF16>
 __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ sums, const float* __restrict__ weights, int64_t tokens, int top_k,
-                                                      int64_t outputs, typename Value<DTYPE>::stored* __restrict__ out, int64_t out_stride) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, t = at / outputs, o = at % outputs;
-  if (t >= tokens) return;
-  float v = 0.f;
-  for (int j = 0; j < top_k; j++) {
-    const int64_t s = t * top_k + j;
-    v += weights ? weights[s] * sums[s * outputs + o] : sums[s * outputs + o];
+                                                      int64_t outputs, uint16_t* __restrict__ out, int64_t out_stride) {
+  const int64_t across = (outputs + 3) / 4, step = (int64_t)gridDim.x * 256;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < tokens * across; at += step) {
+    const int64_t t = at / across, o = at % across * 4;
+    const int here = (int)min(outputs - o, (int64_t)4);
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < top_k; j++) {
+      const int64_t s = t * top_k + j;
+      const float by = weights ? weights[s] : 1.f;
+      const float* from = sums + s * outputs + o;
+      if (here == 4) {
+        const f32x4_t u = __builtin_bit_cast(f32x4_t, *reinterpret_cast<const QuadAt4*>(from));
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = fmaf(by, u[i], v[i]);
+      } else {
+        for (int i = 0; i < here; i++) v[i] = fmaf(by, from[i], v[i]);
+      }
+    }
+    const uint32_t two[2] = {pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3])};
+    uint16_t* to = out + t * out_stride + o;
+    if (here == 4) *reinterpret_cast<PairAt2*>(to) = PairAt2{two[0], two[1]};
+    else
+      for (int i = 0; i < here; i++) to[i] = (uint16_t)(two[i / 2] >> (16 * (i & 1)));
   }
-  out[t * out_stride + o] = Value<DTYPE>::round(v);
 }
 
 static int weights_check(const char* who, int64_t experts, int64_t inputs, int64_t outputs, int64_t group, int dtype) {
@@ -181,10 +395,42 @@ static int product_check(const char* who, const Product4& p, int dtype, int64_t 
   return STK_OK;
 }
 
-static void launch_product(const Product4& p, int dtype, hipStream_t stream) {
-  const dim3 grid((unsigned)((p.outputs + 255) / 256), (unsigned)(p.rows < 65535 ? p.rows : 65535));
-  if (dtype == STK_BF16) hipLaunchKernelGGL((product_kernel<STK_BF16>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((product_kernel<STK_F16>), grid, dim3(256), 0, stream, p);
+template <int KW, int NW, int NT, int MT>
+static void launch_stream(const Product4& p, bool bf16, int64_t row_tiles, hipStream_t stream) {
+  constexpr int lds = (KW - 1) * NW * NT * MT * 1024;
+  const int64_t across = (pieces_out(p.outputs) + NW * NT - 1) / (NW * NT);
+  const auto launch = [&](auto kernel) {
+    set_lds_limit(kernel, lds);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)across, (unsigned)row_tiles), dim3(64 * KW * NW), lds, stream, p);
+  };
+  const bool sub = p.group < kPieceInputs;
+  if (bf16) {
+    if (p.offsets) sub ? launch(stream_kernel<true, true, 4, KW, NW, NT, MT>) : launch(stream_kernel<true, true, 1, KW, NW, NT, MT>);
+    else sub ? launch(stream_kernel<true, false, 4, KW, NW, NT, MT>) : launch(stream_kernel<true, false, 1, KW, NW, NT, MT>);
+  } else {
+    if (p.offsets) sub ? launch(stream_kernel<false, true, 4, KW, NW, NT, MT>) : launch(stream_kernel<false, true, 1, KW, NW, NT, MT>);
+    else sub ? launch(stream_kernel<false, false, 4, KW, NW, NT, MT>) : launch(stream_kernel<false, false, 1, KW, NW, NT, MT>);
+  }
+}
+
+// Tiles of `of` rows that the rows of the experts can be at most.
+static int64_t most_tiles(const Product4& p, int64_t of) {
+  const int64_t hit = p.experts < p.rows ? p.experts : p.rows;
+  return (p.rows + (of - 1) * hit) / of;
+}
+
+static int launch_product(const char* who, const Product4& p, int dtype, hipStream_t stream) {
+  const bool bf16 = dtype == STK_BF16;
+  const int64_t hit = p.experts < p.rows ? p.experts : p.rows, each = p.rows / hit;   // rows of an expert, about
+  const int64_t along = pieces_in(p.inputs);
+  if (most_tiles(p, 16) > 65535) return fail(STK_ERR_UNSUPPORTED, "%s: %lld rows", who, (long long)p.rows);
+  if (each > 32) launch_stream<1, 4, 2, 4>(p, bf16, most_tiles(p, 64), stream);
+  else if (each > 16) launch_stream<2, 2, 2, 2>(p, bf16, most_tiles(p, 32), stream);
+  else if (along >= 64) launch_stream<16, 1, 1, 1>(p, bf16, most_tiles(p, 16), stream);
+  else if (along >= 32 && hit == 1) launch_stream<8, 1, 1, 1>(p, bf16, most_tiles(p, 16), stream);
+  else if (along >= 16) launch_stream<4, 1, 1, 1>(p, bf16, most_tiles(p, 16), stream);
+  else launch_stream<2, 2, 1, 1>(p, bf16, most_tiles(p, 16), stream);
+  return STK_OK;
 }
 
 }  // namespace stk
@@ -265,7 +511,7 @@ extern "C" int stk_matmul_4bit(const void* x, int64_t rows, int64_t x_stride, co
                       out, out_stride, nullptr, activation};
   if (int rc = product_check(who, p, dtype, rows)) return rc;
   if (rows == 0) return STK_OK;
-  launch_product(p, dtype, static_cast<hipStream_t>(stream));
+  if (int rc = launch_product(who, p, dtype, static_cast<hipStream_t>(stream))) return rc;
   return check_launch(who);
 }
 
@@ -279,7 +525,7 @@ extern "C" int stk_gather_matmul_4bit(const void* x, int64_t tokens, int64_t x_s
   if (int rc = product_check(who, p, dtype, tokens)) return rc;
   if (tokens == 0) return STK_OK;
   if (!indices || !bins) return fail(STK_ERR_DIMS, "%s: missing pointer", who);
-  launch_product(p, dtype, static_cast<hipStream_t>(stream));
+  if (int rc = launch_product(who, p, dtype, static_cast<hipStream_t>(stream))) return rc;
   return check_launch(who);
 }
 
@@ -301,15 +547,11 @@ extern "C" int stk_matmul_4bit_scatter(const void* x, int64_t x_stride, const in
   if (int rc = product_check(who, p, dtype, slots)) return rc;
   if (tokens == 0) return STK_OK;
   if (!indices || !bins || !out || out_stride < outputs) return fail(STK_ERR_DIMS, "%s: missing pointer", who);
-  if (tokens * outputs / 256 >= INT32_MAX) return fail(STK_ERR_UNSUPPORTED, "%s: size exceeds 32-bit range", who);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  launch_product(p, dtype, s);
-  const unsigned grid = (unsigned)((tokens * outputs + 255) / 256);
-  if (dtype == STK_BF16)
-    hipLaunchKernelGGL((combine_kernel<STK_BF16>), dim3(grid), dim3(256), 0, s, static_cast<const float*>(workspace), weights, tokens, top_k, outputs,
-                       static_cast<Value<STK_BF16>::stored*>(out), out_stride);
-  else
-    hipLaunchKernelGGL((combine_kernel<STK_F16>), dim3(grid), dim3(256), 0, s, static_cast<const float*>(workspace), weights, tokens, top_k, outputs,
-                       static_cast<Value<STK_F16>::stored*>(out), out_stride);
+  if (int rc = launch_product(who, p, dtype, s)) return rc;
+  const int64_t groups = (tokens * ((outputs + 3) / 4) + 255) / 256;
+  const dim3 grid((unsigned)(groups < 65536 ? groups : 65536));
+  const auto combine = dtype == STK_BF16 ? combine_kernel<true> : combine_kernel<false>;
+  hipLaunchKernelGGL(combine, grid, dim3(256), 0, s, static_cast<const float*>(workspace), weights, tokens, top_k, outputs, static_cast<uint16_t*>(out), out_stride);
   return check_launch(who);
 }

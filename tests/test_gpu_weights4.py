@@ -286,3 +286,30 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         stk.ops.matmul_4bit_scatter(x, r, experts, torch.ones(3, 1))
     assert hip_kernels.matmul_4bit(x, *w[:3], *w[4:]).shape == (3, 32)
+
+
+@pytest.mark.parametrize("rows", [2, 20, 100])
+def test_infinite_and_nan_rows(rows):
+    """They are NaN throughout, whatever the weights, and leave the other rows alone."""
+    for dtype in HALF:
+        codes, scales, offsets = _weights((300, 40), 32, True, dtype, 9)
+        x = torch.randn(rows, 300, generator=torch.Generator().manual_seed(rows)).to(dtype).to(DEV)
+        for w in (_pack(codes, scales, None, 32), _pack(codes, scales, offsets, 32)):
+            want = stk.ops.matmul_4bit(x, w)
+            bad = x.clone()
+            bad[1, 299] = float("inf")
+            bad[rows - 1, 5] = float("nan")
+            got = stk.ops.matmul_4bit(bad, w)
+            for r in range(rows):
+                assert torch.isnan(got[r]).all() if r in (1, rows - 1) else torch.equal(got[r], want[r])
+
+
+def test_values_behind_the_last_input_are_not_used():
+    """Rows of 100 inputs in storage that holds NaN right behind each of them."""
+    codes, scales, _ = _weights((100, 20), 64, False, torch.bfloat16, 10)
+    w = _pack(codes, scales, None, 64)
+    for rows in (1, 30, 90):
+        wide = torch.full((rows, 104), float("nan"), dtype=torch.bfloat16, device=DEV)
+        wide[:, :100] = torch.randn(rows, 100, generator=torch.Generator().manual_seed(rows)).to(DEV)
+        assert torch.equal(stk.ops.matmul_4bit(wide[:, :100], w), stk.ops.matmul_4bit(wide[:, :100].contiguous(), w))
+        assert torch.isfinite(stk.ops.matmul_4bit(wide[:, :100], w)).all()
