@@ -652,7 +652,7 @@ int stk_top_experts_backward(const void* scores, int64_t stride, const int32_t* 
  * with offsets scale = round((max - min) / 15) and offset = round(min), then the nearest codes.
  * stk_pack_4bit lays them out for the products, once: stk_4bit_packed_bytes bytes, 16-byte aligned, of codes and stk_4bit_scales
  * 16-bit elements of scales and of offsets, whose order is the library's own.  stk_dequantize_4bit writes the weights
- * [experts, inputs, outputs] that a packed form stands for, each rounded once.  No counterpart in the reference.
+ * [experts, inputs, outputs] that a packed form stands for, each rounded once.  Packed arrays start at multiples of 16 bytes.  No counterpart in the reference.
  */
 int64_t stk_4bit_packed_bytes(int64_t experts, int64_t inputs, int64_t outputs);
 int64_t stk_4bit_scales(int64_t experts, int64_t inputs, int64_t outputs, int64_t group_size);
@@ -672,7 +672,7 @@ int stk_dequantize_4bit(const void* packed, const void* scales, const void* offs
  *   stk_matmul_4bit_scatter   out[t] = sum over j < top_k, in that order, of weights[s] * (x[p] w[e]), s = t * top_k + j = indices[p]
  *                             (weights NULL: ones; x has a row for each sorted position).  The sums stay fp32 up to the one
  *                             rounding.
- * A row of x with an infinity or a NaN gives NaN throughout its result.  Weights of experts without rows are not read.  workspace: the
+ * A row of x with an infinity, a NaN or sums of more than 2^120 gives NaN throughout its result.  Weights of experts without rows are not read.  workspace: the
  * stk_matmul_4bit*_workspace_bytes, 16-byte aligned, nothing in it is read before it is written (0: may be NULL).
  */
 size_t stk_matmul_4bit_workspace_bytes(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs);

@@ -805,7 +805,7 @@ std::tuple<Tensor, Tensor, OptTensor> pack_4bit(const Tensor& codes_, const Tens
   }
   const int64_t along = (inputs + 127) / 128, down = (outputs + 15) / 16;
   Tensor packed = at::empty({experts, down, along, stk_4bit_packed_bytes(1, 1, 1)}, codes.options());
-  Tensor packed_scales = at::empty({experts, down, groups, 16}, scales.options());
+  Tensor packed_scales = at::empty({experts, down, stk_4bit_scales(1, inputs, 1, group)}, scales.options());
   if (offsets) packed_offsets = at::empty_like(packed_scales);
   check(stk_pack_4bit(ptr<uint8_t>(codes), ptr<void>(scales), ptr<void>(offsets), experts, inputs, outputs, group, ptr<void>(packed), ptr<void>(packed_scales),
                       ptr<void>(packed_offsets), stream_of(codes)));

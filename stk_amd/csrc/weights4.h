@@ -4,8 +4,9 @@
 // codes - output l % 16, of every 32 inputs the eight from 8 (l / 16) on - in the 16 bytes from 16 l on, one dword for each step of
 // 32 inputs.  Bits [4p, 4p + 4) of a dword are the code of input 2p of the eight, the same bits 16 higher that of input 2p + 1, so that
 // one shift and one and-or make a pair of 16-bit values of each.  Pieces follow each other along the inputs, then along the outputs, then
-// expert by expert.  Scales (16-bit): [expert][16 outputs][group][16], so that the four outputs a lane accumulates are 8 bytes.
-// Inputs beyond the last hold code 8, outputs beyond the last scale 0.
+// expert by expert.  Scales (16-bit) come in blocks that belong to 16 outputs and the groups of a piece, or one group of whole
+// pieces: [expert][16 outputs][block][quarter of the outputs][group][4], so that what a lane needs of a block (it accumulates the four outputs
+// of quarter l / 16) is next to each other.  Inputs beyond the last hold code 8, outputs and groups beyond the last scale 0.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -17,6 +18,13 @@ constexpr int kPieceInputs = 128, kPieceOutputs = 16, kPieceBytes = 1024;
 __host__ __device__ inline int64_t pieces_in(int64_t inputs) { return (inputs + kPieceInputs - 1) / kPieceInputs; }
 __host__ __device__ inline int64_t pieces_out(int64_t outputs) { return (outputs + kPieceOutputs - 1) / kPieceOutputs; }
 __host__ __device__ inline int64_t groups_of(int64_t inputs, int64_t group) { return (inputs + group - 1) / group; }
+__host__ __device__ inline int64_t groups_in_block(int64_t group) { return group < kPieceInputs ? kPieceInputs / group : 1; }
+__host__ __device__ inline int64_t scale_blocks(int64_t inputs, int64_t group) { return (groups_of(inputs, group) + groups_in_block(group) - 1) / groups_in_block(group); }
+// Where the scale of output o (0 .. 15) of the tile-th 16 outputs and group g is.
+__host__ __device__ inline int64_t scale_at(int64_t tile, int o, int64_t g, int64_t inputs, int64_t group) {
+  const int64_t sub = groups_in_block(group);
+  return ((tile * scale_blocks(inputs, group) + g / sub) * 4 + o / 4) * 4 * sub + g % sub * 4 + o % 4;
+}
 
 // Byte of a piece and shift in it where the code of output o % 16 and input i % 128 is.
 __host__ __device__ inline void code_at(int o, int i, int* byte, int* shift) {

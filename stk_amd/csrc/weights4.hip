@@ -62,22 +62,25 @@ __global__ __launch_bounds__(256) void pack_codes_kernel(const uint8_t* __restri
   packed[piece * 64 + lane] = u32x4{words[0], words[1], words[2], words[3]};
 }
 
-// Scales [expert][group][output] -> [expert][16 outputs][group][16]; the same for offsets.
-__global__ __launch_bounds__(256) void pack_scales_kernel(const uint16_t* __restrict__ scales, int64_t groups, int64_t outputs, int64_t count,
+// Scales [expert][group][output] -> the order of weights4.h; the same for offsets.
+__global__ __launch_bounds__(256) void pack_scales_kernel(const uint16_t* __restrict__ scales, int64_t inputs, int64_t outputs, int64_t group, int64_t count,
                                                           uint16_t* __restrict__ packed) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= count) return;
-  const int64_t down = pieces_out(outputs), g = at / 16 % groups, o = at / 16 / groups % down * 16 + at % 16, e = at / 16 / groups / down;
-  packed[at] = o < outputs ? scales[(e * groups + g) * outputs + o] : (uint16_t)0;
+  const int64_t sub = groups_in_block(group), blocks = scale_blocks(inputs, group), groups = groups_of(inputs, group), down = pieces_out(outputs);
+  const int64_t within = at % (16 * sub), block = at / (16 * sub) % blocks, tile = at / (16 * sub) / blocks;
+  const int64_t o = tile % down * 16 + within / (4 * sub) * 4 + within % 4, g = block * sub + within / 4 % sub, e = tile / down;
+  packed[at] = o < outputs && g < groups ? scales[(e * groups + g) * outputs + o] : (uint16_t)0;
 }
 
 template <int DTYPE>
 __device__ __forceinline__ float weight_of(const uint8_t* packed, const typename Value<DTYPE>::stored* scales, const typename Value<DTYPE>::stored* offsets,
-                                           int64_t e, int64_t i, int64_t o, int64_t along, int64_t down, int64_t group, int64_t groups) {
+                                           int64_t e, int64_t i, int64_t o, int64_t inputs, int64_t outputs, int64_t group) {
+  const int64_t along = pieces_in(inputs), down = pieces_out(outputs);
   int byte, shift;
   code_at((int)(o & 15), (int)(i & 127), &byte, &shift);
   const int code = packed[((e * down + o / 16) * along + i / 128) * kPieceBytes + byte] >> shift & 15;
-  const int64_t at = ((e * down + o / 16) * groups + i / group) * 16 + o % 16;
+  const int64_t at = scale_at(e * down + o / 16, (int)(o & 15), i / group, inputs, group);
   const float scale = Value<DTYPE>::widen(scales[at]);
   return offsets ? scale * (float)code + Value<DTYPE>::widen(offsets[at]) : scale * (float)(code - 8);
 }
@@ -89,7 +92,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* __restri
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= count) return;
   const int64_t o = at % outputs, i = at / outputs % inputs, e = at / outputs / inputs;
-  out[at] = Value<DTYPE>::round(weight_of<DTYPE>(packed, scales, offsets, e, i, o, pieces_in(inputs), pieces_out(outputs), group, groups_of(inputs, group)));
+  out[at] = Value<DTYPE>::round(weight_of<DTYPE>(packed, scales, offsets, e, i, o, inputs, outputs, group));
 }
 
 __device__ __forceinline__ float activated(float v, int kind) {
@@ -133,14 +136,19 @@ template <> struct Codes<false> {
   static constexpr uint32_t mask = 0x03c003c0u, magic = 0x4c004c00u, minus24 = 0xce00ce00u, minus16 = 0xcc00cc00u;
   static __device__ __forceinline__ uint32_t placed(uint32_t w, int p) { return p == 0 ? w << 6 : p == 1 ? w << 2 : w >> (4 * p - 6); }
 };
+// The mask and the magic number in registers that the compiler takes for variables: with constants it makes two instructions of an
+// and-or, which has no room for two literals.
 template <bool BF16>
-__device__ __forceinline__ u32x4 numbers(uint32_t w) {
-  typedef Codes<BF16> C;
-  u32x4 v;
+struct Decoder {
+  uint32_t mask = Codes<BF16>::mask, magic = Codes<BF16>::magic;
+  __device__ __forceinline__ Decoder() { asm("" : "+s"(mask), "+v"(magic)); }
+  __device__ __forceinline__ u32x4 operator()(uint32_t w) const {
+    u32x4 v;
 #pragma unroll
-  for (int p = 0; p < 4; p++) v[p] = (C::placed(w, p) & C::mask) | C::magic;
-  return v;
-}
+    for (int p = 0; p < 4; p++) v[p] = (Codes<BF16>::placed(w, p) & mask) | magic;
+    return v;
+  }
+};
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 template <bool BF16>
 __device__ __forceinline__ f32x4_t mfma_16x16x32(u32x4 a, u32x4 b, f32x4_t c) {
@@ -188,130 +196,9 @@ __device__ __forceinline__ u32x4 row_values(const uint16_t* row, int i, int inpu
   return v;
 }
 
-// KW wavefronts share the inputs of NW x NT x 16 outputs and 16 MT rows of one expert, a piece of weights at a time; their sums meet
-// in LDS.  SUB: groups of a piece whose sums are scaled apart (1, or 4: groups of 32 or 64).
-template <bool BF16, bool AFFINE, int SUB, int KW, int NW, int NT, int MT>
-__global__ __launch_bounds__(64 * KW * NW) void stream_kernel(Product4 p) {
-  constexpr int kAtOnce = NT * MT == 1 ? 4 : NT * MT == 2 ? 2 : 1;   // pieces whose loads are in flight together
-  extern __shared__ f32x4_t shared[];
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), kw = wave % KW, nw = wave / KW;
-  const RowTile t = row_tile<16 * MT>(p, blockIdx.y, lane);
-  if (t.rows == 0) return;
-  const int along = (int)pieces_in(p.inputs), down = (int)pieces_out(p.outputs), groups = (int)groups_of(p.inputs, p.group);
-  const int row = lane & 15, quarter = lane >> 4;
-  const uint16_t* x[MT];
-  bool has[MT];
-#pragma unroll
-  for (int m = 0; m < MT; m++) {
-    const int r = 16 * m + row;
-    has[m] = r < t.rows;
-    int64_t from = t.first + (has[m] ? r : 0);
-    if (p.top_k > 0) {
-      const int slot = p.indices[from];
-      has[m] = has[m] && (unsigned)slot < (unsigned)p.rows;
-      from = has[m] ? slot / p.top_k : 0;
-    }
-    x[m] = static_cast<const uint16_t*>(p.x) + from * p.x_stride;
-  }
-  int tile[NT];   // (the last tiles of a workgroup may lie beyond the outputs: computed again and not stored)
-  const u32x4* weights[NT];
-  const uint16_t *scales[NT], *offsets[NT];
-#pragma unroll
-  for (int n = 0; n < NT; n++) {
-    tile[n] = ((int)blockIdx.x * NW + nw) * NT + n;
-    const int64_t at = (int64_t)t.expert * down + min(tile[n], down - 1);
-    weights[n] = reinterpret_cast<const u32x4*>(p.packed + at * along * kPieceBytes) + lane;
-    scales[n] = static_cast<const uint16_t*>(p.scales) + at * groups * 16 + 4 * quarter;
-    offsets[n] = static_cast<const uint16_t*>(p.offsets) + at * groups * 16 + 4 * quarter;
-  }
-  const int share = (along + KW - 1) / KW, begin = min(kw * share, along), end = min(begin + share, along);
-  const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-  f32x4_t total[NT][MT];
-#pragma unroll
-  for (int n = 0; n < NT; n++)
-#pragma unroll
-    for (int m = 0; m < MT; m++) total[n][m] = zero;
-  constexpr uint32_t minus = AFFINE ? Codes<BF16>::minus16 : Codes<BF16>::minus24;
-  const u32x4 constant = {minus, minus, minus, minus};
-  const int per_group = (int)(p.group / kPieceInputs), steps = (int)(p.group / 32);   // pieces of a group, or steps of one
-  for (int piece = begin; piece < end; piece += kAtOnce) {
-    u32x4 w[kAtOnce][NT], v[kAtOnce][MT][4];
-    u32x2 s[kAtOnce][NT][SUB], o[kAtOnce][NT][AFFINE ? SUB : 1];
-#pragma unroll
-    for (int u = 0; u < kAtOnce; u++) {
-      const int at = min(piece + u, end - 1);
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        w[u][n] = __builtin_nontemporal_load(weights[n] + (int64_t)at * 64);
-#pragma unroll
-        for (int g = 0; g < SUB; g++) {
-          const int group = min(SUB == 1 ? at / per_group : (4 * at + g) / steps, groups - 1);
-          s[u][n][g] = *reinterpret_cast<const u32x2*>(scales[n] + group * 16);
-          if constexpr (AFFINE) o[u][n][g] = *reinterpret_cast<const u32x2*>(offsets[n] + group * 16);
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int d = 0; d < 4; d++) {
-          v[u][m][d] = u32x4{0u, 0u, 0u, 0u};
-          if (has[m] && piece + u < end) v[u][m][d] = row_values(x[m], at * kPieceInputs + 32 * d + 8 * quarter, (int)p.inputs);
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < kAtOnce; u++)
-#pragma unroll
-      for (int g = 0; g < SUB; g++) {
-        f32x4_t start[MT];
-#pragma unroll
-        for (int m = 0; m < MT; m++) {
-          start[m] = zero;
-#pragma unroll
-          for (int d = 4 / SUB * g; d < 4 / SUB * (g + 1); d++) start[m] = mfma_16x16x32<BF16>(constant, v[u][m][d], start[m]);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          const f32x2_t s0 = unpack2<BF16>(s[u][n][g].x), s1 = unpack2<BF16>(s[u][n][g].y);
-          const f32x4_t scale = {s0.x, s0.y, s1.x, s1.y};
-          f32x4_t sum[MT];
-#pragma unroll
-          for (int m = 0; m < MT; m++) sum[m] = start[m];
-#pragma unroll
-          for (int d = 4 / SUB * g; d < 4 / SUB * (g + 1); d++) {
-            const u32x4 a = numbers<BF16>(w[u][n][d]);
-#pragma unroll
-            for (int m = 0; m < MT; m++) sum[m] = mfma_16x16x32<BF16>(a, v[u][m][d], sum[m]);
-          }
-#pragma unroll
-          for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) total[n][m][i] = fmaf(scale[i], sum[m][i], total[n][m][i]);
-          if constexpr (AFFINE) {
-            const f32x2_t o0 = unpack2<BF16>(o[u][n][g].x), o1 = unpack2<BF16>(o[u][n][g].y);
-            const f32x4_t offset = {o0.x, o0.y, o1.x, o1.y};
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-              for (int i = 0; i < 4; i++) total[n][m][i] = fmaf(offset[i], start[m][i] * -0.0625f, total[n][m][i]);   // start = -16 sum(x)
-          }
-        }
-      }
-  }
-  if constexpr (KW > 1) {
-    if (kw > 0) {
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int m = 0; m < MT; m++) shared[(((kw - 1) * NW + nw) * NT * MT + n * MT + m) * 64 + lane] = total[n][m];
-    }
-    __syncthreads();
-    if (kw > 0) return;
-    for (int k = 0; k < KW - 1; k++)
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int m = 0; m < MT; m++) total[n][m] += shared[((k * NW + nw) * NT * MT + n * MT + m) * 64 + lane];
-  }
+// The sums of a wavefront: total[n][m][i] belongs to output 16 tile[n] + 4 quarter + i and row 16 m + row of the tile.
+template <bool BF16, int NT, int MT>
+__device__ __forceinline__ void store(const Product4& p, const RowTile& t, const int (&tile)[NT], const f32x4_t (&total)[NT][MT], int row, int quarter) {
 #pragma unroll
   for (int m = 0; m < MT; m++) {
     if (16 * m + row >= t.rows) continue;
@@ -342,6 +229,353 @@ __global__ __launch_bounds__(64 * KW * NW) void stream_kernel(Product4 p) {
         for (int i = 0; i < here; i++) at[i] = (uint16_t)(two[i / 2] >> (16 * (i & 1)));
     }
   }
+}
+
+// The products of one group of a piece, scaled and added to the totals.  v(m, d): the fragment of rows 16 m .. 16 m + 15 for step d.
+template <bool BF16, bool AFFINE, int SUB, int NT, int MT, class V>
+__device__ __forceinline__ void add_group(const Decoder<BF16>& numbers, f32x4_t (&total)[NT][MT], int k, const u32x4 (&w)[NT], const u32x2 (&s)[NT][SUB], const u32x2 (&o)[NT][AFFINE ? SUB : 1], V&& v) {
+  constexpr uint32_t minus = AFFINE ? Codes<BF16>::minus16 : Codes<BF16>::minus24;
+  const u32x4 constant = {minus, minus, minus, minus};
+  constexpr int kSteps = 4 / SUB;
+  u32x4 x[kSteps][MT];
+  f32x4_t start[MT];
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    start[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < kSteps; d++) {
+      x[d][m] = v(m, kSteps * k + d);
+      start[m] = mfma_16x16x32<BF16>(constant, x[d][m], start[m]);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    f32x4_t sum[MT];
+#pragma unroll
+    for (int m = 0; m < MT; m++) sum[m] = start[m];
+#pragma unroll
+    for (int d = 0; d < kSteps; d++) {
+      const u32x4 a = numbers(w[n][kSteps * k + d]);
+#pragma unroll
+      for (int m = 0; m < MT; m++) sum[m] = mfma_16x16x32<BF16>(a, x[d][m], sum[m]);
+    }
+    const f32x2_t s0 = unpack2<BF16>(s[n][k].x), s1 = unpack2<BF16>(s[n][k].y);
+    const f32x4_t scale = {s0.x, s0.y, s1.x, s1.y};
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) total[n][m][i] = fmaf(scale[i], sum[m][i], total[n][m][i]);
+    if constexpr (AFFINE) {
+      const f32x2_t o0 = unpack2<BF16>(o[n][k].x), o1 = unpack2<BF16>(o[n][k].y);
+      const f32x4_t offset = {o0.x, o0.y, o1.x, o1.y};
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) total[n][m][i] = fmaf(offset[i], start[m][i] * -0.0625f, total[n][m][i]);   // start = -16 sum(x)
+    }
+  }
+}
+
+// What a wavefront holds of a piece: the codes of NT x 16 outputs, their scales and offsets, and MT x 16 rows of x.
+template <int NT, int MT, int SUB, bool AFFINE>
+struct Stage {
+  u32x4 w[NT], v[MT > 0 ? MT : 1][4];
+  u32x2 s[NT][SUB], o[NT][AFFINE ? SUB : 1];
+};
+
+// Few rows: KW wavefronts share the inputs of NW x NT x 16 outputs and up to 16 rows of one expert, a piece of weights at a time; their sums meet
+// in LDS.  Two pieces are on their way at a time (three or four: the same or slower, registers cost wavefronts).  SUB: groups of a piece whose sums are scaled apart (4, 2 or 1: groups of 32, 64, more).
+// Rows beyond those of the tile are read from its first one: what they give stays in columns that are not stored.
+template <bool BF16, bool AFFINE, int SUB, int KW, int NW, int NT>
+__global__ __launch_bounds__(64 * KW * NW) void stream_kernel(Product4 p) {
+  constexpr int MT = 1, DEPTH = 2;
+  extern __shared__ f32x4_t shared[];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), kw = wave % KW, nw = wave / KW;
+  const RowTile t = row_tile<16 * MT>(p, (int)(blockIdx.z * gridDim.y + blockIdx.y), lane);
+  if (t.rows == 0) return;
+  const int along = (int)pieces_in(p.inputs), down = (int)pieces_out(p.outputs), blocks = (int)scale_blocks(p.inputs, p.group);
+  const int row = lane & 15, quarter = lane >> 4;
+  int tile[NT];   // (the last tiles of a workgroup may lie beyond the outputs: computed again and not stored)
+  const u32x4* weights[NT];
+  const uint16_t *scales[NT], *offsets[NT];
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    tile[n] = ((int)blockIdx.x * NW + nw) * NT + n;
+    const int64_t at = (int64_t)t.expert * down + min(tile[n], down - 1);
+    weights[n] = reinterpret_cast<const u32x4*>(p.packed + at * along * kPieceBytes) + lane;
+    scales[n] = static_cast<const uint16_t*>(p.scales) + (at * blocks * 4 + quarter) * (4 * SUB);
+    offsets[n] = static_cast<const uint16_t*>(p.offsets) + (at * blocks * 4 + quarter) * (4 * SUB);
+  }
+  const uint16_t* x[MT];
+  int64_t from[MT];
+  int slot[MT];
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    from[m] = t.first + (16 * m + row < t.rows ? 16 * m + row : 0);
+    slot[m] = p.top_k > 0 ? p.indices[from[m]] : 0;
+  }
+  const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+  f32x4_t total[NT][MT];
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int m = 0; m < MT; m++) total[n][m] = zero;
+  const int per_block = SUB > 1 ? 1 : (int)(p.group / kPieceInputs);   // pieces with the same scales
+  const Decoder<BF16> numbers;
+  typedef Stage<NT, MT, SUB, AFFINE> S;
+
+  const auto load_weights = [&](S& g, int piece) {
+    const int block = SUB > 1 || per_block == 1 ? piece : piece / per_block;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      g.w[n] = __builtin_nontemporal_load(weights[n] + (int64_t)piece * 64);
+#pragma unroll
+      for (int k = 0; k < SUB; k++) {
+        g.s[n][k] = reinterpret_cast<const u32x2*>(scales[n] + (int64_t)block * (16 * SUB))[k];
+        if constexpr (AFFINE) g.o[n][k] = reinterpret_cast<const u32x2*>(offsets[n] + (int64_t)block * (16 * SUB))[k];
+      }
+    }
+  };
+  const auto load_rows = [&](S& g, int piece) {
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int d = 0; d < 4; d++) g.v[m][d] = __builtin_bit_cast(u32x4, *reinterpret_cast<const QuadAt2*>(x[m] + piece * kPieceInputs + 32 * d));
+  };
+  const auto add = [&](const S& g) {
+#pragma unroll
+    for (int k = 0; k < SUB; k++) add_group<BF16, AFFINE, SUB>(numbers, total, k, g.w, g.s, g.o, [&](int m, int d) { return g.v[m][d]; });
+  };
+
+  const int share = (along + KW - 1) / KW, begin = min(kw * share, along), end = min(begin + share, along);
+  const int whole = max(begin, min(end, (int)(p.inputs / kPieceInputs)));   // the pieces in front of it have all their inputs
+  S stage[DEPTH];
+  int piece = begin;
+  if (piece < whole) load_weights(stage[0], piece);
+  // (the slots were asked for in front of the weights: waiting for them does not wait for those)
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    if (p.top_k > 0) from[m] = (unsigned)slot[m] < (unsigned)p.rows ? slot[m] / p.top_k : 0;
+    x[m] = static_cast<const uint16_t*>(p.x) + from[m] * p.x_stride + 8 * quarter;
+  }
+  if (piece < whole) {
+    load_rows(stage[0], piece);
+#pragma unroll
+    for (int u = 1; u < DEPTH; u++) load_weights(stage[u], min(piece + u, whole - 1)), load_rows(stage[u], min(piece + u, whole - 1));
+    for (; piece + 2 * DEPTH <= whole; piece += DEPTH)
+#pragma unroll
+      for (int u = 0; u < DEPTH; u++) add(stage[u]), load_weights(stage[u], piece + DEPTH + u), load_rows(stage[u], piece + DEPTH + u);
+#pragma unroll
+    for (int u = 0; u < DEPTH; u++) {
+      if (piece + u < whole) add(stage[u]);
+      if (piece + DEPTH + u < whole) load_weights(stage[u], piece + DEPTH + u), load_rows(stage[u], piece + DEPTH + u);
+    }
+#pragma unroll
+    for (int u = 0; u < DEPTH; u++)
+      if (piece + DEPTH + u < whole) add(stage[u]);
+  }
+  if (end > whole) {   // the last piece, whose inputs end inside it
+    load_weights(stage[0], whole);
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int d = 0; d < 4; d++) stage[0].v[m][d] = row_values(x[m], whole * kPieceInputs + 32 * d, (int)p.inputs - 8 * quarter);
+    add(stage[0]);
+  }
+  if constexpr (KW > 1) {
+    if (kw > 0) {
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int m = 0; m < MT; m++) shared[(((kw - 1) * NW + nw) * NT * MT + n * MT + m) * 64 + lane] = total[n][m];
+    }
+    __syncthreads();
+    if (kw > 0) return;
+    for (int k = 0; k < KW - 1; k++)
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int m = 0; m < MT; m++) total[n][m] += shared[((k * NW + nw) * NT * MT + n * MT + m) * 64 + lane];
+  }
+  store<BF16>(p, t, tile, total, row, quarter);
+}
+
+// Many rows: four wavefronts, side by side on 64 NT outputs, share 16 MT rows of one expert, whose values pass through LDS in pieces of
+// 128 inputs (two of them, one being multiplied and one being written).  A code then becomes a number once for 16 MT rows.
+template <bool BF16, bool AFFINE, int SUB, int NT, int MT>
+__global__ __launch_bounds__(256) void tile_kernel(Product4 p) {
+  __shared__ u32x4 values[2][16 * MT * 16];   // [row][eight inputs], the place within a row swizzled by the row
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const RowTile t = row_tile<16 * MT>(p, (int)(blockIdx.z * gridDim.y + blockIdx.y), lane);
+  if (t.rows == 0) return;
+  const int along = (int)pieces_in(p.inputs), down = (int)pieces_out(p.outputs), blocks = (int)scale_blocks(p.inputs, p.group);
+  const int whole = (int)(p.inputs / kPieceInputs), row = lane & 15, quarter = lane >> 4;
+  // what this thread carries to LDS: eight inputs, number `eight` of a piece, of every 16th row
+  const int eight = threadIdx.x & 15, carried = threadIdx.x >> 4;
+  const uint16_t* x[MT];
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    int64_t from = t.first + (16 * m + carried < t.rows ? 16 * m + carried : 0);
+    if (p.top_k > 0) {
+      const int slot = p.indices[from];
+      from = (unsigned)slot < (unsigned)p.rows ? slot / p.top_k : 0;
+    }
+    x[m] = static_cast<const uint16_t*>(p.x) + from * p.x_stride;
+  }
+  int tile[NT];
+  const u32x4* weights[NT];
+  const uint16_t *scales[NT], *offsets[NT];
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    tile[n] = ((int)blockIdx.x * 4 + wave) * NT + n;
+    const int64_t at = (int64_t)t.expert * down + min(tile[n], down - 1);
+    weights[n] = reinterpret_cast<const u32x4*>(p.packed + at * along * kPieceBytes) + lane;
+    scales[n] = static_cast<const uint16_t*>(p.scales) + (at * blocks * 4 + quarter) * (4 * SUB);
+    offsets[n] = static_cast<const uint16_t*>(p.offsets) + (at * blocks * 4 + quarter) * (4 * SUB);
+  }
+  const int per_block = SUB > 1 ? 1 : (int)(p.group / kPieceInputs);
+  const Decoder<BF16> numbers;
+  u32x4 carry[MT];
+  Stage<NT, 0, SUB, AFFINE> ahead;   // the weights of the next piece
+  const auto load_weights = [&](int piece) {
+    const int block = SUB > 1 || per_block == 1 ? piece : piece / per_block;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      ahead.w[n] = weights[n][(int64_t)piece * 64];
+#pragma unroll
+      for (int k = 0; k < SUB; k++) {
+        ahead.s[n][k] = reinterpret_cast<const u32x2*>(scales[n] + (int64_t)block * (16 * SUB))[k];
+        if constexpr (AFFINE) ahead.o[n][k] = reinterpret_cast<const u32x2*>(offsets[n] + (int64_t)block * (16 * SUB))[k];
+      }
+    }
+  };
+  const auto load_rows = [&](int piece) {
+    const int i = piece * kPieceInputs + 8 * eight;
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+      carry[m] = piece < whole ? __builtin_bit_cast(u32x4, *reinterpret_cast<const QuadAt2*>(x[m] + i)) : row_values(x[m], i, (int)p.inputs);
+  };
+  const auto write_rows = [&](u32x4* to) {
+#pragma unroll
+    for (int m = 0; m < MT; m++) to[(16 * m + carried) * 16 + (eight ^ carried)] = carry[m];
+  };
+  f32x4_t total[NT][MT];
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int m = 0; m < MT; m++) total[n][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  load_rows(0);
+  load_weights(0);
+  write_rows(values[0]);
+  __syncthreads();
+  for (int piece = 0; piece < along; piece++) {
+    const auto here = ahead;
+    if (piece + 1 < along) load_rows(piece + 1), load_weights(piece + 1);
+    const u32x4* from = values[piece & 1];
+#pragma unroll
+    for (int k = 0; k < SUB; k++)
+      add_group<BF16, AFFINE, SUB>(numbers, total, k, here.w, here.s, here.o, [&](int m, int d) { return from[(16 * m + row) * 16 + ((4 * d + quarter) ^ row)]; });
+    if (piece + 1 < along) write_rows(values[(piece + 1) & 1]);
+    __syncthreads();
+  }
+  store<BF16>(p, t, tile, total, row, quarter);
+}
+
+// The same with everything on its way to LDS without registers, a piece of x, codes and scales being multiplied and the next one
+// arriving: rows whose values come in whole 16-byte pieces at multiples of 16 bytes.  What counts is how many wavefronts are on a compute
+// unit (16384 rows over 64 experts, 1024 x 4096: 212 us; three stages of the same 263, the kernel above 314).
+static __device__ u32x4 no_values;   // (what lies behind the last input)
+// 16 bytes per lane from any addresses into the LDS bytes from lds_base on, lane after lane.
+__device__ __forceinline__ void dma16_any(const void* from, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(uniform((int)lds_base)), "v"((uint64_t)from) : "memory", "m0");
+}
+template <int NT, int MT>
+struct Stage16 {
+  static constexpr int kRows = MT * 4096, kCodes = 4 * NT * 1024, kScales = 4 * 512;   // bytes of a stage
+  static constexpr int bytes(bool affine) { return kRows + kCodes + (affine ? 2 : 1) * kScales; }
+};
+template <bool BF16, bool AFFINE, int SUB, int NT, int MT>
+__global__ __launch_bounds__(256, 2) void ring_kernel(Product4 p) {
+  typedef Stage16<NT, MT> R;
+  constexpr int kStage = R::bytes(AFFINE);
+  extern __shared__ char smem[];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const RowTile t = row_tile<16 * MT>(p, (int)(blockIdx.z * gridDim.y + blockIdx.y), lane);
+  if (t.rows == 0) return;
+  const int along = (int)pieces_in(p.inputs), down = (int)pieces_out(p.outputs), blocks = (int)scale_blocks(p.inputs, p.group);
+  const int row = lane & 15, quarter = lane >> 4;
+  // a transfer carries four rows; this lane eight inputs of one of them, put where that row's swizzle wants them
+  const char* x[MT];
+  int first_input[MT];
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    const int r = 4 * (m * 4 + wave) + quarter;
+    int64_t from = t.first + (r < t.rows ? r : 0);
+    if (p.top_k > 0) {
+      const int slot = p.indices[from];
+      from = (unsigned)slot < (unsigned)p.rows ? slot / p.top_k : 0;
+    }
+    first_input[m] = 8 * (row ^ (r & 15));
+    x[m] = reinterpret_cast<const char*>(static_cast<const uint16_t*>(p.x) + from * p.x_stride + first_input[m]);
+  }
+  int tile[NT];
+  gptr_t weights[NT];
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    tile[n] = ((int)blockIdx.x * 4 + wave) * NT + n;
+    weights[n] = uniform_global(p.packed + ((int64_t)t.expert * down + min(tile[n], down - 1)) * along * kPieceBytes);
+  }
+  const int per_block = SUB > 1 ? 1 : (int)(p.group / kPieceInputs);
+  // lanes that carry scales: 2 SUB for each 16 outputs
+  const int mine = min(((int)blockIdx.x * 4 + wave) * NT + lane / (2 * SUB), down - 1);
+  const int64_t scale_from = ((int64_t)t.expert * down + mine) * blocks * (32 * SUB) + lane % (2 * SUB) * 16;
+  const uint32_t lds = (uint32_t)(uintptr_t)(STK_LDS char*)smem;
+  const auto issue = [&](int piece, int stage) {
+    const uint32_t to = lds + stage * kStage;
+    const bool last = (piece + 1) * kPieceInputs > p.inputs;
+#pragma unroll
+    for (int n = 0; n < NT; n++) dma16(weights[n] + (int64_t)piece * kPieceBytes, lane * 16, to + R::kRows + (wave * NT + n) * 1024);
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+      const char* from = x[m] + (int64_t)piece * (2 * kPieceInputs);
+      if (last && piece * kPieceInputs + first_input[m] >= p.inputs) from = reinterpret_cast<const char*>(&no_values);
+      dma16_any(from, to + (m * 4 + wave) * 1024);
+    }
+    if (lane < NT * 2 * SUB) {
+      const int64_t at = scale_from + (int64_t)(SUB > 1 || per_block == 1 ? piece : piece / per_block) * (32 * SUB);
+      dma16_any(static_cast<const char*>(p.scales) + at, to + R::kRows + R::kCodes + wave * 512);
+      if constexpr (AFFINE) dma16_any(static_cast<const char*>(p.offsets) + at, to + R::kRows + R::kCodes + R::kScales + wave * 512);
+    }
+  };
+  const Decoder<BF16> numbers;
+  f32x4_t total[NT][MT];
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int m = 0; m < MT; m++) total[n][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  issue(0, 0);
+  for (int piece = 0; piece < along; piece++) {
+    wait_vmcnt<0>();
+    __syncthreads();   // everybody's part of the piece is there, and everybody is done with the one whose place is filled now
+    if (piece + 1 < along) issue(piece + 1, (piece + 1) & 1);
+    const char* from = smem + (piece & 1) * kStage;
+    u32x4 w[NT];
+    u32x2 s[NT][SUB], o[NT][AFFINE ? SUB : 1];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      w[n] = reinterpret_cast<const u32x4*>(from + R::kRows + (wave * NT + n) * 1024)[lane];
+#pragma unroll
+      for (int k = 0; k < SUB; k++) {
+        s[n][k] = reinterpret_cast<const u32x2*>(from + R::kRows + R::kCodes + wave * 512 + n * 32 * SUB)[quarter * SUB + k];
+        if constexpr (AFFINE) o[n][k] = reinterpret_cast<const u32x2*>(from + R::kRows + R::kCodes + R::kScales + wave * 512 + n * 32 * SUB)[quarter * SUB + k];
+      }
+    }
+    const u32x4* values = reinterpret_cast<const u32x4*>(from);
+#pragma unroll
+    for (int k = 0; k < SUB; k++)
+      add_group<BF16, AFFINE, SUB>(numbers, total, k, w, s, o, [&](int m, int d) { return values[(16 * m + row) * 16 + ((4 * d + quarter) ^ row)]; });
+  }
+  store<BF16>(p, t, tile, total, row, quarter);
 }
 
 // out[t] = sum over the choices j of a token, in their order, of (weights[s]) sums[s], s = t top_k + j; rounded once.  A thread per
@@ -390,27 +624,8 @@ static int product_check(const char* who, const Product4& p, int dtype, int64_t 
   if (p.activation < 0 || p.activation > kSilu) return fail(STK_ERR_UNSUPPORTED, "%s: activation %d", who, p.activation);
   if (p.x_stride < 0 || (p.out && p.out_stride < p.outputs)) return fail(STK_ERR_DIMS, "%s: strides", who);
   if (p.rows > 0 && (!p.x || !p.packed || !p.scales || (!p.out && !p.sums))) return fail(STK_ERR_DIMS, "%s: missing pointer", who);
-  if (!aligned16(p.packed) || (reinterpret_cast<uintptr_t>(p.scales) & 7) || (reinterpret_cast<uintptr_t>(p.offsets) & 7))
-    return fail(STK_ERR_UNSUPPORTED, "%s: packed weights at multiples of 16 bytes, scales of 8", who);
+  if (!aligned16(p.packed) || !aligned16(p.scales) || !aligned16(p.offsets)) return fail(STK_ERR_UNSUPPORTED, "%s: packed weights and scales at multiples of 16 bytes", who);
   return STK_OK;
-}
-
-template <int KW, int NW, int NT, int MT>
-static void launch_stream(const Product4& p, bool bf16, int64_t row_tiles, hipStream_t stream) {
-  constexpr int lds = (KW - 1) * NW * NT * MT * 1024;
-  const int64_t across = (pieces_out(p.outputs) + NW * NT - 1) / (NW * NT);
-  const auto launch = [&](auto kernel) {
-    set_lds_limit(kernel, lds);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)across, (unsigned)row_tiles), dim3(64 * KW * NW), lds, stream, p);
-  };
-  const bool sub = p.group < kPieceInputs;
-  if (bf16) {
-    if (p.offsets) sub ? launch(stream_kernel<true, true, 4, KW, NW, NT, MT>) : launch(stream_kernel<true, true, 1, KW, NW, NT, MT>);
-    else sub ? launch(stream_kernel<true, false, 4, KW, NW, NT, MT>) : launch(stream_kernel<true, false, 1, KW, NW, NT, MT>);
-  } else {
-    if (p.offsets) sub ? launch(stream_kernel<false, true, 4, KW, NW, NT, MT>) : launch(stream_kernel<false, true, 1, KW, NW, NT, MT>);
-    else sub ? launch(stream_kernel<false, false, 4, KW, NW, NT, MT>) : launch(stream_kernel<false, false, 1, KW, NW, NT, MT>);
-  }
 }
 
 // Tiles of `of` rows that the rows of the experts can be at most.
@@ -418,18 +633,89 @@ static int64_t most_tiles(const Product4& p, int64_t of) {
   const int64_t hit = p.experts < p.rows ? p.experts : p.rows;
   return (p.rows + (of - 1) * hit) / of;
 }
+// Row tiles lie along y, and beyond what y holds along z (those that there are not end at once).
+static dim3 grid_of(int64_t across, int64_t row_tiles) {
+  const int64_t layers = (row_tiles + 65534) / 65535;
+  return dim3((unsigned)across, (unsigned)((row_tiles + layers - 1) / layers), (unsigned)layers);
+}
+// fn(bf16, affine, groups of a piece) as constants.
+template <class Fn>
+static void for_form(const Product4& p, bool bf16, Fn&& fn) {
+  const auto by_group = [&](auto type, auto affine) {
+    if (p.group == 32) fn(type, affine, std::integral_constant<int, 4>());
+    else if (p.group == 64) fn(type, affine, std::integral_constant<int, 2>());
+    else fn(type, affine, std::integral_constant<int, 1>());
+  };
+  const auto by_offsets = [&](auto type) {
+    if (p.offsets) by_group(type, std::true_type());
+    else by_group(type, std::false_type());
+  };
+  if (bf16) by_offsets(std::true_type());
+  else by_offsets(std::false_type());
+}
+template <int KW, int NW, int NT>
+static void launch_stream(const Product4& p, bool bf16, hipStream_t stream) {
+  for_form(p, bf16, [&](auto type, auto affine, auto sub) {
+    constexpr int lds = (KW - 1) * NW * NT * 1024;
+    const auto kernel = stream_kernel<decltype(type)::value, decltype(affine)::value, decltype(sub)::value, KW, NW, NT>;
+    set_lds_limit(kernel, lds);
+    const int64_t across = (pieces_out(p.outputs) + NW * NT - 1) / (NW * NT);
+    hipLaunchKernelGGL(kernel, grid_of(across, most_tiles(p, 16)), dim3(64 * KW * NW), lds, stream, p);
+  });
+}
+template <int NT, int MT>
+static void launch_tiles(const Product4& p, bool bf16, hipStream_t stream) {
+  for_form(p, bf16, [&](auto type, auto affine, auto sub) {
+    const auto kernel = tile_kernel<decltype(type)::value, decltype(affine)::value, decltype(sub)::value, NT, MT>;
+    const int64_t across = (pieces_out(p.outputs) + 4 * NT - 1) / (4 * NT);
+    hipLaunchKernelGGL(kernel, grid_of(across, most_tiles(p, 16 * MT)), dim3(256), 0, stream, p);
+  });
+}
 
+template <int NT, int MT>
+static void launch_ring(const Product4& p, bool bf16, hipStream_t stream) {
+  for_form(p, bf16, [&](auto type, auto affine, auto sub) {
+    constexpr int lds = 2 * Stage16<NT, MT>::bytes(decltype(affine)::value);
+    const auto kernel = ring_kernel<decltype(type)::value, decltype(affine)::value, decltype(sub)::value, NT, MT>;
+    set_lds_limit(kernel, lds);
+    const int64_t across = (pieces_out(p.outputs) + 4 * NT - 1) / (4 * NT);
+    hipLaunchKernelGGL(kernel, grid_of(across, most_tiles(p, 16 * MT)), dim3(256), lds, stream, p);
+  });
+}
+
+// Which kernel.  With T tiles of 16 rows and 16 outputs, and pieces along the inputs, the streams want some thousand wavefronts and then
+// as many outputs for one as possible: a fragment of x serves all of them.  Rows in some number share codes instead (ring, or tile
+// where x is no whole 16-byte pieces).  us at T, pieces, in the order of the rule below, KW x NW x NT (bf16, groups of 128, cold):
+//                                   8x1x1  4x1x2  2x2x2  4x1x4  1x4x4     ring, rows x outputs:  16x128  32x128  32x256
+//   256, 32   (1 row, 4096 x 4096)    7.9    9.9   14.3   12.4   24.5
+//   512, 32   (32 rows, the same)    13.9   11.3   15.4   13.6   28.5                             21.7    25.9    39.7
+//   1024, 32  (64 rows)              21.8   15.6   15.8   13.9   29.3                             22.0    26.2    39.9
+//   4096, 32  (256 rows)             69.8   43.0   43.7   32.4   31.3                             27.7    27.5    40.0
+//   2048, 8   (16 rows, 8 experts, 1024 x 4096) 19.8 10.5 10.4 10.9 13.8                          11.0    12.0    16.2
+//   6144, 8   (32 rows, 24 of 64 experts)       52.9 22.0 19.5 24.6 19.2
+//   16384, 8  (256 rows, 64 experts) 144    50.8   40.8   56.7   34.4                             35.1    37.9    40.4
+//   4096, 32  (256 rows, 64 experts, 4096 x 1024) 65.0 44.5 43.8 40.6 42.8                        40.8    45.4    49.4
+//   (512 rows over 8 experts, 1024 x 4096)                                                        19.1    18.4    21.9
+//   (2048 rows over 64 experts)                                                                   57.9    53.2    50.2
+//   (16384 rows over 64 experts)                                                                  --     237     212
 static int launch_product(const char* who, const Product4& p, int dtype, hipStream_t stream) {
   const bool bf16 = dtype == STK_BF16;
-  const int64_t hit = p.experts < p.rows ? p.experts : p.rows, each = p.rows / hit;   // rows of an expert, about
-  const int64_t along = pieces_in(p.inputs);
-  if (most_tiles(p, 16) > 65535) return fail(STK_ERR_UNSUPPORTED, "%s: %lld rows", who, (long long)p.rows);
-  if (each > 32) launch_stream<1, 4, 2, 4>(p, bf16, most_tiles(p, 64), stream);
-  else if (each > 16) launch_stream<2, 2, 2, 2>(p, bf16, most_tiles(p, 32), stream);
-  else if (along >= 64) launch_stream<16, 1, 1, 1>(p, bf16, most_tiles(p, 16), stream);
-  else if (along >= 32 && hit == 1) launch_stream<8, 1, 1, 1>(p, bf16, most_tiles(p, 16), stream);
-  else if (along >= 16) launch_stream<4, 1, 1, 1>(p, bf16, most_tiles(p, 16), stream);
-  else launch_stream<2, 2, 1, 1>(p, bf16, most_tiles(p, 16), stream);
+  if (most_tiles(p, 16) > (int64_t)65535 * 65535) return fail(STK_ERR_UNSUPPORTED, "%s: %lld rows", who, (long long)p.rows);
+  const int64_t along = pieces_in(p.inputs), down = pieces_out(p.outputs);
+  // as if the rows were spread evenly over the experts: where they really are only the device knows
+  const int64_t hit = p.experts < p.rows ? p.experts : p.rows, each = (p.rows + hit - 1) / hit;
+  const int64_t tiles = hit * ((each + 15) / 16) * down, across8 = (down + 7) / 8, across16 = (down + 15) / 16, tall = hit * ((each + 31) / 32);
+  if (along >= 24 ? each > 16 && tiles > 3000 : each >= 8 && tiles >= 1536) {
+    const bool whole = p.inputs % 8 == 0 && p.x_stride % 8 == 0 && aligned16(p.x);
+    if (!whole) launch_tiles<2, 2>(p, bf16, stream);
+    else if (each >= 24 && tall * across16 >= 512) launch_ring<4, 2>(p, bf16, stream);
+    else if (each >= 12 && tall * across8 >= 256) launch_ring<2, 2>(p, bf16, stream);
+    else launch_ring<2, 1>(p, bf16, stream);
+  } else if (tiles <= 320) launch_stream<8, 1, 1>(p, bf16, stream);
+  else if (tiles <= 640) launch_stream<4, 1, 2>(p, bf16, stream);
+  else if (along >= 24) launch_stream<4, 1, 4>(p, bf16, stream);
+  else if (tiles <= 4096) launch_stream<2, 2, 2>(p, bf16, stream);
+  else launch_stream<1, 4, 4>(p, bf16, stream);
   return STK_OK;
 }
 
@@ -441,7 +727,7 @@ extern "C" int64_t stk_4bit_packed_bytes(int64_t experts, int64_t inputs, int64_
   return experts < 1 || inputs < 1 || outputs < 1 ? 0 : experts * pieces_in(inputs) * pieces_out(outputs) * kPieceBytes;
 }
 extern "C" int64_t stk_4bit_scales(int64_t experts, int64_t inputs, int64_t outputs, int64_t group_size) {
-  return experts < 1 || inputs < 1 || outputs < 1 || group_size < 1 ? 0 : experts * groups_of(inputs, group_size) * pieces_out(outputs) * kPieceOutputs;
+  return experts < 1 || inputs < 1 || outputs < 1 || group_size < 1 ? 0 : experts * scale_blocks(inputs, group_size) * groups_in_block(group_size) * pieces_out(outputs) * kPieceOutputs;
 }
 
 extern "C" int stk_quantize_4bit(const void* w, int64_t stride_e, int64_t stride_i, int64_t stride_o, int64_t experts, int64_t inputs, int64_t outputs,
@@ -475,12 +761,11 @@ extern "C" int stk_pack_4bit(const uint8_t* codes, const void* scales, const voi
   if (!aligned16(packed)) return fail(STK_ERR_UNSUPPORTED, "%s: packed weights at a multiple of 16 bytes", who);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t pieces = experts * pieces_in(inputs) * pieces_out(outputs), count = stk_4bit_scales(experts, inputs, outputs, group_size);
-  const int64_t groups = groups_of(inputs, group_size);
   hipLaunchKernelGGL(pack_codes_kernel, dim3((unsigned)((pieces + 3) / 4)), dim3(256), 0, s, codes, inputs, outputs, pieces, static_cast<u32x4*>(packed));
-  hipLaunchKernelGGL(pack_scales_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, s, static_cast<const uint16_t*>(scales), groups, outputs, count,
+  hipLaunchKernelGGL(pack_scales_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, s, static_cast<const uint16_t*>(scales), inputs, outputs, group_size, count,
                      static_cast<uint16_t*>(packed_scales));
   if (offsets)
-    hipLaunchKernelGGL(pack_scales_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, s, static_cast<const uint16_t*>(offsets), groups, outputs, count,
+    hipLaunchKernelGGL(pack_scales_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, s, static_cast<const uint16_t*>(offsets), inputs, outputs, group_size, count,
                        static_cast<uint16_t*>(packed_offsets));
   return check_launch(who);
 }

@@ -135,6 +135,30 @@ def test_product(rows, inputs, outputs, group, affine, dtype):
     _check(stk.ops.matmul_4bit(x.to(DEV), w, activation), sums, slack, dtype, activation)
 
 
+# one size for every kernel that the launch rule chooses from; inputs of no multiple of eight take the way through registers
+BY_RULE = [(2100, 392, 2050, 128), (2100, 395, 2050, 32), (530, 264, 2048, 64), (530, 257, 2048, 128), (200, 136, 2050, 32), (200, 3080, 2050, 128), (550, 3080, 2050, 64),
+           (40, 520, 2050, 128), (9, 300, 12001, 64), (3, 3080, 11000, 128)]
+
+
+@pytest.mark.parametrize("dtype,affine", [(torch.bfloat16, False), (torch.float16, True)])
+@pytest.mark.parametrize("rows,inputs,outputs,group", BY_RULE)
+def test_product_of_every_kernel(rows, inputs, outputs, group, affine, dtype):
+    codes, scales, offsets = _weights((inputs, outputs), group, affine, dtype, rows + inputs)
+    x = torch.randn(rows, inputs, generator=torch.Generator().manual_seed(rows)).to(dtype)
+    got = stk.ops.matmul_4bit(x.to(DEV), _pack(codes, scales, offsets, group))
+    _check(got, _n64(x) @ L.weights4(codes.numpy(), _n64(scales), group, _n64(offsets)), _slack(x, codes, scales, offsets, group), dtype)
+
+
+@pytest.mark.parametrize("rows", [40, 300])
+def test_rows_of_a_view_give_the_same(rows):
+    """Rows that lie in whole 16-byte pieces and rows that do not: another kernel, sums in the same order."""
+    codes, scales, _ = _weights((264, 2064), 128, False, torch.bfloat16, 11)
+    w = _pack(codes, scales, None, 128)
+    x = torch.randn(rows, 264, generator=torch.Generator().manual_seed(rows)).bfloat16().to(DEV)
+    off = torch.empty(rows * 264 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(rows, 264).copy_(x)
+    assert torch.equal(stk.ops.matmul_4bit(off, w), stk.ops.matmul_4bit(x, w))
+
+
 @pytest.mark.parametrize("activation", list(ACT))
 def test_activations(activation):
     codes, scales, _ = _weights((256, 64), 128, False, torch.bfloat16, 1)
@@ -177,7 +201,8 @@ def _route(tokens, experts, top_k, how, blocking, seed):
 ROUTED = [(1, 4, 1, 128, 16, 128, "any", 1), (1, 64, 2, 256, 48, 64, "any", 128), (3, 4, 4, 200, 33, 32, "any", 1), (64, 64, 2, 256, 64, 128, "any", 1),
           (100, 8, 2, 384, 100, 128, "half", 1), (50, 200, 1, 64, 16, 64, "any", 1), (300, 4, 1, 130, 40, 32, "one", 1), (33, 16, 3, 512, 80, 256, "any", 64),
           (500, 6, 2, 256, 96, 128, "half", 1), (17, 1, 1, 128, 20, 128, "any", 1), (40, 32, 8, 96, 24, 32, "any", 1), (5, 1024, 2, 32, 16, 32, "any", 1),
-          (2000, 3, 1, 160, 144, 32, "any", 128)]
+          (2000, 3, 1, 160, 144, 32, "any", 128), (160, 64, 2, 136, 1120, 128, "any", 1), (600, 16, 2, 264, 528, 64, "half", 1), (1000, 8, 2, 264, 1040, 32, "half", 1),
+          (300, 8, 2, 137, 1040, 128, "any", 1), (2, 4, 2, 3200, 700, 64, "any", 1)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -211,7 +236,7 @@ def test_routed_products(tokens, experts, top_k, inputs, outputs, group, how, bl
 def test_experts_without_rows_are_not_read():
     """Scales of NaN in experts that no token is sent to."""
     codes, scales, _ = _weights((8, 128, 32), 128, False, torch.bfloat16, 4)
-    scales[[0, 2, 3, 7]] = float("nan")
+    scales[[0, 2, 3, 7]] = float("nan")   # (their codes' numbers and scales would make NaN of whatever they met)
     w = _pack(codes, scales, None, 128)
     top = torch.tensor([[1, 4], [5, 6], [6, 1]], dtype=torch.int32, device=DEV)
     r = stk.ops.route(top, 8, 1)
@@ -288,11 +313,11 @@ def test_refusals():
     assert hip_kernels.matmul_4bit(x, *w[:3], *w[4:]).shape == (3, 32)
 
 
-@pytest.mark.parametrize("rows", [2, 20, 100])
-def test_infinite_and_nan_rows(rows):
+@pytest.mark.parametrize("rows,outputs", [(2, 40), (20, 40), (100, 40), (100, 4100), (700, 1100)])
+def test_infinite_and_nan_rows(rows, outputs):
     """They are NaN throughout, whatever the weights, and leave the other rows alone."""
     for dtype in HALF:
-        codes, scales, offsets = _weights((300, 40), 32, True, dtype, 9)
+        codes, scales, offsets = _weights((300, outputs), 32, True, dtype, 9)
         x = torch.randn(rows, 300, generator=torch.Generator().manual_seed(rows)).to(dtype).to(DEV)
         for w in (_pack(codes, scales, None, 32), _pack(codes, scales, offsets, 32)):
             want = stk.ops.matmul_4bit(x, w)
@@ -306,9 +331,9 @@ def test_infinite_and_nan_rows(rows):
 
 def test_values_behind_the_last_input_are_not_used():
     """Rows of 100 inputs in storage that holds NaN right behind each of them."""
-    codes, scales, _ = _weights((100, 20), 64, False, torch.bfloat16, 10)
+    codes, scales, _ = _weights((100, 2000), 64, False, torch.bfloat16, 10)
     w = _pack(codes, scales, None, 64)
-    for rows in (1, 30, 90):
+    for rows in (1, 30, 90, 300):
         wide = torch.full((rows, 104), float("nan"), dtype=torch.bfloat16, device=DEV)
         wide[:, :100] = torch.randn(rows, 100, generator=torch.Generator().manual_seed(rows)).to(DEV)
         assert torch.equal(stk.ops.matmul_4bit(wide[:, :100], w), stk.ops.matmul_4bit(wide[:, :100].contiguous(), w))

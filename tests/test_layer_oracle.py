@@ -122,7 +122,8 @@ def test_abi_refusals_of_top_experts():
 def test_abi_refusals_and_sizes_of_4bit_weights():
     lib, one = _lib.load(), ctypes.c_void_p(256)
     assert lib.stk_4bit_packed_bytes(3, 129, 17) == 3 * 2 * 2 * 1024 and lib.stk_4bit_packed_bytes(1, 0, 17) == 0
-    assert lib.stk_4bit_scales(3, 129, 17, 32) == 3 * 5 * 32 and lib.stk_4bit_scales(1, 128, 16, 256) == 16
+    # whole pieces of 128 inputs, whole blocks of the groups of a piece, 16 outputs
+    assert lib.stk_4bit_scales(3, 129, 17, 32) == 3 * 8 * 32 and lib.stk_4bit_scales(1, 128, 16, 256) == 16
     mm = lambda group=128, dtype=_lib.STK_BF16, act=0, x=one, out_stride=16, packed=one: lib.stk_matmul_4bit(
         x, 4, 128, packed, one, None, 128, 16, group, one, out_stride, act, dtype, None, 0, None)
     _bad(mm(group=48), _lib.STK_ERR_UNSUPPORTED, "groups of 32, 64 or a multiple of 128")
