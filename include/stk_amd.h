@@ -672,18 +672,16 @@ int stk_dequantize_4bit(const void* packed, const void* scales, const void* offs
  *   stk_matmul_4bit_scatter   out[t] = sum over j < top_k, in that order, of weights[s] * (x[p] w[e]), s = t * top_k + j = indices[p]
  *                             (weights NULL: ones; x has a row for each sorted position).  The sums stay fp32 up to the one
  *                             rounding.
- * A row of x with an infinity, a NaN or sums of more than 2^120 gives NaN throughout its result.  Weights of experts without rows are not read.  workspace: the
- * stk_matmul_4bit*_workspace_bytes, 16-byte aligned, nothing in it is read before it is written (0: may be NULL).
+ * A row of x with an infinity, a NaN or sums of more than 2^120 gives NaN throughout its result.  Weights of experts without rows are not read.  workspace:
+ * stk_matmul_4bit_scatter_workspace_bytes(tokens * top_k, outputs) bytes, 16-byte aligned, nothing in it is read before it is written.
  */
-size_t stk_matmul_4bit_workspace_bytes(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs);
 int stk_matmul_4bit(const void* x, int64_t rows, int64_t x_stride, const void* packed, const void* scales, const void* offsets,
                     int64_t inputs, int64_t outputs, int64_t group_size, void* out, int64_t out_stride, int activation, int dtype,
-                    void* workspace, size_t workspace_bytes, stk_stream_t stream);
+                    stk_stream_t stream);
 int stk_gather_matmul_4bit(const void* x, int64_t tokens, int64_t x_stride, const int32_t* indices, const int32_t* bins, int top_k,
                            const void* packed, const void* scales, const void* offsets, int64_t experts, int64_t inputs, int64_t outputs,
-                           int64_t group_size, void* out, int64_t out_stride, int activation, int dtype,
-                           void* workspace, size_t workspace_bytes, stk_stream_t stream);
-size_t stk_matmul_4bit_scatter_workspace_bytes(int64_t slots, int64_t experts, int64_t inputs, int64_t outputs);
+                           int64_t group_size, void* out, int64_t out_stride, int activation, int dtype, stk_stream_t stream);
+size_t stk_matmul_4bit_scatter_workspace_bytes(int64_t slots, int64_t outputs);
 int stk_matmul_4bit_scatter(const void* x, int64_t x_stride, const int32_t* indices, const int32_t* bins, int top_k, int64_t tokens,
                             const float* weights, const void* packed, const void* scales, const void* offsets, int64_t experts,
                             int64_t inputs, int64_t outputs, int64_t group_size, void* out, int64_t out_stride, int dtype,

@@ -79,10 +79,9 @@ SIGNATURES = {
     "stk_quantize_4bit": (_int, [_p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _int, _int, _p]),
     "stk_pack_4bit": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p]),
     "stk_dequantize_4bit": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _int, _p]),
-    "stk_matmul_4bit_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
-    "stk_matmul_4bit": (_int, [_p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _int, _int, _p, _sz, _p]),
-    "stk_gather_matmul_4bit": (_int, [_p, _i64, _i64, _p, _p, _int, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _int, _int, _p, _sz, _p]),
-    "stk_matmul_4bit_scatter_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "stk_matmul_4bit": (_int, [_p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _int, _int, _p]),
+    "stk_gather_matmul_4bit": (_int, [_p, _i64, _i64, _p, _p, _int, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _int, _int, _p]),
+    "stk_matmul_4bit_scatter_workspace_bytes": (_sz, [_i64, _i64]),
     "stk_matmul_4bit_scatter": (_int, [_p, _i64, _p, _p, _int, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _int, _p, _sz, _p]),
     "stk_dsd_scatter": (_int, [_i64, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _i64, _int, _int, _int, _p, _p, _i64, _p]),
 }

@@ -847,10 +847,6 @@ Tensor rows4(const Tensor& x_, const Tensor& scales, int64_t inputs) {
   const Tensor x = x_.detach();
   return inputs == 1 || x.stride(1) == 1 ? x : x.contiguous();
 }
-OptTensor workspace4(size_t bytes, const Tensor& like) {
-  if (bytes == 0) return {};
-  return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
-}
 Tensor matmul_4bit(const Tensor& x_, PACKED_ARGS, int activation) {
   const Packed w(packed, scales, offsets, inputs, outputs, group);
   require(w.experts == 1, "matmul_4bit: the weights of one matrix");
@@ -858,10 +854,8 @@ Tensor matmul_4bit(const Tensor& x_, PACKED_ARGS, int activation) {
   const Tensor x = rows4(x_, scales, inputs);
   const int64_t rows = x.size(0);
   Tensor out = at::empty({rows, outputs}, x.options());
-  const size_t bytes = stk_matmul_4bit_workspace_bytes(rows, 1, inputs, outputs);
-  const OptTensor ws = workspace4(bytes, x);
   check(stk_matmul_4bit(ptr<void>(x), rows, x.stride(0), ptr<void>(packed), ptr<void>(scales), ptr<void>(offsets), inputs, outputs, group, ptr<void>(out), outputs,
-                        activation, value_dtype(x), ptr<void>(ws), bytes, stream_of(x)));
+                        activation, value_dtype(x), stream_of(x)));
   return out;
 }
 void check_routing(const Tensor& indices, const Tensor& bins, const Packed& w, const Tensor& scales) {
@@ -878,11 +872,8 @@ Tensor gather_matmul_4bit(const Tensor& x_, const Tensor& indices, const Tensor&
   const int64_t slots = indices.numel();
   require(top_k >= 1 && x.size(0) * top_k == slots, "one row per token");
   Tensor out = at::empty({slots, outputs}, x.options());
-  const size_t bytes = stk_matmul_4bit_workspace_bytes(slots, w.experts, inputs, outputs);
-  const OptTensor ws = workspace4(bytes, x);
   check(stk_gather_matmul_4bit(ptr<void>(x), x.size(0), x.stride(0), ptr<int32_t>(indices), ptr<int32_t>(bins), top_k, ptr<void>(packed), ptr<void>(scales),
-                               ptr<void>(offsets), w.experts, inputs, outputs, group, ptr<void>(out), outputs, activation, value_dtype(x), ptr<void>(ws), bytes,
-                               stream_of(x)));
+                               ptr<void>(offsets), w.experts, inputs, outputs, group, ptr<void>(out), outputs, activation, value_dtype(x), stream_of(x)));
   return out;
 }
 Tensor matmul_4bit_scatter(const Tensor& x_, const Tensor& indices, const Tensor& bins, int top_k, PACKED_ARGS, const OptTensor& weights) {
@@ -894,8 +885,8 @@ Tensor matmul_4bit_scatter(const Tensor& x_, const Tensor& indices, const Tensor
   require(top_k >= 1 && slots % top_k == 0 && x.size(0) == slots, "one row per slot");
   const OptTensor by_slot = weights32(weights, slots);
   Tensor out = at::empty({slots / top_k, outputs}, x.options());
-  const size_t bytes = stk_matmul_4bit_scatter_workspace_bytes(slots, w.experts, inputs, outputs);
-  const OptTensor ws = workspace4(bytes, x);
+  const size_t bytes = stk_matmul_4bit_scatter_workspace_bytes(slots, outputs);
+  const Tensor ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
   check(stk_matmul_4bit_scatter(ptr<void>(x), x.stride(0), ptr<int32_t>(indices), ptr<int32_t>(bins), top_k, slots / top_k, ptr<float>(by_slot), ptr<void>(packed),
                                 ptr<void>(scales), ptr<void>(offsets), w.experts, inputs, outputs, group, ptr<void>(out), outputs, value_dtype(x), ptr<void>(ws), bytes,
                                 stream_of(x)));

@@ -39,38 +39,39 @@ __global__ __launch_bounds__(256) void quantize_kernel(const typename Value<DTYP
   }
 }
 
-// A wavefront per piece: lane l gathers the 32 codes of its 16 bytes.
-__global__ __launch_bounds__(256) void pack_codes_kernel(const uint8_t* __restrict__ codes, int64_t inputs, int64_t outputs, int64_t pieces, u32x4* __restrict__ packed) {
+// A wavefront per piece: lane l gathers the 32 codes of its 16 bytes.  The eight wavefronts of a workgroup take neighbouring outputs: 128 bytes
+// of each row of codes.
+__global__ __launch_bounds__(512) void pack_codes_kernel(const uint8_t* __restrict__ codes, int64_t inputs, int64_t outputs, int64_t pieces, u32x4* __restrict__ packed) {
   const int lane = threadIdx.x & 63;
-  const int64_t piece = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (piece >= pieces) return;
   const int64_t along = pieces_in(inputs), down = pieces_out(outputs);
-  const int64_t first_i = piece % along * kPieceInputs, first_o = piece / along % down * kPieceOutputs, e = piece / (along * down);
-  const int64_t o = first_o + (lane & 15);
-  uint32_t words[4];
+  for (int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 6); at < pieces; at += (int64_t)gridDim.x * 8) {
+    const int64_t tile = at % down, k = at / down % along, e = at / (down * along);
+    const int64_t first = k * kPieceInputs, o = tile * kPieceOutputs + (lane & 15);
+    uint32_t words[4];
 #pragma unroll
-  for (int d = 0; d < 4; d++) {
-    uint32_t word = 0;
+    for (int d = 0; d < 4; d++) {
+      uint32_t word = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const int64_t i = first_i + 32 * d + 8 * (lane >> 4) + j;
-      const uint32_t code = i < inputs && o < outputs ? codes[(e * inputs + i) * outputs + o] & 15u : 8u;
-      word |= code << (4 * (j >> 1) + 16 * (j & 1));
+      for (int j = 0; j < 8; j++) {
+        const int64_t i = first + 32 * d + 8 * (lane >> 4) + j;
+        const uint32_t code = i < inputs && o < outputs ? codes[(e * inputs + i) * outputs + o] & 15u : 8u;
+        word |= code << (4 * (j >> 1) + 16 * (j & 1));
+      }
+      words[d] = word;
     }
-    words[d] = word;
+    packed[((e * down + tile) * along + k) * 64 + lane] = u32x4{words[0], words[1], words[2], words[3]};
   }
-  packed[piece * 64 + lane] = u32x4{words[0], words[1], words[2], words[3]};
 }
 
 // Scales [expert][group][output] -> the order of weights4.h; the same for offsets.
 __global__ __launch_bounds__(256) void pack_scales_kernel(const uint16_t* __restrict__ scales, int64_t inputs, int64_t outputs, int64_t group, int64_t count,
                                                           uint16_t* __restrict__ packed) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= count) return;
   const int64_t sub = groups_in_block(group), blocks = scale_blocks(inputs, group), groups = groups_of(inputs, group), down = pieces_out(outputs);
-  const int64_t within = at % (16 * sub), block = at / (16 * sub) % blocks, tile = at / (16 * sub) / blocks;
-  const int64_t o = tile % down * 16 + within / (4 * sub) * 4 + within % 4, g = block * sub + within / 4 % sub, e = tile / down;
-  packed[at] = o < outputs && g < groups ? scales[(e * groups + g) * outputs + o] : (uint16_t)0;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < count; at += (int64_t)gridDim.x * 256) {
+    const int64_t within = at % (16 * sub), block = at / (16 * sub) % blocks, tile = at / (16 * sub) / blocks;
+    const int64_t o = tile % down * 16 + within / (4 * sub) * 4 + within % 4, g = block * sub + within / 4 % sub, e = tile / down;
+    packed[at] = o < outputs && g < groups ? scales[(e * groups + g) * outputs + o] : (uint16_t)0;
+  }
 }
 
 template <int DTYPE>
@@ -89,19 +90,9 @@ template <int DTYPE>
 __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* __restrict__ packed, const typename Value<DTYPE>::stored* __restrict__ scales,
                                                          const typename Value<DTYPE>::stored* __restrict__ offsets, int64_t inputs, int64_t outputs,
                                                          int64_t group, int64_t count, typename Value<DTYPE>::stored* __restrict__ out) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= count) return;
-  const int64_t o = at % outputs, i = at / outputs % inputs, e = at / outputs / inputs;
-  out[at] = Value<DTYPE>::round(weight_of<DTYPE>(packed, scales, offsets, e, i, o, inputs, outputs, group));
-}
-
-__device__ __forceinline__ float activated(float v, int kind) {
-  switch (kind) {
-    case kRelu: return activate<kRelu>(v);
-    case kGeluTanh: return activate<kGeluTanh>(v);
-    case kGeluErf: return activate<kGeluErf>(v);
-    case kSilu: return activate<kSilu>(v);
-    default: return v;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < count; at += (int64_t)gridDim.x * 256) {
+    const int64_t o = at % outputs, i = at / outputs % inputs, e = at / outputs / inputs;
+    out[at] = Value<DTYPE>::round(weight_of<DTYPE>(packed, scales, offsets, e, i, o, inputs, outputs, group));
   }
 }
 
@@ -196,9 +187,31 @@ __device__ __forceinline__ u32x4 row_values(const uint16_t* row, int i, int inpu
   return v;
 }
 
+// total = activation(total); the kind is the same for all, so that the functions of many values overlap.
+template <int KIND, int NT, int MT>
+__device__ __forceinline__ void activate_each(f32x4_t (&total)[NT][MT]) {
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) total[n][m][i] = activate<KIND>(total[n][m][i]);
+}
+template <int NT, int MT>
+__device__ __forceinline__ void activate_sums(f32x4_t (&total)[NT][MT], int kind) {
+  switch (kind) {
+    case kRelu: activate_each<kRelu>(total); break;
+    case kGeluTanh: activate_each<kGeluTanh>(total); break;
+    case kGeluErf: activate_each<kGeluErf>(total); break;
+    case kSilu: activate_each<kSilu>(total); break;
+    default: break;
+  }
+}
+
 // The sums of a wavefront: total[n][m][i] belongs to output 16 tile[n] + 4 quarter + i and row 16 m + row of the tile.
 template <bool BF16, int NT, int MT>
-__device__ __forceinline__ void store(const Product4& p, const RowTile& t, const int (&tile)[NT], const f32x4_t (&total)[NT][MT], int row, int quarter) {
+__device__ __forceinline__ void store(const Product4& p, const RowTile& t, const int (&tile)[NT], f32x4_t (&total)[NT][MT], int row, int quarter) {
+  activate_sums(total, p.activation);
 #pragma unroll
   for (int m = 0; m < MT; m++) {
     if (16 * m + row >= t.rows) continue;
@@ -219,9 +232,7 @@ __device__ __forceinline__ void store(const Product4& p, const RowTile& t, const
           for (int i = 0; i < here; i++) at[i] = total[n][m][i];
         continue;
       }
-      float y[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) y[i] = activated(total[n][m][i], p.activation);
+      const f32x4_t y = total[n][m];
       const uint32_t two[2] = {pack2<BF16>(y[0], y[1]), pack2<BF16>(y[2], y[3])};
       uint16_t* at = static_cast<uint16_t*>(p.out) + to * p.out_stride + first;
       if (here == 4) *reinterpret_cast<PairAt2*>(at) = PairAt2{two[0], two[1]};
@@ -483,7 +494,10 @@ __global__ __launch_bounds__(256) void tile_kernel(Product4 p) {
 
 // The same with everything on its way to LDS without registers, a piece of x, codes and scales being multiplied and the next one
 // arriving: rows whose values come in whole 16-byte pieces at multiples of 16 bytes.  What counts is how many wavefronts are on a compute
-// unit (16384 rows over 64 experts, 1024 x 4096: 212 us; three stages of the same 263, the kernel above 314).
+// unit: 16384 rows over 64 experts (1024 x 4096, 137 GFLOP, 302 MB) take 210 us, 655 TFLOP/s, with three pieces on their way 263, through
+// registers (the kernel above) 300; 2048 rows of 4096 x 4096 run at 790.  Vector instructions, of which making numbers of codes is a third,
+// are issued 53 - 70 % of the time and the matrix units are busy 34 % (counters); two of each five MFMAs at 16 rows, one of five at 48 are the
+// sums of x.  Workgroups that walk over tiles, with the next one's first piece on its way, were slower (250).
 static __device__ u32x4 no_values;   // (what lies behind the last input)
 // 16 bytes per lane from any addresses into the LDS bytes from lds_base on, lane after lane.
 __device__ __forceinline__ void dma16_any(const void* from, uint32_t lds_base) {
@@ -588,17 +602,26 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
     const int64_t t = at / across, o = at % across * 4;
     const int here = (int)min(outputs - o, (int64_t)4);
     float v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < top_k; j++) {
-      const int64_t s = t * top_k + j;
-      const float by = weights ? weights[s] : 1.f;
-      const float* from = sums + s * outputs + o;
-      if (here == 4) {
-        const f32x4_t u = __builtin_bit_cast(f32x4_t, *reinterpret_cast<const QuadAt4*>(from));
+    for (int j0 = 0; j0 < top_k; j0 += 4) {   // (the rows of four choices are on their way together)
+      float by[4], u[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = fmaf(by, u[i], v[i]);
-      } else {
-        for (int i = 0; i < here; i++) v[i] = fmaf(by, from[i], v[i]);
+      for (int j = 0; j < 4; j++) {
+        const int64_t s = t * top_k + min(j0 + j, top_k - 1);
+        by[j] = weights ? weights[s] : 1.f;
+        const float* from = sums + s * outputs + o;
+        if (here == 4) {
+          const f32x4_t q = __builtin_bit_cast(f32x4_t, *reinterpret_cast<const QuadAt4*>(from));
+#pragma unroll
+          for (int i = 0; i < 4; i++) u[j][i] = q[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++) u[j][i] = from[min(i, here - 1)];
+        }
       }
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = j0 + j < top_k ? fmaf(by[j], u[j][i], v[i]) : v[i];
     }
     const uint32_t two[2] = {pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3])};
     uint16_t* to = out + t * out_stride + o;
@@ -608,17 +631,23 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
   }
 }
 
+// Workgroups of a kernel that loops over `count` things, `each` of them a workgroup at a time.
+static dim3 loop_grid(int64_t count, int64_t each) {
+  const int64_t groups = (count + each - 1) / each;
+  return dim3((unsigned)(groups < 1 << 18 ? groups : 1 << 18));
+}
+
 static int weights_check(const char* who, int64_t experts, int64_t inputs, int64_t outputs, int64_t group, int dtype) {
   if (dtype != STK_F16 && dtype != STK_BF16) return fail(STK_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
   if (experts < 1 || inputs < 1 || outputs < 1 || group < 1)
     return fail(STK_ERR_DIMS, "%s: %lld experts of %lld x %lld, groups of %lld", who, (long long)experts, (long long)inputs, (long long)outputs, (long long)group);
   if (group != 32 && group != 64 && group % kPieceInputs) return fail(STK_ERR_UNSUPPORTED, "%s: groups of 32, 64 or a multiple of 128 inputs, not %lld", who, (long long)group);
-  if (inputs > INT32_MAX / 2 || outputs > INT32_MAX / 2 || experts > 65535 || pieces_in(inputs) * pieces_out(outputs) * experts > INT32_MAX)
+  if (inputs > 1 << 26 || outputs > 1 << 26 || experts > 65535 || pieces_in(inputs) * pieces_out(outputs) > INT32_MAX / experts)
     return fail(STK_ERR_UNSUPPORTED, "%s: size exceeds 32-bit range", who);
   return STK_OK;
 }
 
-static int product_check(const char* who, const Product4& p, int dtype, int64_t x_rows) {
+static int product_check(const char* who, const Product4& p, int dtype) {
   if (int rc = weights_check(who, p.experts, p.inputs, p.outputs, p.group, dtype)) return rc;
   if (p.rows < 0 || p.rows > INT32_MAX) return fail(STK_ERR_DIMS, "%s: %lld rows", who, (long long)p.rows);
   if (p.activation < 0 || p.activation > kSilu) return fail(STK_ERR_UNSUPPORTED, "%s: activation %d", who, p.activation);
@@ -686,30 +715,32 @@ static void launch_ring(const Product4& p, bool bf16, hipStream_t stream) {
 // Which kernel.  With T tiles of 16 rows and 16 outputs, and pieces along the inputs, the streams want some thousand wavefronts and then
 // as many outputs for one as possible: a fragment of x serves all of them.  Rows in some number share codes instead (ring, or tile
 // where x is no whole 16-byte pieces).  us at T, pieces, in the order of the rule below, KW x NW x NT (bf16, groups of 128, cold):
-//                                   8x1x1  4x1x2  2x2x2  4x1x4  1x4x4     ring, rows x outputs:  16x128  32x128  32x256
+//                                   8x1x1  4x1x2  2x2x2  4x1x4  1x4x4     ring, rows x outputs:  16x128  32x128  48x256
 //   256, 32   (1 row, 4096 x 4096)    7.9    9.9   14.3   12.4   24.5
-//   512, 32   (32 rows, the same)    13.9   11.3   15.4   13.6   28.5                             21.7    25.9    39.7
-//   1024, 32  (64 rows)              21.8   15.6   15.8   13.9   29.3                             22.0    26.2    39.9
-//   4096, 32  (256 rows)             69.8   43.0   43.7   32.4   31.3                             27.7    27.5    40.0
-//   2048, 8   (16 rows, 8 experts, 1024 x 4096) 19.8 10.5 10.4 10.9 13.8                          11.0    12.0    16.2
+//   512, 32   (32 rows, the same)    13.9   11.3   15.4   13.6   28.5                             21.7    25.9
+//   1024, 32  (64 rows)              21.8   15.6   15.8   13.9   29.3                             22.0    26.2
+//   4096, 32  (256 rows)             69.8   43.0   43.7   32.4   31.3                             27.7    27.5
+//   2048, 8   (16 rows, 8 experts, 1024 x 4096) 19.8 10.5 10.4 10.9 13.8                          11.0    12.0
 //   6144, 8   (32 rows, 24 of 64 experts)       52.9 22.0 19.5 24.6 19.2
-//   16384, 8  (256 rows, 64 experts) 144    50.8   40.8   56.7   34.4                             35.1    37.9    40.4
-//   4096, 32  (256 rows, 64 experts, 4096 x 1024) 65.0 44.5 43.8 40.6 42.8                        40.8    45.4    49.4
-//   (512 rows over 8 experts, 1024 x 4096)                                                        19.1    18.4    21.9
-//   (2048 rows over 64 experts)                                                                   57.9    53.2    50.2
-//   (16384 rows over 64 experts)                                                                  --     237     212
+//   16384, 8  (256 rows, 64 experts) 144    50.8   40.8   56.7   34.4                             35.1    37.9
+//   4096, 32  (256 rows, 64 experts, 4096 x 1024) 65.0 44.5 43.8 40.6 42.8                        40.8    45.4
+//   (512 rows over 8 experts, 1024 x 4096)                                                        19.1    18.4
+//   (2048 rows over 64 experts)                                                                   56.6    51.1    46.1
+//   (16384 rows over 64 experts)                                                                  312     234     210
+//   (8192 rows over 64 experts, 4096 x 1024, groups of 64 with offsets)                           180     137     149
+// (64 x 256 needs more registers than two workgroups of a compute unit have: 270 us on the 16384 rows.)
 static int launch_product(const char* who, const Product4& p, int dtype, hipStream_t stream) {
   const bool bf16 = dtype == STK_BF16;
   if (most_tiles(p, 16) > (int64_t)65535 * 65535) return fail(STK_ERR_UNSUPPORTED, "%s: %lld rows", who, (long long)p.rows);
   const int64_t along = pieces_in(p.inputs), down = pieces_out(p.outputs);
   // as if the rows were spread evenly over the experts: where they really are only the device knows
   const int64_t hit = p.experts < p.rows ? p.experts : p.rows, each = (p.rows + hit - 1) / hit;
-  const int64_t tiles = hit * ((each + 15) / 16) * down, across8 = (down + 7) / 8, across16 = (down + 15) / 16, tall = hit * ((each + 31) / 32);
+  const int64_t tiles = hit * ((each + 15) / 16) * down, across8 = (down + 7) / 8, across16 = (down + 15) / 16;
   if (along >= 24 ? each > 16 && tiles > 3000 : each >= 8 && tiles >= 1536) {
     const bool whole = p.inputs % 8 == 0 && p.x_stride % 8 == 0 && aligned16(p.x);
     if (!whole) launch_tiles<2, 2>(p, bf16, stream);
-    else if (each >= 24 && tall * across16 >= 512) launch_ring<4, 2>(p, bf16, stream);
-    else if (each >= 12 && tall * across8 >= 256) launch_ring<2, 2>(p, bf16, stream);
+    else if (p.group >= kPieceInputs && each >= 24 && hit * ((each + 47) / 48) * across16 >= 512) launch_ring<4, 3>(p, bf16, stream);
+    else if (each >= 12 && hit * ((each + 31) / 32) * across8 >= 256) launch_ring<2, 2>(p, bf16, stream);
     else launch_ring<2, 1>(p, bf16, stream);
   } else if (tiles <= 320) launch_stream<8, 1, 1>(p, bf16, stream);
   else if (tiles <= 640) launch_stream<4, 1, 2>(p, bf16, stream);
@@ -761,11 +792,11 @@ extern "C" int stk_pack_4bit(const uint8_t* codes, const void* scales, const voi
   if (!aligned16(packed)) return fail(STK_ERR_UNSUPPORTED, "%s: packed weights at a multiple of 16 bytes", who);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t pieces = experts * pieces_in(inputs) * pieces_out(outputs), count = stk_4bit_scales(experts, inputs, outputs, group_size);
-  hipLaunchKernelGGL(pack_codes_kernel, dim3((unsigned)((pieces + 3) / 4)), dim3(256), 0, s, codes, inputs, outputs, pieces, static_cast<u32x4*>(packed));
-  hipLaunchKernelGGL(pack_scales_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, s, static_cast<const uint16_t*>(scales), inputs, outputs, group_size, count,
+  hipLaunchKernelGGL(pack_codes_kernel, loop_grid(pieces, 8), dim3(512), 0, s, codes, inputs, outputs, pieces, static_cast<u32x4*>(packed));
+  hipLaunchKernelGGL(pack_scales_kernel, loop_grid(count, 256), dim3(256), 0, s, static_cast<const uint16_t*>(scales), inputs, outputs, group_size, count,
                      static_cast<uint16_t*>(packed_scales));
   if (offsets)
-    hipLaunchKernelGGL(pack_scales_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, s, static_cast<const uint16_t*>(offsets), inputs, outputs, group_size, count,
+    hipLaunchKernelGGL(pack_scales_kernel, loop_grid(count, 256), dim3(256), 0, s, static_cast<const uint16_t*>(offsets), inputs, outputs, group_size, count,
                        static_cast<uint16_t*>(packed_offsets));
   return check_launch(who);
 }
@@ -778,7 +809,7 @@ extern "C" int stk_dequantize_4bit(const void* packed, const void* scales, const
   const int64_t count = experts * inputs * outputs;
   const auto launch = [&](auto d) {
     typedef typename Value<d()>::stored T;
-    hipLaunchKernelGGL((dequantize_kernel<d()>), dim3((unsigned)((count + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream),
+    hipLaunchKernelGGL((dequantize_kernel<d()>), loop_grid(count, 256), dim3(256), 0, static_cast<hipStream_t>(stream),
                        static_cast<const uint8_t*>(packed), static_cast<const T*>(scales), static_cast<const T*>(offsets), inputs, outputs, group_size, count,
                        static_cast<T*>(out));
   };
@@ -787,14 +818,12 @@ extern "C" int stk_dequantize_4bit(const void* packed, const void* scales, const
   return check_launch(who);
 }
 
-extern "C" size_t stk_matmul_4bit_workspace_bytes(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs) { return 0; }
-
 extern "C" int stk_matmul_4bit(const void* x, int64_t rows, int64_t x_stride, const void* packed, const void* scales, const void* offsets, int64_t inputs,
-                               int64_t outputs, int64_t group_size, void* out, int64_t out_stride, int activation, int dtype, void*, size_t, stk_stream_t stream) {
+                               int64_t outputs, int64_t group_size, void* out, int64_t out_stride, int activation, int dtype, stk_stream_t stream) {
   const char* who = "stk_matmul_4bit";
   const Product4 p = {x, x_stride, rows, static_cast<const uint8_t*>(packed), scales, offsets, 1, inputs, outputs, group_size, nullptr, nullptr, 0,
                       out, out_stride, nullptr, activation};
-  if (int rc = product_check(who, p, dtype, rows)) return rc;
+  if (int rc = product_check(who, p, dtype)) return rc;
   if (rows == 0) return STK_OK;
   if (int rc = launch_product(who, p, dtype, static_cast<hipStream_t>(stream))) return rc;
   return check_launch(who);
@@ -802,19 +831,19 @@ extern "C" int stk_matmul_4bit(const void* x, int64_t rows, int64_t x_stride, co
 
 extern "C" int stk_gather_matmul_4bit(const void* x, int64_t tokens, int64_t x_stride, const int32_t* indices, const int32_t* bins, int top_k, const void* packed,
                                       const void* scales, const void* offsets, int64_t experts, int64_t inputs, int64_t outputs, int64_t group_size, void* out,
-                                      int64_t out_stride, int activation, int dtype, void*, size_t, stk_stream_t stream) {
+                                      int64_t out_stride, int activation, int dtype, stk_stream_t stream) {
   const char* who = "stk_gather_matmul_4bit";
-  if (tokens < 0 || top_k < 1) return fail(STK_ERR_DIMS, "%s: %lld tokens, top_k %d", who, (long long)tokens, top_k);
+  if (tokens < 0 || top_k < 1 || tokens > INT32_MAX / top_k) return fail(STK_ERR_DIMS, "%s: %lld tokens, top_k %d", who, (long long)tokens, top_k);
   const Product4 p = {x, x_stride, tokens * top_k, static_cast<const uint8_t*>(packed), scales, offsets, experts, inputs, outputs, group_size, indices, bins, top_k,
                       out, out_stride, nullptr, activation};
-  if (int rc = product_check(who, p, dtype, tokens)) return rc;
+  if (int rc = product_check(who, p, dtype)) return rc;
   if (tokens == 0) return STK_OK;
   if (!indices || !bins) return fail(STK_ERR_DIMS, "%s: missing pointer", who);
   if (int rc = launch_product(who, p, dtype, static_cast<hipStream_t>(stream))) return rc;
   return check_launch(who);
 }
 
-extern "C" size_t stk_matmul_4bit_scatter_workspace_bytes(int64_t slots, int64_t experts, int64_t inputs, int64_t outputs) {
+extern "C" size_t stk_matmul_4bit_scatter_workspace_bytes(int64_t slots, int64_t outputs) {
   return slots < 1 || outputs < 1 ? 0 : (size_t)(slots * outputs) * sizeof(float);
 }
 
@@ -823,19 +852,18 @@ extern "C" int stk_matmul_4bit_scatter(const void* x, int64_t x_stride, const in
                                        int64_t outputs, int64_t group_size, void* out, int64_t out_stride, int dtype, void* workspace, size_t workspace_bytes,
                                        stk_stream_t stream) {
   const char* who = "stk_matmul_4bit_scatter";
-  if (tokens < 0 || top_k < 1) return fail(STK_ERR_DIMS, "%s: %lld tokens, top_k %d", who, (long long)tokens, top_k);
+  if (tokens < 0 || top_k < 1 || tokens > INT32_MAX / top_k) return fail(STK_ERR_DIMS, "%s: %lld tokens, top_k %d", who, (long long)tokens, top_k);
   const int64_t slots = tokens * top_k;
   const Product4 p = {x, x_stride, slots, static_cast<const uint8_t*>(packed), scales, offsets, experts, inputs, outputs, group_size, indices, bins, 0,
                       nullptr, 0, static_cast<float*>(workspace), 0};
-  if (slots > 0 && (!workspace || workspace_bytes < stk_matmul_4bit_scatter_workspace_bytes(slots, experts, inputs, outputs)))
-    return fail(STK_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", who, stk_matmul_4bit_scatter_workspace_bytes(slots, experts, inputs, outputs));
-  if (int rc = product_check(who, p, dtype, slots)) return rc;
+  if (slots > 0 && (!workspace || workspace_bytes < stk_matmul_4bit_scatter_workspace_bytes(slots, outputs)))
+    return fail(STK_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", who, stk_matmul_4bit_scatter_workspace_bytes(slots, outputs));
+  if (int rc = product_check(who, p, dtype)) return rc;
   if (tokens == 0) return STK_OK;
   if (!indices || !bins || !out || out_stride < outputs) return fail(STK_ERR_DIMS, "%s: missing pointer", who);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (int rc = launch_product(who, p, dtype, s)) return rc;
-  const int64_t groups = (tokens * ((outputs + 3) / 4) + 255) / 256;
-  const dim3 grid((unsigned)(groups < 65536 ? groups : 65536));
+  const dim3 grid = loop_grid(tokens * ((outputs + 3) / 4), 256);
   const auto combine = dtype == STK_BF16 ? combine_kernel<true> : combine_kernel<false>;
   hipLaunchKernelGGL(combine, grid, dim3(256), 0, s, static_cast<const float*>(workspace), weights, tokens, top_k, outputs, static_cast<uint16_t*>(out), out_stride);
   return check_launch(who);

@@ -8,7 +8,7 @@ from collections import namedtuple
 
 import torch
 
-from stk_amd.backend import hip_kernels
+from stk_amd.backend import autocast, hip_kernels
 from stk_amd.backend.autograd import applies
 
 # packed, scales, offsets (or None): device tensors in the layout of the products, [experts, ...]; experts: None for a single matrix
@@ -22,6 +22,11 @@ def _batched(t, dims):
 def _no_gradient(*tensors):
     if applies(*tensors):
         raise NotImplementedError("stk_amd: 4-bit weights are for inference: their products have no gradient and are not traced or transformed")
+
+
+def _operand(x):
+    """x as the products of this package see it: under autocast in its type."""
+    return x.to(torch.get_autocast_gpu_dtype()) if autocast.casts(x) else x
 
 
 @torch.no_grad()
@@ -55,9 +60,10 @@ def dequantize_4bit(w):
 
 def matmul_4bit(x, w, activation=None):
     """activation(x @ w) for x [..., inputs] of w's type and a single matrix w; the activations are those of stk.ops.sdd_fused, applied to the
-    fp32 sums.  Inference only: raises where x needs a gradient."""
+    fp32 sums.  Under autocast x is cast to its type like the operands of the other products.  Inference only: raises where x needs a gradient."""
     assert isinstance(w, Weights4) and w.experts is None
     _no_gradient(x)
+    x = _operand(x)
     rows = x if x.dim() == 2 else x.reshape(-1, x.size(-1))
     out = hip_kernels.matmul_4bit(rows, w.packed, w.scales, w.offsets, w.inputs, w.outputs, w.group_size, activation)
     return out if x.dim() == 2 else out.view(*x.shape[:-1], w.outputs)
@@ -68,7 +74,7 @@ def gather_matmul_4bit(x, route, w, activation=None):
     route.indices (by expert, without padding, whatever blocking the routing was made with).  Inference only."""
     assert isinstance(w, Weights4) and w.experts is not None
     _no_gradient(x)
-    return hip_kernels.gather_matmul_4bit(x, route.indices, route.bins, route.top_k, w.packed, w.scales, w.offsets, w.inputs, w.outputs, w.group_size,
+    return hip_kernels.gather_matmul_4bit(_operand(x), route.indices, route.bins, route.top_k, w.packed, w.scales, w.offsets, w.inputs, w.outputs, w.group_size,
                                           activation)
 
 
@@ -78,5 +84,5 @@ def matmul_4bit_scatter(x, route, w, weights=None):
     once.  Inference only."""
     assert isinstance(w, Weights4) and w.experts is not None
     _no_gradient(x, weights)
-    return hip_kernels.matmul_4bit_scatter(x, route.indices, route.bins, route.top_k, w.packed, w.scales, w.offsets, w.inputs, w.outputs, w.group_size,
+    return hip_kernels.matmul_4bit_scatter(_operand(x), route.indices, route.bins, route.top_k, w.packed, w.scales, w.offsets, w.inputs, w.outputs, w.group_size,
                                            weights)

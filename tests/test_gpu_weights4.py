@@ -338,3 +338,22 @@ def test_values_behind_the_last_input_are_not_used():
         wide[:, :100] = torch.randn(rows, 100, generator=torch.Generator().manual_seed(rows)).to(DEV)
         assert torch.equal(stk.ops.matmul_4bit(wide[:, :100], w), stk.ops.matmul_4bit(wide[:, :100].contiguous(), w))
         assert torch.isfinite(stk.ops.matmul_4bit(wide[:, :100], w)).all()
+
+
+def test_autocast_and_inference_mode():
+    """Under autocast rows of another type are cast like those of the other products; without it they are refused."""
+    codes, scales, _ = _weights((2, 128, 48), 64, False, torch.bfloat16, 12)
+    w = _pack(codes, scales, None, 64)
+    one = _pack(codes[0], scales[0], None, 64)
+    x = torch.randn(6, 128, generator=torch.Generator().manual_seed(13)).to(DEV)
+    r = stk.ops.route(torch.tensor([0, 1, 1, 0, 1, 0], dtype=torch.int32, device=DEV).view(6, 1), 2, 1)
+    back = _pack(codes.transpose(1, 2).contiguous(), scales[:, :1, :1].expand(2, 1, 128).contiguous(), None, 64)
+    near = x.bfloat16()
+    for layer in (lambda x: stk.ops.matmul_4bit(x, one), lambda x: stk.ops.matmul_4bit_scatter(stk.ops.gather_matmul_4bit(x, r, w), r, back)):
+        want = layer(near)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            assert torch.equal(layer(x), want)
+        with torch.inference_mode():
+            assert torch.equal(layer(near), want)
+        with pytest.raises(NotImplementedError):
+            layer(x)

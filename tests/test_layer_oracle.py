@@ -125,7 +125,7 @@ def test_abi_refusals_and_sizes_of_4bit_weights():
     # whole pieces of 128 inputs, whole blocks of the groups of a piece, 16 outputs
     assert lib.stk_4bit_scales(3, 129, 17, 32) == 3 * 8 * 32 and lib.stk_4bit_scales(1, 128, 16, 256) == 16
     mm = lambda group=128, dtype=_lib.STK_BF16, act=0, x=one, out_stride=16, packed=one: lib.stk_matmul_4bit(
-        x, 4, 128, packed, one, None, 128, 16, group, one, out_stride, act, dtype, None, 0, None)
+        x, 4, 128, packed, one, None, 128, 16, group, one, out_stride, act, dtype, None)
     _bad(mm(group=48), _lib.STK_ERR_UNSUPPORTED, "groups of 32, 64 or a multiple of 128")
     _bad(mm(group=0), _lib.STK_ERR_DIMS, "groups of 0")
     _bad(mm(dtype=_lib.STK_F32), _lib.STK_ERR_UNSUPPORTED, "dtype 2")
@@ -133,9 +133,9 @@ def test_abi_refusals_and_sizes_of_4bit_weights():
     _bad(mm(x=None), _lib.STK_ERR_DIMS, "missing pointer")
     _bad(mm(out_stride=15), _lib.STK_ERR_DIMS, "strides")
     _bad(mm(packed=ctypes.c_void_p(264)), _lib.STK_ERR_UNSUPPORTED, "multiples of 16 bytes")
-    _bad(lib.stk_gather_matmul_4bit(one, 4, 128, None, one, 2, one, one, None, 4, 128, 16, 128, one, 16, 0, _lib.STK_BF16, one, 1 << 40, None), _lib.STK_ERR_DIMS,
+    _bad(lib.stk_gather_matmul_4bit(one, 4, 128, None, one, 2, one, one, None, 4, 128, 16, 128, one, 16, 0, _lib.STK_BF16, None), _lib.STK_ERR_DIMS,
          "missing pointer")
-    _bad(lib.stk_gather_matmul_4bit(one, 4, 128, one, one, 0, one, one, None, 4, 128, 16, 128, one, 16, 0, _lib.STK_BF16, one, 1 << 40, None), _lib.STK_ERR_DIMS, "top_k 0")
+    _bad(lib.stk_gather_matmul_4bit(one, 4, 128, one, one, 0, one, one, None, 4, 128, 16, 128, one, 16, 0, _lib.STK_BF16, None), _lib.STK_ERR_DIMS, "top_k 0")
     _bad(lib.stk_matmul_4bit_scatter(one, 128, one, one, 2, 4, None, one, one, None, 4, 128, 16, 128, one, 16, _lib.STK_BF16, None, 0, None), _lib.STK_ERR_WORKSPACE,
          "workspace")
     _bad(lib.stk_pack_4bit(one, one, one, 1, 128, 16, 128, one, one, None, None), _lib.STK_ERR_DIMS, "missing pointer")
