@@ -295,8 +295,12 @@ struct Stage {
 };
 
 // Few rows: KW wavefronts share the inputs of NW x NT x 16 outputs and up to 16 rows of one expert, a piece of weights at a time; their sums meet
-// in LDS.  Two pieces are on their way at a time (three or four: the same or slower, registers cost wavefronts).  SUB: groups of a piece whose sums are scaled apart (4, 2 or 1: groups of 32, 64, more).
-// Rows beyond those of the tile are read from its first one: what they give stays in columns that are not stored.
+// in LDS.  Two pieces are on their way at a time (three or four: the same or slower, registers cost wavefronts).  SUB: groups of a piece whose
+// sums are scaled apart (4, 2 or 1: groups of 32, 64, more).  Rows beyond those of the tile are read from its first one: what they give
+// stays in columns that are not stored.
+// Bound by the bytes of the weights where many experts are hit (16 tokens, top 2, 64 experts of 1024 x 4096: 121 MB in 26.1 us, 4.65 TB/s of the
+// 5.16 of a copy; of 4096 x 1024 with the sum over the choices 30.8, two launches), and by the launch and one trip to memory for a single row
+// (4096 x 4096, 8.7 MB: 5.3 us).
 template <bool BF16, bool AFFINE, int SUB, int KW, int NW, int NT>
 __global__ __launch_bounds__(64 * KW * NW) void stream_kernel(Product4 p) {
   constexpr int MT = 1, DEPTH = 2;
@@ -494,10 +498,12 @@ __global__ __launch_bounds__(256) void tile_kernel(Product4 p) {
 
 // The same with everything on its way to LDS without registers, a piece of x, codes and scales being multiplied and the next one
 // arriving: rows whose values come in whole 16-byte pieces at multiples of 16 bytes.  What counts is how many wavefronts are on a compute
-// unit: 16384 rows over 64 experts (1024 x 4096, 137 GFLOP, 302 MB) take 210 us, 655 TFLOP/s, with three pieces on their way 263, through
-// registers (the kernel above) 300; 2048 rows of 4096 x 4096 run at 790.  Vector instructions, of which making numbers of codes is a third,
-// are issued 53 - 70 % of the time and the matrix units are busy 34 % (counters); two of each five MFMAs at 16 rows, one of five at 48 are the
-// sums of x.  Workgroups that walk over tiles, with the next one's first piece on its way, were slower (250).
+// unit: 16384 rows over 64 experts (1024 x 4096, 137 GFLOP, 302 MB) take 205 - 228 us from one device to the next, 600 - 670 TFLOP/s, with
+// three pieces on their way 263, through registers (the kernel above) 300; 2048 rows of 4096 x 4096 run at 790.  Vector instructions, of which
+// making numbers of codes is a third, are issued 53 - 70 % of the time and the matrix units are busy 34 % (counters); one MFMA of five at 64
+// outputs a wavefront, one of three at 32, is for the sums of x.  What is lost at the ends of a tile shows in short rows of inputs: the rate
+// with 1024 is three quarters of that with 4096.  A raised priority of the wavefronts while they multiply changed nothing; workgroups that
+// walk over tiles, with the next one's first piece on its way, were slower (250).
 static __device__ u32x4 no_values;   // (what lies behind the last input)
 // 16 bytes per lane from any addresses into the LDS bytes from lds_base on, lane after lane.
 __device__ __forceinline__ void dma16_any(const void* from, uint32_t lds_base) {
@@ -725,9 +731,16 @@ static void launch_ring(const Product4& p, bool bf16, hipStream_t stream) {
 //   16384, 8  (256 rows, 64 experts) 144    50.8   40.8   56.7   34.4                             35.1    37.9
 //   4096, 32  (256 rows, 64 experts, 4096 x 1024) 65.0 44.5 43.8 40.6 42.8                        40.8    45.4
 //   (512 rows over 8 experts, 1024 x 4096)                                                        19.1    18.4
-//   (2048 rows over 64 experts)                                                                   56.6    51.1    46.1
-//   (16384 rows over 64 experts)                                                                  312     234     210
-//   (8192 rows over 64 experts, 4096 x 1024, groups of 64 with offsets)                           180     137     149
+// and with many rows, another time                                             ring, rows x outputs:  16x128  32x128  48x128  32x256  48x256
+//   2048 rows over 64 experts, 1024 x 4096                                                             56      51      50      47      46
+//   16384 rows over 64 experts, 1024 x 4096                                                            312     240     231     227     231
+//   the same with groups of 64                                                                         334     251     241     228     233
+//   the same with offsets                                                                              364     257     258     264     242
+//   the same with offsets and groups of 64                                                             411     293     285     308     283
+//   8192 rows over 64 experts, 4096 x 1024                                                             138     120     127     111     121
+//   the same with offsets                                                                              160     132     129     135     132
+//   the same with offsets and groups of 64                                                                     140             154     153
+//   512, 1000, 2048 rows, 4096 x 4096                                                     40, 68, 123   33, 52, 92  40, 53, 93  37, 52, 87  40, 61, 89
 // (64 x 256 needs more registers than two workgroups of a compute unit have: 270 us on the 16384 rows.)
 static int launch_product(const char* who, const Product4& p, int dtype, hipStream_t stream) {
   const bool bf16 = dtype == STK_BF16;
@@ -739,7 +752,8 @@ static int launch_product(const char* who, const Product4& p, int dtype, hipStre
   if (along >= 24 ? each > 16 && tiles > 3000 : each >= 8 && tiles >= 1536) {
     const bool whole = p.inputs % 8 == 0 && p.x_stride % 8 == 0 && aligned16(p.x);
     if (!whole) launch_tiles<2, 2>(p, bf16, stream);
-    else if (p.group >= kPieceInputs && each >= 24 && hit * ((each + 47) / 48) * across16 >= 512) launch_ring<4, 3>(p, bf16, stream);
+    else if (!p.offsets && p.group >= 64 && each >= 24 && hit * ((each + 31) / 32) * across16 >= 512) launch_ring<4, 2>(p, bf16, stream);
+    else if (p.offsets && p.group >= kPieceInputs && each >= 24 && hit * ((each + 47) / 48) * across16 >= 512) launch_ring<4, 3>(p, bf16, stream);
     else if (each >= 12 && hit * ((each + 31) / 32) * across8 >= 256) launch_ring<2, 2>(p, bf16, stream);
     else launch_ring<2, 1>(p, bf16, stream);
   } else if (tiles <= 320) launch_stream<8, 1, 1>(p, bf16, stream);

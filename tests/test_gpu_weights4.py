@@ -137,7 +137,7 @@ def test_product(rows, inputs, outputs, group, affine, dtype):
 
 # one size for every kernel that the launch rule chooses from; inputs of no multiple of eight take the way through registers
 BY_RULE = [(2100, 392, 2050, 128), (2100, 395, 2050, 32), (530, 264, 2048, 64), (530, 257, 2048, 128), (200, 136, 2050, 32), (200, 3080, 2050, 128), (550, 3080, 2050, 64),
-           (40, 520, 2050, 128), (9, 300, 12001, 64), (3, 3080, 11000, 128)]
+           (40, 520, 2050, 128), (9, 300, 12001, 64), (3, 3080, 11000, 128), (3300, 264, 2050, 128)]
 
 
 @pytest.mark.parametrize("dtype,affine", [(torch.bfloat16, False), (torch.float16, True)])
