@@ -54,9 +54,7 @@ __device__ __forceinline__ T moved_key(T v) {
 template <class T>
 __device__ __forceinline__ T larger(T a, T b) { return a > b ? a : b; }
 
-// A token belongs to a team of 16 or 64 lanes, V experts a lane: neighbours, which are one access, where that fills the team, otherwise
-// every 16th or 64th, so that the lanes' single accesses lie next to each other (16384 x 1000 float32 scores, neighbours
-// throughout: backward 90 us, 22 so; forward 39, 30).
+// The largest of a team's keys, in every lane.
 template <int LANES, class T>
 __device__ __forceinline__ T team_max(T v) {
   v = larger(v, moved_key<0xb1>(v)), v = larger(v, moved_key<0x4e>(v)), v = larger(v, moved_key<0x141>(v)), v = larger(v, moved_key<0x140>(v));
@@ -84,6 +82,9 @@ __device__ __forceinline__ float exponential(float x) {
   return t < -149.f ? 0.f : fmaf(y, rest * kLn2, y);   // (below every fp32 number, also for x = -infinity, which makes NaN of the rest)
 }
 
+// A token belongs to a team of 16 or 64 lanes, V experts a lane: neighbours, which are one access, where that fills the team, otherwise
+// every 16th or 64th, so that the lanes' single accesses lie next to each other (16384 x 1000 float32 scores, neighbours
+// throughout: backward 90 us, 22 so; forward 39, 30).
 template <int DTYPE, int LANES, int V>
 __global__ __launch_bounds__(256) void top_experts_kernel(const typename Value<DTYPE>::stored* __restrict__ scores, int64_t stride, int64_t tokens, int experts,
                                                           int top_k, int normalize, int32_t* __restrict__ chosen, float* __restrict__ weights) {
@@ -241,7 +242,7 @@ static int router_check(const char* who, int64_t tokens, int64_t experts, int to
   if (tokens < 0 || experts < 1 || top_k < 1 || top_k > experts)
     return fail(STK_ERR_DIMS, "%s: the top %d of %lld experts, %lld tokens", who, top_k, (long long)experts, (long long)tokens);
   if (experts > kRouterExperts || top_k > kRouterTopK) return fail(STK_ERR_UNSUPPORTED, "%s: at most %d experts, the top %d", who, kRouterExperts, kRouterTopK);
-  if (tokens * top_k > INT32_MAX) return fail(STK_ERR_UNSUPPORTED, "%s: size exceeds 32-bit range", who);
+  if (tokens > INT32_MAX / top_k) return fail(STK_ERR_UNSUPPORTED, "%s: size exceeds 32-bit range", who);
   return STK_OK;
 }
 

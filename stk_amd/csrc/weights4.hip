@@ -298,9 +298,9 @@ struct Stage {
 // in LDS.  Two pieces are on their way at a time (three or four: the same or slower, registers cost wavefronts).  SUB: groups of a piece whose
 // sums are scaled apart (4, 2 or 1: groups of 32, 64, more).  Rows beyond those of the tile are read from its first one: what they give
 // stays in columns that are not stored.
-// Bound by the bytes of the weights where many experts are hit (16 tokens, top 2, 64 experts of 1024 x 4096: 121 MB in 26.1 us, 4.65 TB/s of the
-// 5.16 of a copy; of 4096 x 1024 with the sum over the choices 30.8, two launches), and by the launch and one trip to memory for a single row
-// (4096 x 4096, 8.7 MB: 5.3 us).
+// Bound by the bytes of the weights where many experts are hit (64 tokens, top 2 of 64 experts of 1024 x 4096: 121 MB in 26.1 us,
+// 4.65 TB/s of the 5.16 of a copy; of 4096 x 1024 with the sum over the choices 30.8, two launches), and by the launch and one trip to
+// memory for a single row (4096 x 4096, 8.7 MB: 5.3 us).
 template <bool BF16, bool AFFINE, int SUB, int KW, int NW, int NT>
 __global__ __launch_bounds__(64 * KW * NW) void stream_kernel(Product4 p) {
   constexpr int MT = 1, DEPTH = 2;
@@ -496,14 +496,15 @@ __global__ __launch_bounds__(256) void tile_kernel(Product4 p) {
   store<BF16>(p, t, tile, total, row, quarter);
 }
 
-// The same with everything on its way to LDS without registers, a piece of x, codes and scales being multiplied and the next one
-// arriving: rows whose values come in whole 16-byte pieces at multiples of 16 bytes.  What counts is how many wavefronts are on a compute
-// unit: 16384 rows over 64 experts (1024 x 4096, 137 GFLOP, 302 MB) take 205 - 228 us from one device to the next, 600 - 670 TFLOP/s, with
-// three pieces on their way 263, through registers (the kernel above) 300; 2048 rows of 4096 x 4096 run at 790.  Vector instructions, of which
-// making numbers of codes is a third, are issued 53 - 70 % of the time and the matrix units are busy 34 % (counters); one MFMA of five at 64
-// outputs a wavefront, one of three at 32, is for the sums of x.  What is lost at the ends of a tile shows in short rows of inputs: the rate
-// with 1024 is three quarters of that with 4096.  A raised priority of the wavefronts while they multiply changed nothing; workgroups that
-// walk over tiles, with the next one's first piece on its way, were slower (250).
+// The same with everything on its way to LDS without registers, the next piece of x arriving while one is multiplied, codes and scales
+// (each wavefront reads its own) in one place that is filled again once they are in registers: rows whose values come in whole 16-byte pieces
+// at multiples of 16 bytes.  What counts is how many wavefronts are on a compute unit: 16384 rows over 64 experts (1024 x 4096, 137 GFLOP,
+// 302 MB) take 223 us, 615 TFLOP/s, with three workgroups of 32 x 256 on a unit, 242 with two of 48 x 256, 245 and 266 (48 x 256, 32 x 256)
+// in the case of offsets with two stages of codes, 238 so; 263 with three pieces on their way, 300 through registers (the kernel above); 2048
+// rows of 4096 x 4096 run at 790.  Vector instructions, of which making numbers of codes is a half, are issued three quarters of the time and
+// the matrix units are busy 35 % (counters); one MFMA of five at 64 outputs a wavefront, one of three at 32, is for the sums of x.  What is lost
+// at the ends of a tile shows in short rows of inputs: the rate with 1024 is three quarters of that with 4096.  A raised priority of the wavefronts
+// while they multiply is worth 2 % either way; workgroups that walk over tiles, with the next one's first piece on its way, were slower (250).
 static __device__ u32x4 no_values;   // (what lies behind the last input)
 // 16 bytes per lane from any addresses into the LDS bytes from lds_base on, lane after lane.
 __device__ __forceinline__ void dma16_any(const void* from, uint32_t lds_base) {
@@ -511,13 +512,13 @@ __device__ __forceinline__ void dma16_any(const void* from, uint32_t lds_base) {
 }
 template <int NT, int MT>
 struct Stage16 {
-  static constexpr int kRows = MT * 4096, kCodes = 4 * NT * 1024, kScales = 4 * 512;   // bytes of a stage
-  static constexpr int bytes(bool affine) { return kRows + kCodes + (affine ? 2 : 1) * kScales; }
+  static constexpr int kRows = MT * 4096, kCodes = 4 * NT * 1024, kScales = 4 * 512;   // bytes
+  static constexpr int bytes(bool affine) { return 2 * kRows + kCodes + (affine ? 2 : 1) * kScales; }
 };
 template <bool BF16, bool AFFINE, int SUB, int NT, int MT>
-__global__ __launch_bounds__(256, 2) void ring_kernel(Product4 p) {
+__global__ __launch_bounds__(256, 3) void ring_kernel(Product4 p) {
   typedef Stage16<NT, MT> R;
-  constexpr int kStage = R::bytes(AFFINE);
+  constexpr int kPrivate = 2 * R::kRows;
   extern __shared__ char smem[];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const RowTile t = row_tile<16 * MT>(p, (int)(blockIdx.z * gridDim.y + blockIdx.y), lane);
@@ -550,21 +551,24 @@ __global__ __launch_bounds__(256, 2) void ring_kernel(Product4 p) {
   const int mine = min(((int)blockIdx.x * 4 + wave) * NT + lane / (2 * SUB), down - 1);
   const int64_t scale_from = ((int64_t)t.expert * down + mine) * blocks * (32 * SUB) + lane % (2 * SUB) * 16;
   const uint32_t lds = (uint32_t)(uintptr_t)(STK_LDS char*)smem;
-  const auto issue = [&](int piece, int stage) {
-    const uint32_t to = lds + stage * kStage;
+  const auto issue_rows = [&](int piece, int stage) {
+    const uint32_t to = lds + stage * R::kRows;
     const bool last = (piece + 1) * kPieceInputs > p.inputs;
-#pragma unroll
-    for (int n = 0; n < NT; n++) dma16(weights[n] + (int64_t)piece * kPieceBytes, lane * 16, to + R::kRows + (wave * NT + n) * 1024);
 #pragma unroll
     for (int m = 0; m < MT; m++) {
       const char* from = x[m] + (int64_t)piece * (2 * kPieceInputs);
       if (last && piece * kPieceInputs + first_input[m] >= p.inputs) from = reinterpret_cast<const char*>(&no_values);
       dma16_any(from, to + (m * 4 + wave) * 1024);
     }
+  };
+  const auto issue_codes = [&](int piece) {
+    const uint32_t to = lds + kPrivate;
+#pragma unroll
+    for (int n = 0; n < NT; n++) dma16(weights[n] + (int64_t)piece * kPieceBytes, lane * 16, to + (wave * NT + n) * 1024);
     if (lane < NT * 2 * SUB) {
       const int64_t at = scale_from + (int64_t)(SUB > 1 || per_block == 1 ? piece : piece / per_block) * (32 * SUB);
-      dma16_any(static_cast<const char*>(p.scales) + at, to + R::kRows + R::kCodes + wave * 512);
-      if constexpr (AFFINE) dma16_any(static_cast<const char*>(p.offsets) + at, to + R::kRows + R::kCodes + R::kScales + wave * 512);
+      dma16_any(static_cast<const char*>(p.scales) + at, to + R::kCodes + wave * 512);
+      if constexpr (AFFINE) dma16_any(static_cast<const char*>(p.offsets) + at, to + R::kCodes + R::kScales + wave * 512);
     }
   };
   const Decoder<BF16> numbers;
@@ -573,23 +577,28 @@ __global__ __launch_bounds__(256, 2) void ring_kernel(Product4 p) {
   for (int n = 0; n < NT; n++)
 #pragma unroll
     for (int m = 0; m < MT; m++) total[n][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  issue(0, 0);
+  issue_codes(0), issue_rows(0, 0);
   for (int piece = 0; piece < along; piece++) {
     wait_vmcnt<0>();
     __syncthreads();   // everybody's part of the piece is there, and everybody is done with the one whose place is filled now
-    if (piece + 1 < along) issue(piece + 1, (piece + 1) & 1);
-    const char* from = smem + (piece & 1) * kStage;
+    if (piece + 1 < along) issue_rows(piece + 1, (piece + 1) & 1);
+    const char *from = smem + (piece & 1) * R::kRows, *own = smem + kPrivate;
     u32x4 w[NT];
     u32x2 s[NT][SUB], o[NT][AFFINE ? SUB : 1];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-      w[n] = reinterpret_cast<const u32x4*>(from + R::kRows + (wave * NT + n) * 1024)[lane];
+      w[n] = reinterpret_cast<const u32x4*>(own + (wave * NT + n) * 1024)[lane];
 #pragma unroll
       for (int k = 0; k < SUB; k++) {
-        s[n][k] = reinterpret_cast<const u32x2*>(from + R::kRows + R::kCodes + wave * 512 + n * 32 * SUB)[quarter * SUB + k];
-        if constexpr (AFFINE) o[n][k] = reinterpret_cast<const u32x2*>(from + R::kRows + R::kCodes + R::kScales + wave * 512 + n * 32 * SUB)[quarter * SUB + k];
+        s[n][k] = reinterpret_cast<const u32x2*>(own + R::kCodes + wave * 512 + n * 32 * SUB)[quarter * SUB + k];
+        if constexpr (AFFINE) o[n][k] = reinterpret_cast<const u32x2*>(own + R::kCodes + R::kScales + wave * 512 + n * 32 * SUB)[quarter * SUB + k];
       }
     }
+    // a wavefront's codes and scales are its own: once they are in registers the next ones may arrive in their place
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+#pragma unroll
+    for (int n = 0; n < NT; n++) asm volatile("" : "+v"(w[n]));
+    if (piece + 1 < along) issue_codes(piece + 1);
     const u32x4* values = reinterpret_cast<const u32x4*>(from);
 #pragma unroll
     for (int k = 0; k < SUB; k++)
@@ -710,7 +719,7 @@ static void launch_tiles(const Product4& p, bool bf16, hipStream_t stream) {
 template <int NT, int MT>
 static void launch_ring(const Product4& p, bool bf16, hipStream_t stream) {
   for_form(p, bf16, [&](auto type, auto affine, auto sub) {
-    constexpr int lds = 2 * Stage16<NT, MT>::bytes(decltype(affine)::value);
+    constexpr int lds = Stage16<NT, MT>::bytes(decltype(affine)::value);
     const auto kernel = ring_kernel<decltype(type)::value, decltype(affine)::value, decltype(sub)::value, NT, MT>;
     set_lds_limit(kernel, lds);
     const int64_t across = (pieces_out(p.outputs) + 4 * NT - 1) / (4 * NT);
@@ -731,16 +740,16 @@ static void launch_ring(const Product4& p, bool bf16, hipStream_t stream) {
 //   16384, 8  (256 rows, 64 experts) 144    50.8   40.8   56.7   34.4                             35.1    37.9
 //   4096, 32  (256 rows, 64 experts, 4096 x 1024) 65.0 44.5 43.8 40.6 42.8                        40.8    45.4
 //   (512 rows over 8 experts, 1024 x 4096)                                                        19.1    18.4
-// and with many rows, another time                                             ring, rows x outputs:  16x128  32x128  48x128  32x256  48x256
-//   2048 rows over 64 experts, 1024 x 4096                                                             56      51      50      47      46
-//   16384 rows over 64 experts, 1024 x 4096                                                            312     240     231     227     231
-//   the same with groups of 64                                                                         334     251     241     228     233
-//   the same with offsets                                                                              364     257     258     264     242
-//   the same with offsets and groups of 64                                                             411     293     285     308     283
-//   8192 rows over 64 experts, 4096 x 1024                                                             138     120     127     111     121
-//   the same with offsets                                                                              160     132     129     135     132
-//   the same with offsets and groups of 64                                                                     140             154     153
-//   512, 1000, 2048 rows, 4096 x 4096                                                     40, 68, 123   33, 52, 92  40, 53, 93  37, 52, 87  40, 61, 89
+// and with many rows, another time                                             ring, rows x outputs:         32x128  48x128  32x256  48x256
+//   2048 rows over 64 experts, 1024 x 4096                                                                     52      50      47      47
+//   16384 rows over 64 experts, 1024 x 4096                                                                    238     230     223     243
+//   the same with groups of 64                                                                                 241     225     219     223
+//   the same with offsets                                                                                      257     255     238     253
+//   the same with offsets and groups of 64                                                                     298     292     275     275
+//   the same with groups of 32, and with offsets                                                               269, 363        273, 357
+//   8192 rows over 64 experts, 4096 x 1024                                                                     120     125     110     122
+//   the same with offsets                                                                                      131     129     121     135
+//   512, 1000, 2048 rows, 4096 x 4096                                                                          33, 52, 90  40, 52, 92  37, 51, 87  41, 62, 91
 // (64 x 256 needs more registers than two workgroups of a compute unit have: 270 us on the 16384 rows.)
 static int launch_product(const char* who, const Product4& p, int dtype, hipStream_t stream) {
   const bool bf16 = dtype == STK_BF16;
@@ -752,8 +761,7 @@ static int launch_product(const char* who, const Product4& p, int dtype, hipStre
   if (along >= 24 ? each > 16 && tiles > 3000 : each >= 8 && tiles >= 1536) {
     const bool whole = p.inputs % 8 == 0 && p.x_stride % 8 == 0 && aligned16(p.x);
     if (!whole) launch_tiles<2, 2>(p, bf16, stream);
-    else if (!p.offsets && p.group >= 64 && each >= 24 && hit * ((each + 31) / 32) * across16 >= 512) launch_ring<4, 2>(p, bf16, stream);
-    else if (p.offsets && p.group >= kPieceInputs && each >= 24 && hit * ((each + 47) / 48) * across16 >= 512) launch_ring<4, 3>(p, bf16, stream);
+    else if (each >= 24 && hit * ((each + 31) / 32) * across16 >= 512) launch_ring<4, 2>(p, bf16, stream);
     else if (each >= 12 && hit * ((each + 31) / 32) * across8 >= 256) launch_ring<2, 2>(p, bf16, stream);
     else launch_ring<2, 1>(p, bf16, stream);
   } else if (tiles <= 320) launch_stream<8, 1, 1>(p, bf16, stream);
