@@ -57,7 +57,7 @@ __global__ __launch_bounds__(512) void pack_codes_kernel(const uint8_t* __restri
         const uint32_t code = i < inputs && o < outputs ? codes[(e * inputs + i) * outputs + o] & 15u : 8u;
         word |= code << (4 * (j >> 1) + 16 * (j & 1));
       }
-      words[d] = word;
+      words[d] = word << kCodesTurn | word >> (32 - kCodesTurn);
     }
     packed[((e * down + tile) * along + k) * 64 + lane] = u32x4{words[0], words[1], words[2], words[3]};
   }
@@ -78,9 +78,7 @@ template <int DTYPE>
 __device__ __forceinline__ float weight_of(const uint8_t* packed, const typename Value<DTYPE>::stored* scales, const typename Value<DTYPE>::stored* offsets,
                                            int64_t e, int64_t i, int64_t o, int64_t inputs, int64_t outputs, int64_t group) {
   const int64_t along = pieces_in(inputs), down = pieces_out(outputs);
-  int byte, shift;
-  code_at((int)(o & 15), (int)(i & 127), &byte, &shift);
-  const int code = packed[((e * down + o / 16) * along + i / 128) * kPieceBytes + byte] >> shift & 15;
+  const int code = code_of(reinterpret_cast<const uint32_t*>(packed + ((e * down + o / 16) * along + i / 128) * kPieceBytes), (int)(o & 15), (int)(i & 127));
   const int64_t at = scale_at(e * down + o / 16, (int)(o & 15), i / group, inputs, group);
   const float scale = Value<DTYPE>::widen(scales[at]);
   return offsets ? scale * (float)code + Value<DTYPE>::widen(offsets[at]) : scale * (float)(code - 8);
@@ -116,16 +114,16 @@ struct Product4 {
 // A code becomes the 16-bit number 16 + code: its four bits at the top of the mantissa of a number between 16 and 32.  A group's
 // products are then sums over x (16 + code), and the sums over x that are too much, -24 x (the code's zero at 8) or -16 x (with
 // offsets), are what the accumulator starts from: a product of x with a constant operand, shared by all outputs.  The group's scale
-// multiplies the fp32 sum.  That makes 8 instructions for eight weights and one for a group's four outputs, below half of
+// multiplies the fp32 sum.  That makes 7 instructions for eight weights (8 in float16) and one for a group's four outputs, below half of
 // what a stream of weights at memory speed leaves time for.
 template <bool BF16> struct Codes;
 template <> struct Codes<true> {
   static constexpr uint32_t mask = 0x00780078u, magic = 0x41804180u, minus24 = 0xc1c0c1c0u, minus16 = 0xc180c180u;
-  static __device__ __forceinline__ uint32_t placed(uint32_t w, int p) { return p == 0 ? w << 3 : w >> (4 * p - 3); }
+  static __device__ __forceinline__ uint32_t placed(uint32_t w, int p) { return p == 0 ? w : p == 3 ? __builtin_amdgcn_alignbit(w, w, 12) : w >> (4 * p); }
 };
 template <> struct Codes<false> {
   static constexpr uint32_t mask = 0x03c003c0u, magic = 0x4c004c00u, minus24 = 0xce00ce00u, minus16 = 0xcc00cc00u;
-  static __device__ __forceinline__ uint32_t placed(uint32_t w, int p) { return p == 0 ? w << 6 : p == 1 ? w << 2 : w >> (4 * p - 6); }
+  static __device__ __forceinline__ uint32_t placed(uint32_t w, int p) { return p == 0 ? w << 3 : p == 3 ? __builtin_amdgcn_alignbit(w, w, 9) : w >> (4 * p - 3); }
 };
 // The mask and the magic number in registers that the compiler takes for variables: with constants it makes two instructions of an
 // and-or, which has no room for two literals.
@@ -297,12 +295,13 @@ struct Stage {
 // Few rows: KW wavefronts share the inputs of NW x NT x 16 outputs and up to 16 rows of one expert, a piece of weights at a time; their sums meet
 // in LDS.  Two pieces are on their way at a time (three or four: the same or slower, registers cost wavefronts).  SUB: groups of a piece whose
 // sums are scaled apart (4, 2 or 1: groups of 32, 64, more).  Rows beyond those of the tile are read from its first one: what they give
-// stays in columns that are not stored.
+// stays in columns that are not stored.  The 2 of the launch bounds keeps the compiler from accumulation registers, which it would take beside
+// 130 others: two wavefronts instead of three (4x1x4 on the 128 slots of 64 experts of 4096 x 1024: 31.5 us, 29.6 so).
 // Bound by the bytes of the weights where many experts are hit (64 tokens, top 2 of 64 experts of 1024 x 4096: 121 MB in 26.1 us,
-// 4.65 TB/s of the 5.16 of a copy; of 4096 x 1024 with the sum over the choices 30.8, two launches), and by the launch and one trip to
+// 4.65 TB/s of the 5.16 of a copy; of 4096 x 1024 with the sum over the choices 29.5, two launches), and by the launch and one trip to
 // memory for a single row (4096 x 4096, 8.7 MB: 5.3 us).
 template <bool BF16, bool AFFINE, int SUB, int KW, int NW, int NT>
-__global__ __launch_bounds__(64 * KW * NW) void stream_kernel(Product4 p) {
+__global__ __launch_bounds__(64 * KW * NW, 2) void stream_kernel(Product4 p) {
   constexpr int MT = 1, DEPTH = 2;
   extern __shared__ f32x4_t shared[];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), kw = wave % KW, nw = wave / KW;
@@ -499,8 +498,8 @@ __global__ __launch_bounds__(256) void tile_kernel(Product4 p) {
 // The same with everything on its way to LDS without registers, the next piece of x arriving while one is multiplied, codes and scales
 // (each wavefront reads its own) in one place that is filled again once they are in registers: rows whose values come in whole 16-byte pieces
 // at multiples of 16 bytes.  What counts is how many wavefronts are on a compute unit: 16384 rows over 64 experts (1024 x 4096, 137 GFLOP,
-// 302 MB) take 223 us, 615 TFLOP/s, with three workgroups of 32 x 256 on a unit, 242 with two of 48 x 256, 245 and 266 (48 x 256, 32 x 256)
-// in the case of offsets with two stages of codes, 238 so; 263 with three pieces on their way, 300 through registers (the kernel above); 2048
+// 302 MB) take 216 - 223 us, 615 - 635 TFLOP/s, with three workgroups of 32 x 256 on a unit, 242 with two of 48 x 256; in the case of offsets
+// 266 with two stages of codes, 238 so; 263 with three pieces on their way, 300 through registers (the kernel above); 2048
 // rows of 4096 x 4096 run at 790.  Vector instructions, of which making numbers of codes is a half, are issued three quarters of the time and
 // the matrix units are busy 35 % (counters); one MFMA of five at 64 outputs a wavefront, one of three at 32, is for the sums of x.  What is lost
 // at the ends of a tile shows in short rows of inputs: the rate with 1024 is three quarters of that with 4096.  A raised priority of the wavefronts
@@ -730,26 +729,26 @@ static void launch_ring(const Product4& p, bool bf16, hipStream_t stream) {
 // Which kernel.  With T tiles of 16 rows and 16 outputs, and pieces along the inputs, the streams want some thousand wavefronts and then
 // as many outputs for one as possible: a fragment of x serves all of them.  Rows in some number share codes instead (ring, or tile
 // where x is no whole 16-byte pieces).  us at T, pieces, in the order of the rule below, KW x NW x NT (bf16, groups of 128, cold):
-//                                   8x1x1  4x1x2  2x2x2  4x1x4  1x4x4     ring, rows x outputs:  16x128  32x128  48x256
-//   256, 32   (1 row, 4096 x 4096)    7.9    9.9   14.3   12.4   24.5
-//   512, 32   (32 rows, the same)    13.9   11.3   15.4   13.6   28.5                             21.7    25.9
-//   1024, 32  (64 rows)              21.8   15.6   15.8   13.9   29.3                             22.0    26.2
-//   4096, 32  (256 rows)             69.8   43.0   43.7   32.4   31.3                             27.7    27.5
-//   2048, 8   (16 rows, 8 experts, 1024 x 4096) 19.8 10.5 10.4 10.9 13.8                          11.0    12.0
-//   6144, 8   (32 rows, 24 of 64 experts)       52.9 22.0 19.5 24.6 19.2
-//   16384, 8  (256 rows, 64 experts) 144    50.8   40.8   56.7   34.4                             35.1    37.9
-//   4096, 32  (256 rows, 64 experts, 4096 x 1024) 65.0 44.5 43.8 40.6 42.8                        40.8    45.4
-//   (512 rows over 8 experts, 1024 x 4096)                                                        19.1    18.4
-// and with many rows, another time                                             ring, rows x outputs:         32x128  48x128  32x256  48x256
-//   2048 rows over 64 experts, 1024 x 4096                                                                     52      50      47      47
-//   16384 rows over 64 experts, 1024 x 4096                                                                    238     230     223     243
-//   the same with groups of 64                                                                                 241     225     219     223
-//   the same with offsets                                                                                      257     255     238     253
-//   the same with offsets and groups of 64                                                                     298     292     275     275
-//   the same with groups of 32, and with offsets                                                               269, 363        273, 357
-//   8192 rows over 64 experts, 4096 x 1024                                                                     120     125     110     122
-//   the same with offsets                                                                                      131     129     121     135
-//   512, 1000, 2048 rows, 4096 x 4096                                                                          33, 52, 90  40, 52, 92  37, 51, 87  41, 62, 91
+//                                             8x1x1  4x1x2  2x2x2  4x1x4  1x4x4   ring, rows x outputs:  16x128  32x128  32x256
+//   256, 32   (1 row, 4096 x 4096)              6.9    9.2   12.0   11.1   23.0                            20.5    24.8    33.9
+//   512, 32   (32 rows, the same)              14.0   10.8   15.0   12.6   27.6                            20.2    25.0    34.5
+//   1024, 32  (64 rows)                        22.3   15.2   15.2   12.8   27.6                            20.6    25.0    34.4
+//   4096, 32  (256 rows)                       72.7   43.3   42.2   29.9   28.6                            25.8    25.2    34.3
+//   2048, 8   (16 rows, 8 experts, 1024 x 4096) 19.4  10.0    9.7   10.2   12.0                            10.6    11.6    14.4
+//   7168, 8   (28 rows for 28 of 64 experts)   52.4   21.6   18.1   19.0   17.1                            15.3    17.1    18.9
+//   16384, 8  (256 rows, 64 experts)            140   48.7   38.8   41.4   31.2                            32.2    38.4    39.7
+//   4096, 32  (256 rows, 64 experts, 4096 x 1024) 55.8 34.2  35.6   30.6   31.3                            38.9    39.9    39.1
+//   (512 rows over 8 experts, 1024 x 4096)      102   33.7   29.3   26.4   24.0                            18.3    17.3    19.4
+// and with many rows (other times on other devices: 3 % apart)              ring, rows x outputs:     32x128  48x128  32x256  48x256
+//   2048 rows over 64 experts, 1024 x 4096                                                            52      50      47      47
+//   16384 rows over 64 experts, 1024 x 4096                                                           235     230     216     243
+//   the same with groups of 64                                                                        245     225     222     223
+//   the same with offsets                                                                             255     255     238     253
+//   the same with offsets and groups of 64                                                            290     292     279     275
+//   the same with groups of 32, and with offsets                                                      269, 363        273, 357
+//   8192 rows over 64 experts, 4096 x 1024                                                            119     125     109     122
+//   the same with offsets                                                                             130     129     119     135
+//   512, 1000, 2048 rows, 4096 x 4096                                                                 33, 51, 92      36, 50, 86
 // (64 x 256 needs more registers than two workgroups of a compute unit have: 270 us on the 16384 rows.)
 static int launch_product(const char* who, const Product4& p, int dtype, hipStream_t stream) {
   const bool bf16 = dtype == STK_BF16;
@@ -828,6 +827,7 @@ extern "C" int stk_dequantize_4bit(const void* packed, const void* scales, const
   const char* who = "stk_dequantize_4bit";
   if (int rc = weights_check(who, experts, inputs, outputs, group_size, dtype)) return rc;
   if (!packed || !scales || !out) return fail(STK_ERR_DIMS, "%s: missing pointer", who);
+  if (!aligned16(packed)) return fail(STK_ERR_UNSUPPORTED, "%s: packed weights at a multiple of 16 bytes", who);
   const int64_t count = experts * inputs * outputs;
   const auto launch = [&](auto d) {
     typedef typename Value<d()>::stored T;
