@@ -776,7 +776,7 @@ std::tuple<Tensor, Tensor, OptTensor> quantize_4bit(const Tensor& w_, int64_t gr
   const Tensor w = w_.detach();
   require(w.dim() == 3 && group >= 1, "quantize_4bit: weights are [inputs, outputs] or [experts, inputs, outputs], in groups of inputs");
   const c10::DeviceGuard guard(w.device());
-  const int64_t experts = w.size(0), inputs = w.size(1), outputs = w.size(2), groups = (inputs + group - 1) / group;
+  const int64_t experts = w.size(0), inputs = w.size(1), outputs = w.size(2), groups = inputs / group + (inputs % group != 0);
   Tensor codes = at::empty({experts, inputs, outputs}, w.options().dtype(at::kByte)), scales = at::empty({experts, groups, outputs}, w.options().dtype(dtype));
   OptTensor offsets;
   if (with_offsets) offsets = at::empty_like(scales);
@@ -790,7 +790,7 @@ std::tuple<Tensor, Tensor, OptTensor> pack_4bit(const Tensor& codes_, const Tens
   require(codes_.dim() == 3 && scales_.dim() == 3 && group >= 1, "pack_4bit: codes [experts, inputs, outputs], scales [experts, groups, outputs]");
   if (codes_.scalar_type() != at::kByte) raise(PyExc_NotImplementedError, std::string("stk_amd: 4-bit codes are uint8, one a byte, got ") + c10::toString(codes_.scalar_type()));
   const c10::DeviceGuard guard(codes_.device());
-  const int64_t experts = codes_.size(0), inputs = codes_.size(1), outputs = codes_.size(2), groups = (inputs + group - 1) / group;
+  const int64_t experts = codes_.size(0), inputs = codes_.size(1), outputs = codes_.size(2), groups = inputs / group + (inputs % group != 0);
   require(scales_.size(0) == experts && scales_.size(1) == groups && scales_.size(2) == outputs && scales_.device() == codes_.device(),
           "pack_4bit: one scale per group of inputs and output");
   if (scales_.scalar_type() != at::kHalf && scales_.scalar_type() != at::kBFloat16)

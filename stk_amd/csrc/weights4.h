@@ -21,6 +21,9 @@ __host__ __device__ inline int64_t pieces_out(int64_t outputs) { return (outputs
 __host__ __device__ inline int64_t groups_of(int64_t inputs, int64_t group) { return (inputs + group - 1) / group; }
 __host__ __device__ inline int64_t groups_in_block(int64_t group) { return group < kPieceInputs ? kPieceInputs / group : 1; }
 __host__ __device__ inline int64_t scale_blocks(int64_t inputs, int64_t group) { return (groups_of(inputs, group) + groups_in_block(group) - 1) / groups_in_block(group); }
+// Every multiple of 128 from the inputs on means one group of them all.  What is below the C ABI sees the smallest such size: the kernels
+// count a group's pieces in 32 bits, and the sums above are not to overflow.
+inline int64_t group_within(int64_t inputs, int64_t group) { return group % kPieceInputs == 0 && group >= inputs ? pieces_in(inputs) * kPieceInputs : group; }
 // Where the scale of output o (0 .. 15) of the tile-th 16 outputs and group g is.
 __host__ __device__ inline int64_t scale_at(int64_t tile, int o, int64_t g, int64_t inputs, int64_t group) {
   const int64_t sub = groups_in_block(group);

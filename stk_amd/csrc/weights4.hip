@@ -651,17 +651,19 @@ static dim3 loop_grid(int64_t count, int64_t each) {
   return dim3((unsigned)(groups < 1 << 18 ? groups : 1 << 18));
 }
 
-static int weights_check(const char* who, int64_t experts, int64_t inputs, int64_t outputs, int64_t group, int dtype) {
+// (leaves the group in the kernels' terms)
+static int weights_check(const char* who, int64_t experts, int64_t inputs, int64_t outputs, int64_t& group, int dtype) {
   if (dtype != STK_F16 && dtype != STK_BF16) return fail(STK_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
   if (experts < 1 || inputs < 1 || outputs < 1 || group < 1)
     return fail(STK_ERR_DIMS, "%s: %lld experts of %lld x %lld, groups of %lld", who, (long long)experts, (long long)inputs, (long long)outputs, (long long)group);
   if (group != 32 && group != 64 && group % kPieceInputs) return fail(STK_ERR_UNSUPPORTED, "%s: groups of 32, 64 or a multiple of 128 inputs, not %lld", who, (long long)group);
   if (inputs > 1 << 26 || outputs > 1 << 26 || experts > 65535 || pieces_in(inputs) * pieces_out(outputs) > INT32_MAX / experts)
     return fail(STK_ERR_UNSUPPORTED, "%s: size exceeds 32-bit range", who);
+  group = group_within(inputs, group);
   return STK_OK;
 }
 
-static int product_check(const char* who, const Product4& p, int dtype) {
+static int product_check(const char* who, Product4& p, int dtype) {
   if (int rc = weights_check(who, p.experts, p.inputs, p.outputs, p.group, dtype)) return rc;
   if (p.rows < 0 || p.rows > INT32_MAX) return fail(STK_ERR_DIMS, "%s: %lld rows", who, (long long)p.rows);
   if (p.activation < 0 || p.activation > kSilu) return fail(STK_ERR_UNSUPPORTED, "%s: activation %d", who, p.activation);
@@ -779,7 +781,9 @@ extern "C" int64_t stk_4bit_packed_bytes(int64_t experts, int64_t inputs, int64_
   return experts < 1 || inputs < 1 || outputs < 1 ? 0 : experts * pieces_in(inputs) * pieces_out(outputs) * kPieceBytes;
 }
 extern "C" int64_t stk_4bit_scales(int64_t experts, int64_t inputs, int64_t outputs, int64_t group_size) {
-  return experts < 1 || inputs < 1 || outputs < 1 || group_size < 1 ? 0 : experts * scale_blocks(inputs, group_size) * groups_in_block(group_size) * pieces_out(outputs) * kPieceOutputs;
+  if (experts < 1 || inputs < 1 || outputs < 1 || group_size < 1) return 0;
+  const int64_t group = group_within(inputs, group_size);
+  return experts * scale_blocks(inputs, group) * groups_in_block(group) * pieces_out(outputs) * kPieceOutputs;
 }
 
 extern "C" int stk_quantize_4bit(const void* w, int64_t stride_e, int64_t stride_i, int64_t stride_o, int64_t experts, int64_t inputs, int64_t outputs,
@@ -843,7 +847,7 @@ extern "C" int stk_dequantize_4bit(const void* packed, const void* scales, const
 extern "C" int stk_matmul_4bit(const void* x, int64_t rows, int64_t x_stride, const void* packed, const void* scales, const void* offsets, int64_t inputs,
                                int64_t outputs, int64_t group_size, void* out, int64_t out_stride, int activation, int dtype, stk_stream_t stream) {
   const char* who = "stk_matmul_4bit";
-  const Product4 p = {x, x_stride, rows, static_cast<const uint8_t*>(packed), scales, offsets, 1, inputs, outputs, group_size, nullptr, nullptr, 0,
+  Product4 p = {x, x_stride, rows, static_cast<const uint8_t*>(packed), scales, offsets, 1, inputs, outputs, group_size, nullptr, nullptr, 0,
                       out, out_stride, nullptr, activation};
   if (int rc = product_check(who, p, dtype)) return rc;
   if (rows == 0) return STK_OK;
@@ -856,7 +860,7 @@ extern "C" int stk_gather_matmul_4bit(const void* x, int64_t tokens, int64_t x_s
                                       int64_t out_stride, int activation, int dtype, stk_stream_t stream) {
   const char* who = "stk_gather_matmul_4bit";
   if (tokens < 0 || top_k < 1 || tokens > INT32_MAX / top_k) return fail(STK_ERR_DIMS, "%s: %lld tokens, top_k %d", who, (long long)tokens, top_k);
-  const Product4 p = {x, x_stride, tokens * top_k, static_cast<const uint8_t*>(packed), scales, offsets, experts, inputs, outputs, group_size, indices, bins, top_k,
+  Product4 p = {x, x_stride, tokens * top_k, static_cast<const uint8_t*>(packed), scales, offsets, experts, inputs, outputs, group_size, indices, bins, top_k,
                       out, out_stride, nullptr, activation};
   if (int rc = product_check(who, p, dtype)) return rc;
   if (tokens == 0) return STK_OK;
@@ -876,7 +880,7 @@ extern "C" int stk_matmul_4bit_scatter(const void* x, int64_t x_stride, const in
   const char* who = "stk_matmul_4bit_scatter";
   if (tokens < 0 || top_k < 1 || tokens > INT32_MAX / top_k) return fail(STK_ERR_DIMS, "%s: %lld tokens, top_k %d", who, (long long)tokens, top_k);
   const int64_t slots = tokens * top_k;
-  const Product4 p = {x, x_stride, slots, static_cast<const uint8_t*>(packed), scales, offsets, experts, inputs, outputs, group_size, indices, bins, 0,
+  Product4 p = {x, x_stride, slots, static_cast<const uint8_t*>(packed), scales, offsets, experts, inputs, outputs, group_size, indices, bins, 0,
                       nullptr, 0, static_cast<float*>(workspace), 0};
   if (slots > 0 && (!workspace || workspace_bytes < stk_matmul_4bit_scatter_workspace_bytes(slots, outputs)))
     return fail(STK_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", who, stk_matmul_4bit_scatter_workspace_bytes(slots, outputs));
