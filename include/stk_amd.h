@@ -672,7 +672,9 @@ int stk_dequantize_4bit(const void* packed, const void* scales, const void* offs
  *   stk_matmul_4bit_scatter   out[t] = sum over j < top_k, in that order, of weights[s] * (x[p] w[e]), s = t * top_k + j = indices[p]
  *                             (weights NULL: ones; x has a row for each sorted position).  The sums stay fp32 up to the one
  *                             rounding.
- * A row of x with an infinity, a NaN or sums of more than 2^120 gives NaN throughout its result.  Weights of experts without rows are not read.  workspace:
+ * A row of x with an infinity or a NaN gives NaN throughout its result, whatever the activation (the codes are multiplied as numbers up
+ * to 31, and what is too much is taken off: an infinity cannot be).  Sums of |x| over a group up to 2^123 do not overflow on the way.
+ * Weights of experts without rows are not read.  workspace:
  * stk_matmul_4bit_scatter_workspace_bytes(tokens * top_k, outputs) bytes, 16-byte aligned, nothing in it is read before it is written.
  */
 int stk_matmul_4bit(const void* x, int64_t rows, int64_t x_stride, const void* packed, const void* scales, const void* offsets,

@@ -185,7 +185,8 @@ __device__ __forceinline__ u32x4 row_values(const uint16_t* row, int i, int inpu
   return v;
 }
 
-// total = activation(total); the kind is the same for all, so that the functions of many values overlap.
+// total = activation(total); the kind is the same for all, so that the functions of many values overlap.  A sum that is NaN stays one: an
+// infinity among the rows is NaN here, and relu by the comparison with 0 from the other side would make 0 of it.
 template <int KIND, int NT, int MT>
 __device__ __forceinline__ void activate_each(f32x4_t (&total)[NT][MT]) {
 #pragma unroll
@@ -193,7 +194,10 @@ __device__ __forceinline__ void activate_each(f32x4_t (&total)[NT][MT]) {
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) total[n][m][i] = activate<KIND>(total[n][m][i]);
+      for (int i = 0; i < 4; i++) {
+        const float v = total[n][m][i];
+        total[n][m][i] = KIND == kRelu ? (v <= 0.f ? 0.f : v) : activate<KIND>(v);
+      }
 }
 template <int NT, int MT>
 __device__ __forceinline__ void activate_sums(f32x4_t (&total)[NT][MT], int kind) {

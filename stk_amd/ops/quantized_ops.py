@@ -60,7 +60,8 @@ def dequantize_4bit(w):
 
 def matmul_4bit(x, w, activation=None):
     """activation(x @ w) for x [..., inputs] of w's type and a single matrix w; the activations are those of stk.ops.sdd_fused, applied to the
-    fp32 sums.  Under autocast x is cast to its type like the operands of the other products.  Inference only: raises where x needs a gradient."""
+    fp32 sums.  A row with an infinity or a NaN gives NaN throughout, here and in the products below.  Under autocast x is cast to its type
+    like the operands of the other products.  Inference only: raises where x needs a gradient."""
     assert isinstance(w, Weights4) and w.experts is None
     _no_gradient(x)
     x = _operand(x)
