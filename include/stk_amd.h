@@ -649,7 +649,9 @@ int stk_top_experts_backward(const void* scores, int64_t stride, const int32_t* 
  * codes 0 .. 15 (one a byte, [experts, inputs, outputs]), scales and offsets of STK_F16 / STK_BF16 [experts, groups, outputs], groups =
  * ceil(inputs / group_size); group_size 32, 64 or a multiple of 128 (one group: any such multiple that is not below inputs).
  * stk_quantize_4bit makes them from weights w (element strides; of w_dtype, the scales' type or STK_F32): scale = round(max |w| / 7), or
- * with offsets scale = round((max - min) / 15) and offset = round(min), then the nearest codes.
+ * with offsets scale = round((max - min) / 15) and offset = round(min), then the nearest codes.  A group with a NaN, or whose scale or offset
+ * is infinite in fp32 or once rounded (an infinite weight, or one too large for the scales' type), gets a scale of NaN, which makes NaN of
+ * its weights and of the products with them.
  * stk_pack_4bit lays them out for the products, once: stk_4bit_packed_bytes bytes, 16-byte aligned, of codes and stk_4bit_scales
  * 16-bit elements of scales and of offsets, whose order is the library's own.  stk_dequantize_4bit writes the weights
  * [experts, inputs, outputs] that a packed form stands for, each rounded once.  Packed arrays start at multiples of 16 bytes.  No counterpart in the reference.

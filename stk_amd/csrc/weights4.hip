@@ -11,7 +11,8 @@
 namespace stk {
 
 // Largest and smallest weight of a group -> scale and offset, rounded to the weights' type; then the codes nearest to the weights
-// under the rounded ones.  A thread per group and output.
+// under the rounded ones.  A group with a NaN, or whose rounded scale or offset is no finite number, has a scale of NaN: minimum and
+// maximum pass over a NaN, and an infinite scale would make codes of 0 of every weight.  A thread per group and output.
 template <int DTYPE, int OUT>
 __global__ __launch_bounds__(256) void quantize_kernel(const typename Value<DTYPE>::stored* __restrict__ w, int64_t stride_e, int64_t stride_i, int64_t stride_o,
                                                        int64_t inputs, int64_t outputs, int64_t group, int64_t groups, uint8_t* __restrict__ codes,
@@ -22,12 +23,16 @@ __global__ __launch_bounds__(256) void quantize_kernel(const typename Value<DTYP
     const int64_t lo = g * group, hi = lo + group < inputs ? lo + group : inputs;
     const auto* at = w + e * stride_e + o * stride_o;
     float least = INFINITY, most = -INFINITY;
+    bool finite = true;
     for (int64_t i = lo; i < hi; i++) {
       const float v = Value<DTYPE>::widen(at[i * stride_i]);
       least = fminf(least, v), most = fmaxf(most, v);
+      finite = finite && v == v;
     }
-    const auto scale16 = Value<OUT>::round(offsets ? (most - least) / 15.f : fmaxf(most, -least) / 7.f);
+    auto scale16 = Value<OUT>::round(offsets ? (most - least) / 15.f : fmaxf(most, -least) / 7.f);
     const auto offset16 = Value<OUT>::round(least);
+    finite = finite && Value<OUT>::widen(scale16) < INFINITY && !(offsets && fabsf(Value<OUT>::widen(offset16)) == INFINITY);
+    if (!finite) scale16 = Value<OUT>::round(NAN);
     const float scale = Value<OUT>::widen(scale16), from = offsets ? Value<OUT>::widen(offset16) : -8.f * scale;
     const int64_t to = (e * groups + g) * outputs + o;
     scales[to] = scale16;

@@ -44,7 +44,8 @@ def quantize_4bit(weights, group_size=128, offsets=False, dtype=None):
     """Weights4 nearest to weights [inputs, outputs] or [experts, inputs, outputs] (any strides: the experts' slices of
     [inputs, experts * outputs] are weights.view(inputs, experts, outputs).transpose(0, 1)).
 
-    offsets=False: scale = max |w| of a group / 7.  offsets=True: scale = (max - min) / 15 and the smallest weight as the offset.  dtype:
+    offsets=False: scale = max |w| of a group / 7.  offsets=True: scale = (max - min) / 15 and the smallest weight as the offset.  A group
+    with a NaN or an infinity, or with weights too large for the scales' type, becomes NaN as a whole.  dtype:
     float16 or bfloat16, the type of the scales and of the rows that are multiplied; default: that of the weights."""
     assert weights.dim() in (2, 3)
     codes, scales, from_ = hip_kernels.quantize_4bit(_batched(weights, 3), group_size, offsets, dtype or weights.dtype)
