@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define STK_AMD_ABI_VERSION 22
+#define STK_AMD_ABI_VERSION 23
 
 /* status codes */
 #define STK_OK 0
@@ -690,6 +690,12 @@ int stk_matmul_4bit_scatter(const void* x, int64_t x_stride, const int32_t* indi
                             const float* weights, const void* packed, const void* scales, const void* offsets, int64_t experts,
                             int64_t inputs, int64_t outputs, int64_t group_size, void* out, int64_t out_stride, int dtype,
                             void* workspace, size_t workspace_bytes, stk_stream_t stream);
+/*
+ * Which kernel these products take for so many rows (with routing: slots), so that tests can tell that they reach every one: 0 .. 4
+ * the streams of few rows, 5 rows that are no whole 16-byte pieces, 6 .. 8 the tiles of many rows; -1 for sizes below 1.  whole_pieces:
+ * whether inputs and x_stride are multiples of eight and x is 16-byte aligned.
+ */
+int stk_4bit_product_kernel(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs, int whole_pieces);
 
 #ifdef __cplusplus
 }

@@ -12,7 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "libstk_amd.so")
 NATIVE_PATH = os.path.join(os.path.dirname(_HERE), "_native.so")
 
-ABI_VERSION = 22
+ABI_VERSION = 23
 STK_OK, STK_ERR_DIMS, STK_ERR_UNSUPPORTED, STK_ERR_HIP, STK_ERR_WORKSPACE = 0, 1, 2, 3, 4
 STK_F16, STK_BF16, STK_F32 = 0, 1, 2
 STK_I16, STK_I32 = 0, 1
@@ -81,6 +81,7 @@ SIGNATURES = {
     "stk_dequantize_4bit": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _int, _p]),
     "stk_matmul_4bit": (_int, [_p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _int, _int, _p]),
     "stk_gather_matmul_4bit": (_int, [_p, _i64, _i64, _p, _p, _int, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _int, _int, _p]),
+    "stk_4bit_product_kernel": (_int, [_i64, _i64, _i64, _i64, _int]),
     "stk_matmul_4bit_scatter_workspace_bytes": (_sz, [_i64, _i64]),
     "stk_matmul_4bit_scatter": (_int, [_p, _i64, _p, _p, _int, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _int, _p, _sz, _p]),
     "stk_dsd_scatter": (_int, [_i64, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _i64, _int, _int, _int, _p, _p, _i64, _p]),

@@ -761,24 +761,40 @@ static void launch_ring(const Product4& p, bool bf16, hipStream_t stream) {
 //   the same with offsets                                                                             130     129     119     135
 //   512, 1000, 2048 rows, 4096 x 4096                                                                 33, 51, 92      36, 50, 86
 // (64 x 256 needs more registers than two workgroups of a compute unit have: 270 us on the 16384 rows.)
+enum ProductKernel : int {
+  kStream8x1x1 = 0, kStream4x1x2, kStream4x1x4, kStream2x2x2, kStream1x4x4,   // few rows: KW x NW x NT
+  kTile32x128, kRing32x256, kRing32x128, kRing16x128                          // many: rows x outputs
+};
+static ProductKernel product_kernel(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs, bool whole) {
+  const int64_t along = pieces_in(inputs), down = pieces_out(outputs);
+  // as if the rows were spread evenly over the experts: where they really are only the device knows
+  const int64_t hit = experts < rows ? experts : rows, each = (rows + hit - 1) / hit;
+  const int64_t tiles = hit * ((each + 15) / 16) * down, across8 = (down + 7) / 8, across16 = (down + 15) / 16;
+  if (along >= 24 ? each > 16 && tiles > 3000 : each >= 8 && tiles >= 1536) {
+    if (!whole) return kTile32x128;
+    if (each >= 24 && hit * ((each + 31) / 32) * across16 >= 512) return kRing32x256;
+    if (each >= 12 && hit * ((each + 31) / 32) * across8 >= 256) return kRing32x128;
+    return kRing16x128;
+  }
+  if (tiles <= 320) return kStream8x1x1;
+  if (tiles <= 640) return kStream4x1x2;
+  if (along >= 24) return kStream4x1x4;
+  return tiles <= 4096 ? kStream2x2x2 : kStream1x4x4;
+}
 static int launch_product(const char* who, const Product4& p, int dtype, hipStream_t stream) {
   const bool bf16 = dtype == STK_BF16;
   if (most_tiles(p, 16) > (int64_t)65535 * 65535) return fail(STK_ERR_UNSUPPORTED, "%s: %lld rows", who, (long long)p.rows);
-  const int64_t along = pieces_in(p.inputs), down = pieces_out(p.outputs);
-  // as if the rows were spread evenly over the experts: where they really are only the device knows
-  const int64_t hit = p.experts < p.rows ? p.experts : p.rows, each = (p.rows + hit - 1) / hit;
-  const int64_t tiles = hit * ((each + 15) / 16) * down, across8 = (down + 7) / 8, across16 = (down + 15) / 16;
-  if (along >= 24 ? each > 16 && tiles > 3000 : each >= 8 && tiles >= 1536) {
-    const bool whole = p.inputs % 8 == 0 && p.x_stride % 8 == 0 && aligned16(p.x);
-    if (!whole) launch_tiles<2, 2>(p, bf16, stream);
-    else if (each >= 24 && hit * ((each + 31) / 32) * across16 >= 512) launch_ring<4, 2>(p, bf16, stream);
-    else if (each >= 12 && hit * ((each + 31) / 32) * across8 >= 256) launch_ring<2, 2>(p, bf16, stream);
-    else launch_ring<2, 1>(p, bf16, stream);
-  } else if (tiles <= 320) launch_stream<8, 1, 1>(p, bf16, stream);
-  else if (tiles <= 640) launch_stream<4, 1, 2>(p, bf16, stream);
-  else if (along >= 24) launch_stream<4, 1, 4>(p, bf16, stream);
-  else if (tiles <= 4096) launch_stream<2, 2, 2>(p, bf16, stream);
-  else launch_stream<1, 4, 4>(p, bf16, stream);
+  switch (product_kernel(p.rows, p.experts, p.inputs, p.outputs, p.inputs % 8 == 0 && p.x_stride % 8 == 0 && aligned16(p.x))) {
+    case kStream8x1x1: launch_stream<8, 1, 1>(p, bf16, stream); break;
+    case kStream4x1x2: launch_stream<4, 1, 2>(p, bf16, stream); break;
+    case kStream4x1x4: launch_stream<4, 1, 4>(p, bf16, stream); break;
+    case kStream2x2x2: launch_stream<2, 2, 2>(p, bf16, stream); break;
+    case kStream1x4x4: launch_stream<1, 4, 4>(p, bf16, stream); break;
+    case kTile32x128: launch_tiles<2, 2>(p, bf16, stream); break;
+    case kRing32x256: launch_ring<4, 2>(p, bf16, stream); break;
+    case kRing32x128: launch_ring<2, 2>(p, bf16, stream); break;
+    case kRing16x128: launch_ring<2, 1>(p, bf16, stream); break;
+  }
   return STK_OK;
 }
 
@@ -876,6 +892,10 @@ extern "C" int stk_gather_matmul_4bit(const void* x, int64_t tokens, int64_t x_s
   if (!indices || !bins) return fail(STK_ERR_DIMS, "%s: missing pointer", who);
   if (int rc = launch_product(who, p, dtype, static_cast<hipStream_t>(stream))) return rc;
   return check_launch(who);
+}
+
+extern "C" int stk_4bit_product_kernel(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs, int whole_pieces) {
+  return rows < 1 || experts < 1 || inputs < 1 || outputs < 1 ? -1 : (int)product_kernel(rows, experts, inputs, outputs, whole_pieces != 0);
 }
 
 extern "C" size_t stk_matmul_4bit_scatter_workspace_bytes(int64_t slots, int64_t outputs) {
