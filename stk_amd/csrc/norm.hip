@@ -8,13 +8,14 @@
 // makes 0.02 of that in every result.  Adding the mean of the differences from a first mean is as good, and another sum over the
 // row: 32768 x 8192 in 240 us.)
 //
-// A row belongs to a team of 16, 64, 256 or 1024 lanes that holds it in registers, pieces of eight values a lane, so that it is read once.
+// A row belongs to a team of 16, 64, 256, 512 or 1024 lanes that holds it in registers, pieces of eight values a lane, so that it is read once.
 // The last piece of a row whose length is no multiple of eight is moved back over its neighbour; the values it shares with
 // it are left out of the sums and stored twice.
 //
-// Bound by bytes: 32768 x 8192 in bfloat16 take 203 us forward (1.07 GB, 5.3 TB/s, a copy reaches 5.2) and 316 backward (1.61 GB, 5.1 TB/s).
-// 16384 x 1024 takes 15 and 21 + 4 for the sums over the shares, less than the 43 us that the host needs for a step of autograd; 64 rows
-// are a launch (3.6 us).
+// Bound by bytes: 32768 x 8192 in bfloat16 take 208 us forward (1.07 GB, 5.2 TB/s, a copy reaches 5.2) and 316 backward (1.61 GB, 5.1 TB/s).
+// 16384 x 1024 takes 16 and 21 + 4 for the sums over the shares, less than the 43 us that the host needs for a step of autograd; 64 rows
+// are a launch (3.6 us).  Not bound by bytes: the backward pass of float32 rows of 1025 to 2048 values (5003 x 1151: 28 us for 69 MB, a team
+// of 64 lanes with 32 values each takes 247 registers), and the kernels that loop over rows too long for registers (below).
 #include <type_traits>
 
 #include "common.h"
@@ -237,6 +238,9 @@ __global__ __launch_bounds__(1024) void layer_norm_param_kernel(const float* __r
 }
 
 // ---------------------------------------------------------------- rows of fewer than eight values, or too long for registers
+// A value at a time, a row read three times forward, x and dy again for each of dx and the sums: a training pass of 3000 x 20000 in
+// bfloat16 takes 569 us (239 forward), 4.9 times what its bytes would; 8192 x 16384, which fit, 375.
+
 // Sum over the 256 threads of a workgroup; every thread gets it.
 __device__ __forceinline__ float workgroup_sum(float v, float* part) {
   v = wave64_sum(v);
@@ -334,8 +338,9 @@ static void for_types(int dtype, int param_dtype, Fn&& fn) {
 }
 
 // The teams for rows of `size` values, forward and backward with the workgroups that share the rows of a backward pass (each leaves
-// 2 n fp32 sums); rows of other sizes: the kernels above that loop over a row.  Times in us of alternatives as lanes,
-// pieces x threads @ workgroups, bfloat16, cold:
+// 2 n fp32 sums); rows of other sizes: the kernels above that loop over a row.  float32 rows take the same teams, which were measured in
+// bfloat16 only.  Backward 1024,2 has 128 registers a lane and spills 6 to 11 more (28 with bfloat16 parameters).  Times in us of
+// alternatives as lanes, pieces x threads @ workgroups, bfloat16, cold:
 //   16384 x 1024   forward 64,2 15.5, 256,1 22.6          backward 64,2 x512 @512 23.2, x256 @1024 23.2, @512 25.1, 256,1 x256 @1024 34.2
 //   16384 x 2048   forward 256,1 31.9, 64,4 33.6          backward 64,4 x512 @256 47.8, 256,1 x256 @1024 49.0, 64,4 x512 @512 52.9
 //   16384 x 4096   forward 256,2 55.6, 512,1 57.9         backward 512,1 @512 81.8, 256,2 @512 90.8, 512,1 @256 105

@@ -308,7 +308,9 @@ struct Stage {
 // 130 others: two wavefronts instead of three (4x1x4 on the 128 slots of 64 experts of 4096 x 1024: 31.5 us, 29.6 so).
 // Bound by the bytes of the weights where many experts are hit (64 tokens, top 2 of 64 experts of 1024 x 4096: 121 MB in 26.1 us,
 // 4.65 TB/s of the 5.16 of a copy; of 4096 x 1024 with the sum over the choices 29.5, two launches), and by the launch and one trip to
-// memory for a single row (4096 x 4096, 8.7 MB: 5.3 us).
+// memory for a single row (4096 x 4096, 8.7 MB: 5.3 us).  Four tiles with groups of 32 want more than the 256 registers that there are: with
+// offsets 12 to 14 go to scratch memory (55 us for the same tokens, 58 for 4096 x 1024), in bfloat16 without offsets 1x4x4 loses 113, which
+// cost it 99 us where float16 takes 34.5.
 template <bool BF16, bool AFFINE, int SUB, int KW, int NW, int NT>
 __global__ __launch_bounds__(64 * KW * NW, 2) void stream_kernel(Product4 p) {
   constexpr int MT = 1, DEPTH = 2;
@@ -739,7 +741,8 @@ static void launch_ring(const Product4& p, bool bf16, hipStream_t stream) {
 
 // Which kernel.  With T tiles of 16 rows and 16 outputs, and pieces along the inputs, the streams want some thousand wavefronts and then
 // as many outputs for one as possible: a fragment of x serves all of them.  Rows in some number share codes instead (ring, or tile
-// where x is no whole 16-byte pieces).  us at T, pieces, in the order of the rule below, KW x NW x NT (bf16, groups of 128, cold):
+// where x is no whole 16-byte pieces).  The choice between streams and ring was measured in bfloat16 with groups of 128 and no offsets and
+// decides for every form; the ring's tiles were measured in the forms named below.  us at T, pieces, in the order of the rule, KW x NW x NT (cold):
 //                                             8x1x1  4x1x2  2x2x2  4x1x4  1x4x4   ring, rows x outputs:  16x128  32x128  32x256
 //   256, 32   (1 row, 4096 x 4096)              6.9    9.2   12.0   11.1   23.0                            20.5    24.8    33.9
 //   512, 32   (32 rows, the same)              14.0   10.8   15.0   12.6   27.6                            20.2    25.0    34.5
