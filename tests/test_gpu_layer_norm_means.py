@@ -1,8 +1,7 @@
 """GPU: the mean of a row of equal values is that value, so that such a row has no deviation and its result is the bias, to the last bit.
 
-Why that can be asked for: the first sum over n and the quotient are off by some (n / 256 + 16) 2^-24 of the value c; x - mean is then the
-same small difference d for every element, exactly (both are close together), and the mean of the differences is d up to the same relative
-error, far below half a unit in the last place of c: mean + d rounded is c."""
+Why that can be asked for: the mean is the row's first value plus the mean of the differences from it, which are 0 here, exactly, in whatever
+order they are added up."""
 import pytest
 import torch
 
