@@ -12,7 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "libstk_amd.so")
 NATIVE_PATH = os.path.join(os.path.dirname(_HERE), "_native.so")
 
-ABI_VERSION = 23
+ABI_VERSION = 24
 STK_OK, STK_ERR_DIMS, STK_ERR_UNSUPPORTED, STK_ERR_HIP, STK_ERR_WORKSPACE = 0, 1, 2, 3, 4
 STK_F16, STK_BF16, STK_F32 = 0, 1, 2
 STK_I16, STK_I32 = 0, 1
@@ -84,6 +84,24 @@ SIGNATURES = {
     "stk_4bit_product_kernel": (_int, [_i64, _i64, _i64, _i64, _int]),
     "stk_matmul_4bit_scatter_workspace_bytes": (_sz, [_i64, _i64]),
     "stk_matmul_4bit_scatter": (_int, [_p, _i64, _p, _p, _int, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i64, _int, _p, _sz, _p]),
+    "stk_group_top_experts": (_int, [_p, _i64, _i64, _i64, _int, _int, _int, _int, _int, _p, _int, _f32, _p, _p, _int, _p]),
+    "stk_group_top_experts_backward": (_int, [_p, _i64, _p, _p, _p, _i64, _i64, _int, _int, _int, _f32, _p, _i64, _int, _p]),
+    "stk_8bit_piece_bytes": (_i64, [_i64, _i64, _i64]),
+    "stk_8bit_scale_bytes": (_i64, [_i64, _i64, _i64, _int]),
+    "stk_8bit_row_bytes": (_i64, [_i64, _i64]),
+    "stk_8bit_exponent_bytes": (_i64, [_i64, _i64]),
+    "stk_quantize_8bit": (_int, [_p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p, _p, _p, _p, _p]),
+    "stk_pack_8bit": (_int, [_p, _p, _int, _i64, _i64, _i64, _p, _p, _p]),
+    "stk_dequantize_8bit": (_int, [_p, _p, _int, _i64, _i64, _i64, _p, _int, _p]),
+    "stk_quantize_rows_8bit": (_int, [_p, _i64, _i64, _i64, _int, _p, _p, _p, _p, _int, _p]),
+    "stk_matmul_8bit_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "stk_matmul_8bit": (_int, [_p, _i64, _i64, _p, _p, _int, _i64, _i64, _p, _i64, _int, _int, _p, _sz, _p]),
+    "stk_gather_matmul_8bit": (_int, [_p, _i64, _i64, _p, _p, _int, _p, _p, _int, _i64, _i64, _i64, _p, _i64, _int, _int, _p, _sz, _p]),
+    "stk_matmul_8bit_scatter_workspace_bytes": (_sz, [_i64, _int, _i64, _i64, _i64]),
+    "stk_matmul_8bit_scatter": (_int, [_p, _i64, _p, _p, _int, _i64, _p, _p, _p, _int, _i64, _i64, _i64, _p, _i64, _int, _p, _sz, _p]),
+    "stk_8bit_product_kernel": (_int, [_i64, _i64, _i64, _i64]),
+    "stk_linear_8bit": (_int, [_p, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _int, _p]),
+    "stk_weight_gradient_8bit": (_int, [_p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _p, _int, _p]),
     "stk_dsd_scatter": (_int, [_i64, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _i64, _int, _int, _int, _p, _p, _i64, _p]),
 }
 

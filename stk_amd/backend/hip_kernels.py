@@ -564,6 +564,66 @@ def matmul_4bit_scatter(x, indices, bins, top_k, packed, scales, offsets, inputs
     return _lib.native().matmul_4bit_scatter(x, indices, bins, top_k, packed, scales, offsets, inputs, outputs, group_size, weights)
 
 
+def group_top_experts(scores, bias, top_k, groups, top_groups, sigmoid, group_best, normalize, scale):
+    """(chosen int32, weights fp32) of stk_group_top_experts."""
+    return _lib.native().group_top_experts(scores, bias, top_k, groups, top_groups, sigmoid, group_best, normalize, scale)
+
+
+def group_top_experts_graph(scores, bias, top_k, groups, top_groups, sigmoid, group_best, normalize, scale):
+    """The results of group_top_experts, in torch's graph where a gradient is wanted."""
+    return _lib.native().group_top_experts_graph(scores, bias, top_k, groups, top_groups, sigmoid, group_best, normalize, scale)
+
+
+def group_top_experts_backward(scores, chosen, weights, grad, sigmoid, normalize, scale):
+    """Gradient with respect to the scores (stk_group_top_experts_backward)."""
+    return _lib.native().group_top_experts_backward(scores, chosen, weights, grad, sigmoid, normalize, scale)
+
+
+def quantize_8bit(w):
+    """(packed codes, scales) of weights [experts, inputs, outputs] (stk_quantize_8bit)."""
+    return _lib.native().quantize_8bit(w, False)[:2]
+
+
+def pack_8bit(codes, scales):
+    """(packed codes, scales) in the layout of the products (stk_pack_8bit)."""
+    return _lib.native().pack_8bit(codes, scales)
+
+
+def dequantize_8bit(packed, scales, inputs, outputs, dtype):
+    """[experts, inputs, outputs] (stk_dequantize_8bit)."""
+    return _lib.native().dequantize_8bit(packed, scales, inputs, outputs, dtype)
+
+
+def matmul_8bit(x, packed, scales, inputs, outputs, activation=None):
+    """act(x @ w) (stk_matmul_8bit)."""
+    return _lib.native().matmul_8bit(x, packed, scales, inputs, outputs, _forward_activation(activation))
+
+
+def gather_matmul_8bit(x, indices, bins, top_k, packed, scales, inputs, outputs, activation=None):
+    """act(x[indices // top_k] @ w of the expert), a row for each sorted slot (stk_gather_matmul_8bit)."""
+    return _lib.native().gather_matmul_8bit(x, indices, bins, top_k, packed, scales, inputs, outputs, _forward_activation(activation))
+
+
+def matmul_8bit_scatter(x, indices, bins, top_k, packed, scales, inputs, outputs, weights=None):
+    """The tokens' weighted sums of x @ w of the expert (stk_matmul_8bit_scatter)."""
+    return _lib.native().matmul_8bit_scatter(x, indices, bins, top_k, packed, scales, inputs, outputs, weights)
+
+
+def linear_8bit(x, w, bins=None):
+    """x @ w on operands quantised to 8 bits (stk_linear_8bit), in torch's graph where a gradient is wanted."""
+    return _lib.native().linear_8bit_graph(x, w, bins)
+
+
+def linear_8bit_forward(x, w, bins, want_x, want_w):
+    """(x @ w, what linear_8bit_backward takes)."""
+    return _lib.native().linear_8bit_forward(x, w, bins, want_x, want_w)
+
+
+def linear_8bit_backward(grad, saved, bins, x_shape, w_shape, want_x, want_w):
+    """(dx, dw) of linear_8bit, None for what is not wanted (stk_linear_8bit, stk_weight_gradient_8bit)."""
+    return _lib.native().linear_8bit_backward(grad, saved, bins, list(x_shape), list(w_shape), want_x, want_w)
+
+
 def _forward_activation(activation):
     if activation not in ACTIVATIONS or ACTIVATIONS[activation] > ACTIVATIONS["silu"]:
         raise ValueError(f"unknown activation {activation!r}; one of {sorted(k for k, v in ACTIVATIONS.items() if k and v <= ACTIVATIONS['silu'])}")

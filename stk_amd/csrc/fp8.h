@@ -1,0 +1,55 @@
+// 8-bit floating-point values (e4m3: 4 bits of exponent, 3 of mantissa, at most 448, no infinities) with a scale for every block of 128, as
+// the products take them.
+//
+// Rows: codes [row][blocks x 128], zeros beyond the last input, and one exponent byte (2^(byte - 127)) for each row and block, [row][blocks
+// rounded up to 4], so that a dword holds those of four neighbouring blocks.
+//
+// Pieces: the operand that all rows share, 16 of its lines x 128 inputs in 2048 bytes, in the order of a wavefront's two 16-byte accesses:
+// access h, lane l has inputs 64 h + 16 (l / 16) .. + 15 of line l % 16.  (Which input goes where in v_mfma_scale_f32_16x16x128 does not
+// matter as long as both operands agree, and all inputs of a block have one scale.)  Pieces follow each other along the inputs, then along
+// the lines, then expert by expert.  Lines are dealt to the pieces of 64 so that the four sums that a lane has of each of four pieces belong to
+// 16 neighbouring lines: line 16 q + 4 t + r of the 64 is line 4 q + r of piece t.  Lines are padded to a multiple of 64 with zeros.
+// Scales of pieces: exponent bytes [place of the line][blocks rounded up to 4] ("power"), or fp32 [ceil(lines / 128)][blocks] ("float").
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace stk {
+
+constexpr int kBlock8 = 128, kPieceLines8 = 16, kPieceBytes8 = 2048, kGroupLines8 = 64;
+enum Scales8 : int { kPowerScales = 0, kFloatScales = 1 };
+
+__host__ __device__ inline int64_t blocks8(int64_t size) { return (size + kBlock8 - 1) / kBlock8; }
+__host__ __device__ inline int64_t exponent_stride8(int64_t size) { return (blocks8(size) + 3) / 4 * 4; }
+__host__ __device__ inline int64_t padded_lines8(int64_t lines) { return (lines + kGroupLines8 - 1) / kGroupLines8 * kGroupLines8; }
+__host__ __device__ inline int64_t piece_bytes8(int64_t lines, int64_t size) { return padded_lines8(lines) / kPieceLines8 * blocks8(size) * kPieceBytes8; }
+__host__ __device__ inline int64_t scale_bytes8(int64_t lines, int64_t size, int kind) {
+  return kind == kPowerScales ? padded_lines8(lines) * exponent_stride8(size) : blocks8(lines) * blocks8(size) * 4;
+}
+// Place of a line among those of its pieces.
+__host__ __device__ inline int64_t place8(int64_t line) { return (line & ~(int64_t)63) + ((line >> 2) & 3) * 16 + ((line >> 4) & 3) * 4 + (line & 3); }
+// Byte of (place, input) from the start of an operand's pieces; `blocks` of them along the inputs.
+__host__ __device__ inline int64_t piece_at8(int64_t place, int64_t input, int64_t blocks) {
+  const int64_t piece = place / kPieceLines8 * blocks + input / kBlock8;
+  const int k = (int)(input % kBlock8);
+  return piece * kPieceBytes8 + (k >> 6) * 1024 + ((int)(place & 15) + 16 * ((k & 63) >> 4)) * 16 + (k & 15);
+}
+
+// The exponent byte of values whose largest magnitude has the fp32 bits `most`: the smallest 2^e with most <= 448 2^e, e >= -126.  448 =
+// 1.75 2^8.  An infinity or a NaN: 0 (the codes say that it is one).
+__host__ __device__ inline int exponent_byte8(uint32_t most) {
+  if (most >= 0x7f800000u) return 0;
+  const int e = (int)(most >> 23) - 8 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0);   // 127 more than the exponent
+  return e < 1 ? 1 : e;
+}
+// 1 / 2^(byte - 127), bytes 1 .. 254 (the largest is 247).
+__device__ __forceinline__ float inverse_power8(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
+
+constexpr uint32_t kNan8 = 0x7f7f7f7fu;   // four codes
+// Codes of four values that are at most 448, rounded to nearest, ties to even.
+__device__ __forceinline__ uint32_t codes8(float a, float b, float c, float d) {
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
+}
+__device__ __forceinline__ float value8(uint8_t code) { return __builtin_amdgcn_cvt_f32_fp8((int)code, 0); }
+
+}  // namespace stk

@@ -1,0 +1,422 @@
+// stk_group_top_experts: a router's choice among groups of experts, and the gradient of the chosen weights with respect to the scores.
+//   p = softmax(scores) or sigmoid(scores);   c = p + bias  (a score of -infinity: c = -infinity)
+//   value of a group = the sum of its `best` largest c;   the top_groups groups of the largest values, ties to the lower group
+//   chosen: the top_k experts of these groups with the largest c - without a bias the largest scores - in descending order, ties to the lower expert
+//   weights_j = scale p[chosen_j]      or, normalized, divided by the sum of p over the chosen ones
+// Gradient, with u_j = g_j weights_j and q_j = weights_j / scale:
+//   sigmoid                ds[chosen_j] = (u_j - [normalized] q_j sum u) (1 - p_j)
+//   softmax, normalized    ds[chosen_j] = u_j - q_j sum u
+//   softmax                ds_i = (u_j where i = chosen_j) - p_i sum u
+//
+// Which experts are chosen is to be a matter of the inputs, not of how exp is computed.  Everything is computed in fp32, whose error in c is below
+// 2^-19 of the largest p and |bias|; where two values that decide the choice or its order are closer than four times that, and are not of
+// equal inputs (which are equal whatever the precision), the token is done again in 64 bits.  That is one token in some hundred.
+//
+// A token belongs to a team of 16 or 64 lanes, and expert i to its lane i % LANES, place i / LANES.  A round of the choice is a maximum over
+// keys of 32 bits: the ordered bits of c with the place in the lowest four, so that a lane's maximum says whose it is; what that takes off c is
+// within the margin of the 64-bit check.
+#include <type_traits>
+
+#include "common.h"
+#include "values.h"
+#include "wave_scan.h"
+
+namespace stk {
+
+constexpr int kGroupRouterExperts = 1024, kGroupRouterTopK = 32, kGroupRouterGroups = 64;
+
+struct GroupRouter {
+  const void* scores;
+  int64_t stride, tokens;
+  int experts, groups, top_groups, best, top_k;
+  int sigmoid, normalize;
+  float scale;
+  const float* bias;
+  uint32_t group_size, group_magic;   // i / group_size = i group_magic >> 22
+  int32_t* chosen;
+  float* weights;
+};
+
+template <int LANES, class T>
+__device__ __forceinline__ T from_lane(T v, int lane) { return __shfl(v, lane, LANES); }
+template <int LANES>
+__device__ __forceinline__ bool any_of_team(bool v) {
+  const uint64_t all = __ballot(v);
+  if constexpr (LANES == 64) return all != 0;
+  else return (all >> (threadIdx.x & 48) & 0xffffu) != 0;
+}
+template <int LANES>
+__device__ __forceinline__ uint64_t ballot_of_team(bool v) {
+  const uint64_t all = __ballot(v);
+  if constexpr (LANES == 64) return all;
+  else return all >> (threadIdx.x & 48) & 0xffffu;
+}
+template <int LANES, class T, class Fn>
+__device__ __forceinline__ T reduce_team(T v, Fn&& fn) {
+#pragma unroll
+  for (int d = 1; d < LANES; d *= 2) v = fn(v, __shfl_xor(v, d, LANES));
+  return v;
+}
+template <int CONTROL>
+__device__ __forceinline__ uint32_t moved_key32(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, 0xf, 0xf, true); }
+template <int LANES>
+__device__ __forceinline__ uint32_t largest_key(uint32_t v) {
+  v = max(v, moved_key32<0xb1>(v)), v = max(v, moved_key32<0x4e>(v)), v = max(v, moved_key32<0x141>(v)), v = max(v, moved_key32<0x140>(v));
+  if constexpr (LANES == 64) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int r = 0; r < 64; r += 16) best = max(best, (uint32_t)__builtin_amdgcn_readlane((int)v, r));
+    v = best;
+  }
+  return v;
+}
+
+// Numbers in their order as whole numbers: -0 like 0, NaN on top, nothing at 0.
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return v != v ? 0xffffffffu : v == 0.f ? 0x80000000u : u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t ordered(double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v), sign = 1ull << 63;
+  return v != v ? ~0ull : v == 0. ? sign : u & sign ? ~u : u | sign;
+}
+
+// exp(x), x <= 0, from the hardware's power of two (1 unit in the last place): x log2(e) is rounded, and what that loses is put back
+// to first order.
+__device__ __forceinline__ float exponential_of(float x) {
+  constexpr float kLog2e = 1.44269504088896341f, kLog2eRest = 1.92596299112661746887e-8f, kLn2 = 0.693147180559945309f;
+  const float t = x * kLog2e, rest = fmaf(x, kLog2eRest, fmaf(x, kLog2e, -t)), y = __builtin_amdgcn_exp2f(t);
+  return t < -149.f ? 0.f : fmaf(y, rest * kLn2, y);
+}
+__device__ __forceinline__ double exponential_of(double x) { return exp(x); }
+// 1 / (1 + exp(-s)) from the exponential of -|s|.
+template <class F>
+__device__ __forceinline__ F sigmoid_of(F s) {
+  const F t = exponential_of(s < 0 ? s : -s);
+  return (s < 0 ? t : F(1)) / (F(1) + t);
+}
+
+// The two largest of a group.
+template <class F>
+struct Two {
+  F first, second;
+};
+// Whether a comes in front of b: NaN in front of every number.
+template <class F>
+__device__ __forceinline__ bool in_front(F a, F b) { return a > b || (a != a && b == b); }
+template <class F>
+__device__ __forceinline__ void put(Two<F>& t, F v) {
+  const bool top = in_front(v, t.first);
+  t.second = top ? t.first : in_front(v, t.second) ? v : t.second;
+  t.first = top ? v : t.first;
+}
+
+// One token in the precision of F.  mine: the scores of this lane's experts lane + LANES j.  row: LDS of the team for the c of every expert,
+// and the groups' values behind them.  at, p: the expert that lane k < top_k is to write and its p; sum: that of the chosen p.  false (F =
+// float only): two of the values that decide are too close for it.
+template <class F, int DTYPE, int LANES, int V>
+__device__ __forceinline__ bool choose(const GroupRouter& r, const float (&mine)[V], F* row, int lane, int& at, F& p_at, F& sum) {
+  constexpr bool kFast = std::is_same<F, float>::value;
+  const F kNone = -INFINITY;
+  F c[V];
+  F top = 0, total = 1, largest_p = 0, largest_b = 0;
+  bool strange = false;
+  if (!r.sigmoid) {
+    F most = kNone;
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if (lane + LANES * j < r.experts) most = in_front((F)mine[j], most) ? (F)mine[j] : most;
+    top = reduce_team<LANES>(most, [](F a, F b) { return in_front(a, b) ? a : b; });
+    total = 0;
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if (lane + LANES * j < r.experts) total += top == kNone ? F(0) : exponential_of((F)mine[j] - top);   // (a row of masked experts)
+    total = reduce_team<LANES>(total, [](F a, F b) { return a + b; });
+  }
+  const auto share = [&](F s) {   // p of a score
+    if (r.sigmoid) return sigmoid_of(s);
+    return top == kNone ? F(0) : exponential_of(s - top) / total;
+  };
+#pragma unroll
+  for (int j = 0; j < V; j++) {
+    const int e = lane + LANES * j;
+    c[j] = kNone;
+    if (e < r.experts) {
+      const F s = (F)mine[j], p = share(s), b = r.bias ? (F)r.bias[e] : F(0);
+      c[j] = s == kNone ? kNone : p + b;
+      if constexpr (kFast) {
+        largest_p = fmaxf(largest_p, p);
+        if (fabsf(b) < INFINITY) largest_b = fmaxf(largest_b, fabsf(b));
+        else strange = true;
+        strange |= !(fabsf(c[j]) < INFINITY) && s != kNone;
+      }
+      row[e + (e >> 5)] = c[j];   // (groups of 32 start on different banks)
+    }
+  }
+  asm volatile("" : : : "memory");   // (a team lies in one wavefront, whose LDS accesses are made in order)
+  F margin = 0;
+  if constexpr (kFast) {
+    // infinities and NaN among them: the fp32 comparisons below say nothing
+    if (any_of_team<LANES>(strange)) return false;
+    largest_p = reduce_team<LANES>(largest_p, [](F a, F b) { return fmaxf(a, b); });
+    if (r.bias) largest_b = reduce_team<LANES>(largest_b, [](F a, F b) { return fmaxf(a, b); });
+    margin = (largest_p + largest_b) * 0x1p-17f;
+  }
+  // ------------------------------------------------------------ groups
+  uint64_t kept = ~0ull;
+  if (r.top_groups < r.groups) {
+    // a group's lanes look through it together
+    int along = 1;
+    while (2 * along * r.groups <= LANES) along *= 2;
+    const int group = lane / along, size = (int)r.group_size;
+    Two<F> two = {kNone, kNone};
+    if (group < r.groups)
+      for (int i = lane % along; i < size; i += along) {
+        const int e = group * size + i;
+        put(two, row[e + (e >> 5)]);
+      }
+    for (int d = 1; d < along; d *= 2) {
+      const Two<F> other = {__shfl_xor(two.first, d, LANES), __shfl_xor(two.second, d, LANES)};
+      put(two, other.first), put(two, other.second);
+    }
+    const F value = group < r.groups ? r.best == 2 ? two.first + two.second : two.first : kNone;
+    int rank = 0;
+    uint64_t close = 0;
+    for (int g = 0; g < r.groups; g++) {
+      const F other = from_lane<LANES>(value, g * along);
+      rank += in_front(other, value) || ((other == value || (other != other && value != value)) && g < group) ? 1 : 0;
+      if constexpr (kFast) close |= (uint64_t)(fabsf(other - value) <= 2 * margin) << g;
+    }
+    const bool first_lane = lane % along == 0, is = group < r.groups && rank < r.top_groups;
+    // bits of the groups: those of their first lanes
+    const uint64_t bits = ballot_of_team<LANES>(is && first_lane);
+    kept = 0;
+    for (int g = 0; g < r.groups; g++) kept |= (bits >> (g * along) & 1ull) << g;
+    if constexpr (kFast) {
+      const uint64_t all = r.groups < 64 ? (1ull << r.groups) - 1 : ~0ull;
+      if (any_of_team<LANES>(is && (close & all & ~kept) != 0)) return false;
+    }
+  }
+  // ------------------------------------------------------------ experts
+  // without a bias in the order of the scores, in which sigmoids of 1 are told apart
+  const bool by_score = r.bias == nullptr;
+  typedef std::conditional_t<kFast, uint32_t, uint64_t> key_t;
+  key_t key[V];
+#pragma unroll
+  for (int j = 0; j < V; j++) {
+    const uint32_t e = lane + LANES * j;
+    if (by_score) c[j] = (F)mine[j];
+    const bool in = (int)e < r.experts && (kept >> (r.group_size == 0 ? 0 : e * r.group_magic >> 22) & 1ull);
+    if constexpr (kFast) key[j] = in ? (ordered(c[j]) & ~15u) | (15u - j) : 0u;
+    else key[j] = in ? ordered(c[j]) : 0u;
+    if (!in) c[j] = kNone;
+  }
+  at = 0;
+  F c_last = 0, s_last = 0;
+  for (int k = 0; k < r.top_k; k++) {
+    key_t best = 0;
+#pragma unroll
+    for (int j = 0; j < V; j++) best = max(best, key[j]);
+    int place = 0, who;
+    if constexpr (kFast) {
+      const key_t all = largest_key<LANES>(best);
+      who = __builtin_ctzll(ballot_of_team<LANES>(best == all));
+      place = 15 - (int)(all & 15u);
+      const key_t gone = lane == who ? all : 0u;
+#pragma unroll
+      for (int j = 0; j < V; j++) key[j] = key[j] == gone ? 0u : key[j];
+    } else {
+      // of equal ones the lowest expert: the lowest place, then the lowest lane
+      const key_t all = reduce_team<LANES>(best, [](key_t a, key_t b) { return a > b ? a : b; });
+      int first = V;
+#pragma unroll
+      for (int j = V - 1; j >= 0; j--) first = key[j] == all ? j : first;
+      place = reduce_team<LANES>(first, [](int a, int b) { return a < b ? a : b; });
+      who = __builtin_ctzll(ballot_of_team<LANES>(first == place));
+#pragma unroll
+      for (int j = 0; j < V; j++) key[j] = lane == who && j == place ? 0u : key[j];
+    }
+    if (lane == k) at = who + LANES * place;
+  }
+  // the scores of the chosen: through LDS, where the lanes' experts are
+  asm volatile("" : : : "memory");
+#pragma unroll
+  for (int j = 0; j < V; j++) {
+    const int e = lane + LANES * j;
+    if (e < r.experts) row[e + (e >> 5)] = (F)mine[j];
+  }
+  asm volatile("" : : : "memory");
+  const bool is = lane < r.top_k;
+  const F s_at = row[at + (at >> 5)];
+  if constexpr (kFast) {
+    const F b_at = r.bias ? r.bias[at] : 0.f, c_at = by_score ? s_at : (s_at == kNone ? kNone : share(s_at) + b_at);
+    // the order of the chosen
+    const F next_c = __shfl_down(c_at, 1, LANES), next_s = __shfl_down(s_at, 1, LANES), next_b = __shfl_down(b_at, 1, LANES);
+    const auto too_close = [&](F a, F b) { return fabsf(a - b) <= (by_score ? fminf(fabsf(a), fabsf(b)) * 0x1p-18f : margin); };
+    bool wrong = lane < r.top_k - 1 && too_close(c_at, next_c) && !(s_at == next_s && b_at == next_b);
+    // the last of them and those that are not chosen
+    c_last = from_lane<LANES>(c_at, r.top_k - 1), s_last = from_lane<LANES>(s_at, r.top_k - 1);
+    const F b_last = from_lane<LANES>(b_at, r.top_k - 1);
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if (key[j] != 0 && too_close(c[j], c_last)) wrong |= !(mine[j] == s_last && (by_score || r.bias[lane + LANES * j] == b_last));
+    if (any_of_team<LANES>(wrong)) return false;
+  }
+  p_at = is ? share(s_at) : F(0);
+  sum = reduce_team<LANES>(p_at, [](F a, F b) { return a + b; });
+  return true;
+}
+
+template <int DTYPE, int LANES, int V>
+__global__ __launch_bounds__(256) void group_top_experts_kernel(GroupRouter r) {
+  typedef typename Value<DTYPE>::stored stored;
+  constexpr int kTeams = 256 / LANES, kRow = LANES * V + LANES * V / 32 + 1;
+  __shared__ double rows[kTeams][kRow];
+  const int lane = threadIdx.x % LANES;
+  double* row = rows[threadIdx.x / LANES];
+  for (int64_t t = (int64_t)blockIdx.x * kTeams + threadIdx.x / LANES; t < r.tokens; t += (int64_t)gridDim.x * kTeams) {
+    const stored* from = static_cast<const stored*>(r.scores) + t * r.stride;
+    float mine[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) mine[j] = lane + LANES * j < r.experts ? Value<DTYPE>::widen(from[lane + LANES * j]) : -INFINITY;
+    int at;
+    float p, sum;
+    if (!choose<float, DTYPE, LANES, V>(r, mine, reinterpret_cast<float*>(row), lane, at, p, sum)) {
+      double p64, sum64;
+      choose<double, DTYPE, LANES, V>(r, mine, row, lane, at, p64, sum64);
+      p = (float)p64, sum = (float)sum64;
+    }
+    if (lane < r.top_k) {
+      r.chosen[t * r.top_k + lane] = at;
+      r.weights[t * r.top_k + lane] = !r.normalize ? r.scale * p : sum == 0.f ? 0.f : r.scale * (p / sum);
+    }
+    asm volatile("" : : : "memory");
+  }
+}
+
+// The gradient of a token's row goes through LDS: zeros or what every expert gets, the chosen experts' own terms on top, then out.
+template <int DTYPE, int LANES, int V>
+__global__ __launch_bounds__(256) void group_top_experts_backward_kernel(GroupRouter r, const float* __restrict__ grad, typename Value<DTYPE>::stored* __restrict__ out,
+                                                                         int64_t out_stride) {
+  typedef typename Value<DTYPE>::stored stored;
+  __shared__ float rows[256 / LANES][LANES * V];
+  const int lane = threadIdx.x % LANES;
+  float* row = rows[threadIdx.x / LANES];
+  const auto add = [](float a, float b) { return a + b; };
+  for (int64_t t = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; t < r.tokens; t += (int64_t)gridDim.x * (256 / LANES)) {
+    const stored* from = static_cast<const stored*>(r.scores) + t * r.stride;
+    float w = 0.f, u = 0.f;
+    int at = -1;
+    if (lane < r.top_k) {
+      w = r.weights[t * r.top_k + lane], at = r.chosen[t * r.top_k + lane];
+      u = grad[t * r.top_k + lane] * w;
+    }
+    const float all = reduce_team<LANES>(u, add);
+    float mine[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) mine[j] = 0.f;
+    if (!r.sigmoid && !r.normalize) {
+      float most = -INFINITY, total = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        mine[j] = lane + LANES * j < r.experts ? Value<DTYPE>::widen(from[lane + LANES * j]) : -INFINITY;
+        most = in_front(mine[j], most) ? mine[j] : most;
+      }
+      most = reduce_team<LANES>(most, [](float a, float b) { return in_front(a, b) ? a : b; });
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        mine[j] = most == -INFINITY ? 0.f : exponential_of(mine[j] - most);
+        total += mine[j];
+      }
+      total = reduce_team<LANES>(total, add);
+#pragma unroll
+      for (int j = 0; j < V; j++) mine[j] = most == -INFINITY ? 0.f : -(mine[j] / total) * all;
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++) row[lane + LANES * j] = mine[j];
+    asm volatile("" : : : "memory");   // (a team lies in one wavefront, whose LDS accesses are made in order)
+    if ((unsigned)at < (unsigned)r.experts) {
+      float own = r.normalize ? u - w / r.scale * all : u;
+      if (r.sigmoid) own *= sigmoid_of(-Value<DTYPE>::widen(from[at]));
+      row[at] += own;
+    }
+    asm volatile("" : : : "memory");
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if (lane + LANES * j < r.experts) out[t * out_stride + lane + LANES * j] = Value<DTYPE>::round(row[lane + LANES * j]);
+    asm volatile("" : : : "memory");
+  }
+}
+
+// Teams of 16 lanes have a lane for every choice, and for every group, where these are few.
+template <class Fn>
+static void for_team(const GroupRouter& r, Fn&& fn) {
+  typedef std::integral_constant<int, 16> Sixteen;
+  typedef std::integral_constant<int, 64> Wave;
+  if (r.top_k <= 16 && r.groups <= 16 && r.experts <= 256) {
+    if (r.experts <= 64) fn(Sixteen(), std::integral_constant<int, 4>());
+    else if (r.experts <= 128) fn(Sixteen(), std::integral_constant<int, 8>());
+    else fn(Sixteen(), std::integral_constant<int, 16>());
+  } else if (r.experts <= 256) fn(Wave(), std::integral_constant<int, 4>());
+  else if (r.experts <= 512) fn(Wave(), std::integral_constant<int, 8>());
+  else fn(Wave(), std::integral_constant<int, 16>());
+}
+static dim3 group_router_grid(int64_t tokens, int lanes) {
+  const int64_t groups = (tokens + 256 / lanes - 1) / (256 / lanes);
+  return dim3((unsigned)(groups < 1 << 20 ? groups : 1 << 20));
+}
+static int group_router_check(const char* who, GroupRouter& r, int64_t experts, int dtype) {
+  if (!is_value_dtype(dtype)) return fail(STK_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
+  if (r.tokens < 0 || experts < 1 || r.groups < 1 || experts % r.groups) return fail(STK_ERR_DIMS, "%s: %lld experts in %d groups", who, (long long)experts, r.groups);
+  if (experts > kGroupRouterExperts || r.top_k > kGroupRouterTopK || r.groups > kGroupRouterGroups)
+    return fail(STK_ERR_UNSUPPORTED, "%s: at most %d experts, %d groups, the top %d", who, kGroupRouterExperts, kGroupRouterGroups, kGroupRouterTopK);
+  const int64_t size = experts / r.groups;
+  if (r.top_groups < 1 || r.top_groups > r.groups || r.top_k < 1 || r.top_k > r.top_groups * size)
+    return fail(STK_ERR_DIMS, "%s: the top %d experts of the top %d groups of %lld", who, r.top_k, r.top_groups, (long long)size);
+  if (r.best < 1 || r.best > 2 || r.best > size) return fail(STK_ERR_DIMS, "%s: a group's value from its best %d of %lld experts", who, r.best, (long long)size);
+  if (!(r.scale - r.scale == 0.f) || r.scale == 0.f) return fail(STK_ERR_DIMS, "%s: scale %g", who, (double)r.scale);
+  if (r.tokens > INT32_MAX / r.top_k) return fail(STK_ERR_UNSUPPORTED, "%s: size exceeds 32-bit range", who);
+  r.experts = (int)experts, r.group_size = (uint32_t)size, r.group_magic = (uint32_t)(((1u << 22) + size - 1) / size);
+  return STK_OK;
+}
+
+}  // namespace stk
+
+using namespace stk;
+
+extern "C" int stk_group_top_experts(const void* scores, int64_t tokens, int64_t experts, int64_t stride, int groups, int top_groups, int best, int top_k,
+                                     int sigmoid, const float* bias, int normalize, float scale, int32_t* chosen, float* weights, int dtype, stk_stream_t stream) {
+  const char* who = "stk_group_top_experts";
+  GroupRouter r = {scores, stride, tokens, 0, groups, top_groups, best, top_k, sigmoid, normalize, scale, bias, 0, 0, chosen, weights};
+  if (int rc = group_router_check(who, r, experts, dtype)) return rc;
+  if (tokens == 0) return STK_OK;
+  if (!scores || !chosen || !weights) return fail(STK_ERR_DIMS, "%s: missing pointer", who);
+  if (stride < 0) return fail(STK_ERR_DIMS, "%s: stride %lld", who, (long long)stride);
+  for_dtype(dtype, [&](auto d) {
+    for_team(r, [&](auto lanes, auto v) {
+      constexpr int D = decltype(d)::value, L = decltype(lanes)::value, V = decltype(v)::value;
+      hipLaunchKernelGGL((group_top_experts_kernel<D, L, V>), group_router_grid(tokens, L), dim3(256), 0, static_cast<hipStream_t>(stream), r);
+    });
+  });
+  return check_launch(who);
+}
+
+extern "C" int stk_group_top_experts_backward(const void* scores, int64_t stride, const int32_t* chosen, const float* weights, const float* grad, int64_t tokens,
+                                              int64_t experts, int top_k, int sigmoid, int normalize, float scale, void* dscores, int64_t dscores_stride, int dtype,
+                                              stk_stream_t stream) {
+  const char* who = "stk_group_top_experts_backward";
+  GroupRouter r = {scores, stride, tokens, 0, 1, 1, 1, top_k, sigmoid, normalize, scale, nullptr, 0, 0, const_cast<int32_t*>(chosen), const_cast<float*>(weights)};
+  if (int rc = group_router_check(who, r, experts, dtype)) return rc;
+  if (tokens == 0) return STK_OK;
+  if (!scores || !chosen || !weights || !grad || !dscores) return fail(STK_ERR_DIMS, "%s: missing pointer", who);
+  if (stride < 0 || dscores_stride < experts) return fail(STK_ERR_DIMS, "%s: strides %lld, %lld", who, (long long)stride, (long long)dscores_stride);
+  for_dtype(dtype, [&](auto d) {
+    typedef typename Value<d()>::stored T;
+    for_team(r, [&](auto lanes, auto v) {
+      constexpr int D = decltype(d)::value, L = decltype(lanes)::value, V = decltype(v)::value;
+      hipLaunchKernelGGL((group_top_experts_backward_kernel<D, L, V>), group_router_grid(tokens, L), dim3(256), 0, static_cast<hipStream_t>(stream), r, grad,
+                         static_cast<T*>(dscores), dscores_stride);
+    });
+  });
+  return check_launch(who);
+}

@@ -893,6 +893,292 @@ Tensor matmul_4bit_scatter(const Tensor& x_, const Tensor& indices, const Tensor
   return out;
 }
 
+// ------------------------------------------------------------------------------------------------ router with groups
+struct GroupChoice {
+  int64_t top_k, groups, top_groups, best;
+  bool sigmoid, normalize;
+  double scale;
+};
+#define GROUP_CHOICE_ARGS int64_t top_k, int64_t groups, int64_t top_groups, bool sigmoid, int64_t best, bool normalize, double scale
+#define GROUP_CHOICE \
+  GroupChoice { top_k, groups, top_groups, best, sigmoid, normalize, scale }
+int small(int64_t v) { return (int)std::min<int64_t>(std::max<int64_t>(v, INT32_MIN), INT32_MAX); }
+std::tuple<Tensor, Tensor> group_choice(const Tensor& scores_, const OptTensor& bias_, const GroupChoice& c) {
+  need_gpu(scores_);
+  const int dtype = value_dtype(scores_);
+  const c10::DeviceGuard guard(scores_.device());
+  const Tensor scores = score_rows(scores_);
+  const int64_t tokens = scores.size(0), experts = scores.size(1);
+  OptTensor bias;
+  if (bias_) {
+    need_gpu(*bias_);
+    require(bias_->dim() == 1 && bias_->numel() == experts && bias_->device() == scores.device(), "group_top_experts: one bias for each expert");
+    bias = bias_->detach().to(at::kFloat).contiguous();
+  }
+  require(c.top_k >= 1 && c.top_k <= experts, "group_top_experts: top_k of 1 up to the number of experts");
+  Tensor chosen = at::empty({tokens, c.top_k}, scores.options().dtype(at::kInt)), weights = at::empty({tokens, c.top_k}, scores.options().dtype(at::kFloat));
+  check(stk_group_top_experts(ptr<void>(scores), tokens, experts, scores.stride(0), small(c.groups), small(c.top_groups), small(c.best), small(c.top_k), c.sigmoid,
+                              ptr<float>(bias), c.normalize, (float)c.scale, ptr<int32_t>(chosen), ptr<float>(weights), dtype, stream_of(scores)));
+  return {chosen, weights};
+}
+std::tuple<Tensor, Tensor> group_top_experts(const Tensor& scores, const OptTensor& bias, GROUP_CHOICE_ARGS) { return group_choice(scores, bias, GROUP_CHOICE); }
+Tensor group_top_experts_backward(const Tensor& scores_, const Tensor& chosen, const Tensor& weights, const Tensor& grad_, bool sigmoid, bool normalize, double scale) {
+  need_gpu(grad_);
+  const c10::DeviceGuard guard(scores_.device());
+  const Tensor scores = score_rows(scores_), grad = grad_.detach().to(at::kFloat).contiguous();
+  require(grad.sizes() == weights.sizes(), "group_top_experts: one gradient per weight");
+  Tensor out = at::empty(scores.sizes(), scores.options());
+  check(stk_group_top_experts_backward(ptr<void>(scores), scores.stride(0), ptr<int32_t>(chosen), ptr<float>(weights), ptr<float>(grad), scores.size(0),
+                                       scores.size(1), (int)weights.size(1), sigmoid, normalize, (float)scale, ptr<void>(out), out.size(1), value_dtype(scores),
+                                       stream_of(scores)));
+  return out;
+}
+struct GroupTopExperts : torch::autograd::Function<GroupTopExperts> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& scores, const OptTensor& bias, const GroupChoice& c) {
+    auto [chosen, weights] = group_choice(scores, bias, c);
+    ctx->save_for_backward({scores, chosen, weights});
+    ctx->saved_data["sigmoid"] = c.sigmoid, ctx->saved_data["normalize"] = c.normalize, ctx->saved_data["scale"] = c.scale;
+    ctx->mark_non_differentiable({chosen});
+    return {chosen, weights};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    if (!grads[1].defined()) return {Tensor(), Tensor(), Tensor()};
+    return once_differentiable({group_top_experts_backward(saved[0], saved[1], saved[2], grads[1], ctx->saved_data["sigmoid"].toBool(),
+                                                           ctx->saved_data["normalize"].toBool(), ctx->saved_data["scale"].toDouble()),
+                                Tensor(), Tensor()},
+                               "group_top_experts");
+  }
+};
+std::tuple<Tensor, Tensor> group_top_experts_graph(const Tensor& scores, const OptTensor& bias, GROUP_CHOICE_ARGS) {
+  if (!at::GradMode::is_enabled() || !scores.requires_grad()) return group_choice(scores, bias, GROUP_CHOICE);
+  const auto out = GroupTopExperts::apply(scores, bias ? OptTensor(bias->detach()) : bias, GROUP_CHOICE);
+  return {out[0], out[1]};
+}
+
+// ------------------------------------------------------------------------------------------------ 8-bit floating-point weights
+// (packed codes, scales) of weights [experts, inputs, outputs], and where wanted those of their transpose.
+std::tuple<Tensor, Tensor, OptTensor, OptTensor> quantize_8bit(const Tensor& w_, bool with_transpose) {
+  need_gpu(w_);
+  const int dtype = value_dtype(w_);
+  const Tensor w = w_.detach();
+  require(w.dim() == 3 && w.numel() > 0, "quantize_8bit: weights are [inputs, outputs] or [experts, inputs, outputs]");
+  const c10::DeviceGuard guard(w.device());
+  const int64_t experts = w.size(0), inputs = w.size(1), outputs = w.size(2);
+  const auto bytes = w.options().dtype(at::kByte);
+  Tensor packed = at::empty({experts, stk_8bit_piece_bytes(1, inputs, outputs)}, bytes), scales = at::empty({experts, stk_8bit_scale_bytes(1, inputs, outputs, 0)}, bytes);
+  OptTensor packed_t, scales_t;
+  if (with_transpose)
+    packed_t = at::empty({experts, stk_8bit_piece_bytes(1, outputs, inputs)}, bytes), scales_t = at::empty({experts, stk_8bit_scale_bytes(1, outputs, inputs, 0)}, bytes);
+  check(stk_quantize_8bit(ptr<void>(w), w.stride(0), w.stride(1), w.stride(2), experts, inputs, outputs, dtype, ptr<void>(packed), ptr<void>(scales),
+                          ptr<void>(packed_t), ptr<void>(scales_t), stream_of(w)));
+  return {packed, scales, packed_t, scales_t};
+}
+// codes [experts, inputs, outputs] and scales [experts, input blocks, output blocks]
+std::tuple<Tensor, Tensor> pack_8bit(const Tensor& codes_, const Tensor& scales_) {
+  need_gpu(codes_), need_gpu(scales_);
+  require(codes_.dim() == 3 && scales_.dim() == 3 && codes_.numel() > 0, "pack_8bit: codes [experts, inputs, outputs], scales [experts, input blocks, output blocks]");
+  if (codes_.scalar_type() != at::kFloat8_e4m3fn)
+    raise(PyExc_NotImplementedError, std::string("stk_amd: 8-bit codes are float8_e4m3fn, got ") + c10::toString(codes_.scalar_type()));
+  const bool float_scales = scales_.scalar_type() == at::kFloat;
+  if (!float_scales && scales_.scalar_type() != at::kFloat8_e8m0fnu)
+    raise(PyExc_NotImplementedError, std::string("stk_amd: 8-bit weights have scales of float32 or float8_e8m0fnu, got ") + c10::toString(scales_.scalar_type()));
+  const c10::DeviceGuard guard(codes_.device());
+  const int64_t experts = codes_.size(0), inputs = codes_.size(1), outputs = codes_.size(2);
+  require(scales_.size(0) == experts && scales_.size(1) == (inputs + 127) / 128 && scales_.size(2) == (outputs + 127) / 128 && scales_.device() == codes_.device(),
+          "pack_8bit: one scale for every block of 128 inputs and 128 outputs");
+  const Tensor codes = codes_.contiguous(), scales = scales_.detach().contiguous();
+  const auto bytes = codes.options().dtype(at::kByte);
+  Tensor packed = at::empty({experts, stk_8bit_piece_bytes(1, inputs, outputs)}, bytes);
+  const int64_t size = stk_8bit_scale_bytes(1, inputs, outputs, float_scales);
+  Tensor packed_scales = float_scales ? at::empty({experts, size / 4}, scales.options()) : at::empty({experts, size}, bytes);
+  check(stk_pack_8bit(ptr<uint8_t>(codes), ptr<void>(scales), float_scales, experts, inputs, outputs, ptr<void>(packed), ptr<void>(packed_scales), stream_of(codes)));
+  return {packed, packed_scales};
+}
+// Packed weights as the calls take them: what pack_8bit or quantize_8bit made.
+struct Packed8 {
+  int64_t experts, inputs, outputs;
+  bool float_scales;
+  Packed8(const Tensor& packed, const Tensor& scales, int64_t inputs_, int64_t outputs_) : experts(0), inputs(inputs_), outputs(outputs_), float_scales(false) {
+    need_gpu(packed), need_gpu(scales);
+    float_scales = scales.scalar_type() == at::kFloat;
+    require(packed.dim() == 2 && packed.scalar_type() == at::kByte && packed.is_contiguous() && scales.is_contiguous() && inputs > 0 && outputs > 0 &&
+                (float_scales || scales.scalar_type() == at::kByte) && scales.device() == packed.device(),
+            "packed 8-bit weights come from pack_8bit or quantize_8bit");
+    experts = packed.size(0);
+    require(packed.numel() == stk_8bit_piece_bytes(experts, inputs, outputs) &&
+                scales.numel() * (float_scales ? 4 : 1) == stk_8bit_scale_bytes(experts, inputs, outputs, float_scales),
+            "packed 8-bit weights come from pack_8bit or quantize_8bit");
+  }
+};
+#define PACKED8_ARGS const Tensor &packed, const Tensor &scales, int64_t inputs, int64_t outputs
+Tensor dequantize_8bit(PACKED8_ARGS, at::ScalarType dtype) {
+  const Packed8 w(packed, scales, inputs, outputs);
+  const c10::DeviceGuard guard(packed.device());
+  Tensor out = at::empty({w.experts, inputs, outputs}, packed.options().dtype(dtype));
+  check(stk_dequantize_8bit(ptr<void>(packed), ptr<void>(scales), w.float_scales, w.experts, inputs, outputs, ptr<void>(out), value_dtype(out), stream_of(packed)));
+  return out;
+}
+// Rows of the products: `inputs` 16-bit values, next to each other.
+Tensor rows8(const Tensor& x_, const Tensor& packed, int64_t inputs) {
+  need_gpu(x_);
+  require(x_.dim() == 2 && x_.size(1) == inputs, "incompatible dimensions");
+  require(x_.device() == packed.device(), "operands are on one device");
+  if (x_.scalar_type() != at::kHalf && x_.scalar_type() != at::kBFloat16)
+    raise(PyExc_NotImplementedError, std::string("stk_amd: rows for 8-bit weights are float16 or bfloat16, got ") + c10::toString(x_.scalar_type()));
+  const Tensor x = x_.detach();
+  return (inputs == 1 || x.stride(1) == 1) && x.stride(0) >= 0 ? x : x.contiguous();
+}
+Tensor bytes_like(const Tensor& t, size_t bytes) { return at::empty({(int64_t)bytes}, t.options().dtype(at::kByte)); }
+Tensor matmul_8bit(const Tensor& x_, PACKED8_ARGS, int activation) {
+  const Packed8 w(packed, scales, inputs, outputs);
+  require(w.experts == 1, "matmul_8bit: the weights of one matrix");
+  const c10::DeviceGuard guard(packed.device());
+  const Tensor x = rows8(x_, packed, inputs);
+  const int64_t rows = x.size(0);
+  Tensor out = at::empty({rows, outputs}, x.options());
+  const size_t bytes = stk_matmul_8bit_workspace_bytes(rows, rows, 1, inputs, outputs);
+  const Tensor ws = bytes_like(x, bytes);
+  check(stk_matmul_8bit(ptr<void>(x), rows, x.stride(0), ptr<void>(packed), ptr<void>(scales), w.float_scales, inputs, outputs, ptr<void>(out), outputs, activation,
+                        value_dtype(x), ptr<void>(ws), bytes, stream_of(x)));
+  return out;
+}
+void check_routing8(const Tensor& indices, const Tensor& bins, const Packed8& w, const Tensor& packed) {
+  need_gpu(indices), need_gpu(bins);
+  for (const Tensor* t : {&indices, &bins})
+    require(t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == packed.device(), "the routing's arrays come from route");
+  require(bins.numel() == w.experts, "one bin for each expert's weights");
+}
+Tensor gather_matmul_8bit(const Tensor& x_, const Tensor& indices, const Tensor& bins, int top_k, PACKED8_ARGS, int activation) {
+  const Packed8 w(packed, scales, inputs, outputs);
+  check_routing8(indices, bins, w, packed);
+  const c10::DeviceGuard guard(packed.device());
+  const Tensor x = rows8(x_, packed, inputs);
+  const int64_t slots = indices.numel();
+  require(top_k >= 1 && x.size(0) * top_k == slots, "one row per token");
+  Tensor out = at::empty({slots, outputs}, x.options());
+  const size_t bytes = stk_matmul_8bit_workspace_bytes(x.size(0), slots, w.experts, inputs, outputs);
+  const Tensor ws = bytes_like(x, bytes);
+  check(stk_gather_matmul_8bit(ptr<void>(x), x.size(0), x.stride(0), ptr<int32_t>(indices), ptr<int32_t>(bins), top_k, ptr<void>(packed), ptr<void>(scales),
+                               w.float_scales, w.experts, inputs, outputs, ptr<void>(out), outputs, activation, value_dtype(x), ptr<void>(ws), bytes, stream_of(x)));
+  return out;
+}
+Tensor matmul_8bit_scatter(const Tensor& x_, const Tensor& indices, const Tensor& bins, int top_k, PACKED8_ARGS, const OptTensor& weights) {
+  const Packed8 w(packed, scales, inputs, outputs);
+  check_routing8(indices, bins, w, packed);
+  const c10::DeviceGuard guard(packed.device());
+  const Tensor x = rows8(x_, packed, inputs);
+  const int64_t slots = indices.numel();
+  require(top_k >= 1 && slots % top_k == 0 && x.size(0) == slots, "one row per slot");
+  const OptTensor by_slot = weights32(weights, slots);
+  require(!by_slot || by_slot->device() == x.device(), "operands are on one device");
+  Tensor out = at::empty({slots / top_k, outputs}, x.options());
+  const size_t bytes = stk_matmul_8bit_scatter_workspace_bytes(slots, top_k, w.experts, inputs, outputs);
+  const Tensor ws = bytes_like(x, bytes);
+  check(stk_matmul_8bit_scatter(ptr<void>(x), x.stride(0), ptr<int32_t>(indices), ptr<int32_t>(bins), top_k, slots / top_k, ptr<float>(by_slot), ptr<void>(packed),
+                                ptr<void>(scales), w.float_scales, w.experts, inputs, outputs, ptr<void>(out), outputs, value_dtype(x), ptr<void>(ws), bytes, stream_of(x)));
+  return out;
+}
+
+// ------------------------------------------------------------------------------------------------ training with 8-bit products
+typedef std::vector<OptTensor> Saved;
+// Rows quantised along their values (codes, exponents) and, as rows or pieces, down the columns.
+struct Quantised8 {
+  Tensor codes, exponents, columns, column_exponents;
+  Quantised8(const Rows& x, bool along, bool down, bool pieces) {
+    const auto bytes = x.t.options().dtype(at::kByte);
+    if (along) codes = at::empty({stk_8bit_row_bytes(x.rows, x.size)}, bytes), exponents = at::empty({stk_8bit_exponent_bytes(x.rows, x.size)}, bytes);
+    if (down) {
+      columns = at::empty({pieces ? stk_8bit_piece_bytes(1, x.rows, x.size) : stk_8bit_row_bytes(x.size, x.rows)}, bytes);
+      column_exponents = at::empty({pieces ? stk_8bit_scale_bytes(1, x.rows, x.size, 0) : stk_8bit_exponent_bytes(x.size, x.rows)}, bytes);
+    }
+    const auto at = [](const Tensor& t) { return t.defined() ? ptr<void>(t) : nullptr; };
+    if (x.rows > 0 && (along || down))
+      check(stk_quantize_rows_8bit(ptr<void>(x.t), x.rows, x.size, x.stride, value_dtype(x.t), at(codes), at(exponents), at(columns), at(column_exponents), pieces,
+                                   stream_of(x.t)));
+  }
+};
+// y of x [..., inputs] and weights [inputs, outputs] or, with the bins of the padded layout, [experts, inputs, outputs]; then what the backward pass
+// takes: the columns of x and their exponents where the gradient of the weights is wanted, the transposed weights where that of x is.
+std::tuple<Tensor, Saved> linear_8bit_forward(const Tensor& x_, const Tensor& w_, const OptTensor& bins, bool want_x, bool want_w) {
+  need_gpu(x_), need_gpu(w_);
+  require(x_.dim() >= 1 && (bins ? x_.dim() == 2 && w_.dim() == 3 : w_.dim() == 2), "linear_8bit: x [..., inputs] and w [inputs, outputs], or the rows of a routing and w [experts, inputs, outputs]");
+  const int64_t inputs = w_.size(-2), outputs = w_.size(-1), experts = bins ? w_.size(0) : 1;
+  require(x_.size(-1) == inputs && inputs > 0 && outputs > 0 && experts > 0, "incompatible dimensions");
+  require(x_.device() == w_.device(), "operands are on one device");
+  if (x_.scalar_type() != w_.scalar_type() || (x_.scalar_type() != at::kHalf && x_.scalar_type() != at::kBFloat16))
+    raise(PyExc_NotImplementedError, std::string("stk_amd: linear_8bit takes rows and weights that are both float16 or both bfloat16, got ") +
+                                         c10::toString(x_.scalar_type()) + " and " + c10::toString(w_.scalar_type()));
+  if (bins) {
+    need_gpu(*bins);
+    require(bins->scalar_type() == at::kInt && bins->is_contiguous() && bins->device() == x_.device() && bins->numel() == experts,
+            "linear_8bit: one bin of the routing for each expert's weights");
+  }
+  const c10::DeviceGuard guard(x_.device());
+  const Rows x(x_);
+  auto sizes = x_.sizes().vec();
+  sizes.back() = outputs;
+  Tensor y = at::empty(sizes, x_.options());
+  if (x.rows == 0) return {y, Saved(4)};
+  const Quantised8 q(x, true, want_w, false);
+  const auto [packed, scales, packed_t, scales_t] = quantize_8bit(bins ? w_ : w_.unsqueeze(0), want_x);
+  check(stk_linear_8bit(ptr<void>(q.codes), ptr<void>(q.exponents), x.rows, ptr<int32_t>(bins), ptr<void>(packed), ptr<void>(scales), experts, inputs, outputs,
+                        ptr<void>(y), outputs, value_dtype(x_), stream_of(x_)));
+  Saved saved(4);
+  if (want_w) saved[0] = q.columns, saved[1] = q.column_exponents;
+  if (want_x) saved[2] = packed_t, saved[3] = scales_t;
+  return {y, saved};
+}
+// (dx, dw), those that are wanted.
+std::tuple<OptTensor, OptTensor> linear_8bit_backward(const Tensor& grad_, const Saved& saved, const OptTensor& bins, at::IntArrayRef x_sizes, at::IntArrayRef w_sizes,
+                                                      bool want_x, bool want_w) {
+  need_gpu(grad_);
+  const c10::DeviceGuard guard(grad_.device());
+  const Rows g(grad_);
+  const int64_t inputs = w_sizes[w_sizes.size() - 2], outputs = w_sizes.back(), experts = bins ? w_sizes[0] : 1;
+  OptTensor dx, dw;
+  if (want_x) dx = at::empty(x_sizes, grad_.options());
+  if (g.rows == 0) {
+    if (want_w) dw = at::zeros(w_sizes, grad_.options());
+    return {dx, dw};
+  }
+  const Quantised8 q(g, want_x, want_w, true);
+  if (want_x)
+    check(stk_linear_8bit(ptr<void>(q.codes), ptr<void>(q.exponents), g.rows, ptr<int32_t>(bins), ptr<void>(saved[2]), ptr<void>(saved[3]), experts, outputs, inputs,
+                          ptr<void>(dx), inputs, value_dtype(grad_), stream_of(grad_)));
+  if (want_w) {
+    dw = at::empty(w_sizes, grad_.options());
+    check(stk_weight_gradient_8bit(ptr<void>(saved[0]), ptr<void>(saved[1]), ptr<void>(q.columns), ptr<void>(q.column_exponents), g.rows, ptr<int32_t>(bins), experts,
+                                   inputs, outputs, ptr<void>(dw), value_dtype(grad_), stream_of(grad_)));
+  }
+  return {dx, dw};
+}
+struct Linear8 : torch::autograd::Function<Linear8> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bins) {
+    auto [y, saved] = linear_8bit_forward(x, w, bins, x.requires_grad(), w.requires_grad());
+    torch::autograd::variable_list keep;
+    for (const OptTensor& t : saved) keep.push_back(t ? *t : Tensor());
+    keep.push_back(bins ? *bins : Tensor());
+    ctx->save_for_backward(keep);
+    ctx->saved_data["x"] = x.sizes(), ctx->saved_data["w"] = w.sizes();
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto kept = ctx->get_saved_variables();
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
+    Saved saved;
+    for (size_t i = 0; i < 4; i++) saved.push_back(kept[i].defined() ? OptTensor(kept[i]) : OptTensor());
+    const OptTensor bins = kept[4].defined() ? OptTensor(kept[4]) : OptTensor();
+    const auto x_sizes = ctx->saved_data["x"].toIntVector(), w_sizes = ctx->saved_data["w"].toIntVector();
+    const auto [dx, dw] = linear_8bit_backward(grads[0], saved, bins, x_sizes, w_sizes, ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+    return once_differentiable({dx.value_or(Tensor()), dw.value_or(Tensor()), Tensor()}, "linear_8bit");
+  }
+};
+Tensor linear_8bit_graph(const Tensor& x, const Tensor& w, const OptTensor& bins) {
+  if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad())) return Linear8::apply(x, w, bins);
+  return std::get<0>(linear_8bit_forward(x, w, bins, false, false));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -933,4 +1219,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("matmul_4bit", &matmul_4bit, py::call_guard<py::gil_scoped_release>());
   m.def("gather_matmul_4bit", &gather_matmul_4bit, py::call_guard<py::gil_scoped_release>());
   m.def("matmul_4bit_scatter", &matmul_4bit_scatter, py::call_guard<py::gil_scoped_release>());
+  m.def("group_top_experts", &group_top_experts, py::call_guard<py::gil_scoped_release>());
+  m.def("group_top_experts_graph", &group_top_experts_graph, py::call_guard<py::gil_scoped_release>());
+  m.def("group_top_experts_backward", &group_top_experts_backward, py::call_guard<py::gil_scoped_release>());
+  m.def("quantize_8bit", &quantize_8bit, py::call_guard<py::gil_scoped_release>());
+  m.def("pack_8bit", &pack_8bit, py::call_guard<py::gil_scoped_release>());
+  m.def("dequantize_8bit", &dequantize_8bit, py::call_guard<py::gil_scoped_release>());
+  m.def("matmul_8bit", &matmul_8bit, py::call_guard<py::gil_scoped_release>());
+  m.def("gather_matmul_8bit", &gather_matmul_8bit, py::call_guard<py::gil_scoped_release>());
+  m.def("matmul_8bit_scatter", &matmul_8bit_scatter, py::call_guard<py::gil_scoped_release>());
+  m.def("linear_8bit_graph", &linear_8bit_graph, py::call_guard<py::gil_scoped_release>());
+  m.def("linear_8bit_forward", &linear_8bit_forward, py::call_guard<py::gil_scoped_release>());
+  m.def("linear_8bit_backward", [](const Tensor& grad, const Saved& saved, const OptTensor& bins, const std::vector<int64_t>& x_sizes, const std::vector<int64_t>& w_sizes,
+                                   bool want_x, bool want_w) { return linear_8bit_backward(grad, saved, bins, x_sizes, w_sizes, want_x, want_w); },
+        py::call_guard<py::gil_scoped_release>());
 }

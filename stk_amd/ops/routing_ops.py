@@ -70,6 +70,49 @@ def top_experts(scores, top_k, normalize=False):
     return hip_kernels.top_experts_graph(scores, top_k, normalize)
 
 
+class _GroupTopExperts(torch.autograd.Function):
+    """As _TopExperts."""
+
+    @staticmethod
+    def forward(ctx, scores, bias, *choice):
+        chosen, weights = hip_kernels.group_top_experts(scores, bias, *choice)
+        ctx.save_for_backward(scores, chosen, weights)
+        _, _, _, sigmoid, _, normalize, scale = choice
+        ctx.formula = sigmoid, normalize, scale
+        ctx.mark_non_differentiable(chosen)
+        return chosen, weights
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _, grad):
+        scores, chosen, weights = ctx.saved_tensors
+        return hip_kernels.group_top_experts_backward(scores, chosen, weights, grad, *ctx.formula), *(None,) * 8
+
+
+def group_top_experts(scores, top_k, groups=1, top_groups=1, scoring="sigmoid", bias=None, group_best=2, normalize=True, scale=1.0):
+    """A router's choice among groups of experts given scores [tokens, experts] on the GPU: (experts, weights), both [tokens, top_k].
+
+    With p the scores' softmax over all experts or their sigmoid (scoring), and c = p + bias (one value for each expert, to balance them; None: 0): the experts
+    are `groups` groups of equal size, neighbours; a group counts as the sum of its group_best (1 or 2) largest c; the top_groups groups that count most are
+    kept, ties to the lower group.  Where all groups are kept group_best has no say.
+    experts  int32, the top_k experts of these groups with the largest c (without a bias: the largest scores) in descending order, ties to the lower number: what
+             route takes
+    weights  fp32, scale times p - without the bias - at these places, with normalize divided by its sum over them: what padded_scatter takes;
+             differentiable with respect to the scores
+
+    scores float16, bfloat16 or float32, at most 1024 experts, 64 groups, the top 32.  Which experts are chosen does not depend on how p is rounded: what fp32 does
+    not tell apart is compared in 64 bits.  A score of -infinity masks an expert: it is chosen only where the kept groups have too few
+    others, and its weight is 0 (as every weight is where the sum of a normalised row is 0).  In a row with a NaN (softmax: or +infinity) the experts are valid
+    and distinct, and weights that it enters are NaN."""
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"unknown scoring {scoring!r}; one of ['sigmoid', 'softmax']")
+    best = group_best if top_groups < groups else 1
+    choice = top_k, groups, top_groups, scoring == "sigmoid", best, normalize, scale
+    if seen_by_python_only():
+        return _GroupTopExperts.apply(scores, bias, *choice)
+    return hip_kernels.group_top_experts_graph(scores, bias, *choice)
+
+
 class _PaddedGather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, route):
