@@ -1,0 +1,323 @@
+"""GPU parity of the 8-bit floating-point weights and their products against the 64-bit definition.
+
+Formats are exact.  Products are held to two measures.  Whole numbers of at most 8 under power-of-two scales of 1 are exact throughout - codes, products
+(at most 65536 in steps of 1024 as codes: below the 13 bits that the matrix units keep) and fp32 sums (below 2^24) - so that only the result's one
+rounding is left: equal bits.  Other values may be off by oracle.float8_oracle.slack_of, the activations' slopes (below 1.2) on it and errors
+(below 2^-20), and half a unit in the last place.
+"""
+import numpy as np
+import pytest
+import torch
+
+import stk_amd as stk
+from oracle import float8_oracle as F
+from stk_amd.backend import _lib
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+SMALL = {torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -24}
+ACT = {None: lambda v: v, "relu": torch.relu, "gelu": torch.nn.functional.gelu, "gelu_tanh": lambda v: torch.nn.functional.gelu(v, approximate="tanh"),
+       "silu": torch.nn.functional.silu}
+
+
+def _n64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _whole(shape, g, most=8):
+    """Whole numbers of up to `most`, which occurs."""
+    v = torch.randint(-most, most + 1, shape, generator=g).float()
+    v.view(-1)[::7] = most
+    return v
+
+
+def _check(got, sums, slack, dtype, activation=None, what=""):
+    want = ACT[activation](torch.from_numpy(np.ascontiguousarray(sums))).numpy()
+    assert got.dtype == dtype and tuple(got.shape) == want.shape, what
+    if activation:
+        slack = 1.2 * slack + 2.0 ** -20 * np.abs(sums)
+    bad = ~(np.abs(_n64(got) - want) <= 1.001 * HALF[dtype] * np.abs(want) + slack + SMALL[dtype])
+    assert not bad.any(), (what, int(bad.sum()), np.argwhere(bad)[0].tolist(), _n64(got)[bad][0], want[bad][0])
+
+
+# ---------------------------------------------------------------------------------------------------- formats
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", [(128, 128), (1, 1), (129, 65), (3, 200, 300), (2, 640, 17), (1, 1000, 64)])
+def test_quantize(shape, dtype):
+    g = torch.Generator().manual_seed(sum(shape))
+    w = (torch.randn(shape, generator=g) * torch.exp(torch.randn(shape, generator=g))).to(dtype)
+    w.view(-1)[::11] = 0
+    got = stk.ops.dequantize_8bit(stk.ops.quantize_8bit(w.to(DEV)), torch.float32)
+    want = np.stack([F.quantised(m, 128, 128)[0] for m in _n64(w).reshape(-1, *shape[-2:])]).reshape(shape)
+    assert np.array_equal(_n64(got), want)
+    # strides: the experts' slices of a wider matrix, and the transpose
+    other = w.transpose(-1, -2).contiguous().to(DEV).transpose(-1, -2)
+    assert torch.equal(stk.ops.quantize_8bit(other).packed, stk.ops.quantize_8bit(w.to(DEV)).packed)
+    wide = torch.zeros(*shape[:-1], shape[-1] + 3, dtype=dtype, device=DEV)
+    wide[..., 1:-2] = w.to(DEV)
+    assert torch.equal(stk.ops.quantize_8bit(wide[..., 1:-2]).packed, stk.ops.quantize_8bit(w.to(DEV)).packed)
+
+
+def test_quantize_extremes():
+    w = torch.zeros(256, 256)
+    w[:128, :128] = 2.0 ** -149        # a scale of 2^-126: nothing is left of them
+    w[:128, 128:] = 3e38
+    w[128:, :128] = 448 * 2.0 ** -126  # the smallest scale
+    w[200, 200] = 449.0
+    got = _n64(stk.ops.dequantize_8bit(stk.ops.quantize_8bit(w.to(DEV)), torch.float32))
+    assert np.array_equal(got, F.quantised(_n64(w), 128, 128)[0]) and got[130, 3] > 0 and got[200, 200] == 448
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        v = w.clone()
+        v[5, 200] = bad
+        got = _n64(stk.ops.dequantize_8bit(stk.ops.quantize_8bit(v.to(DEV)), torch.float32))
+        assert np.isnan(got[:128, 128:]).all() and np.isfinite(got[128:]).all() and np.isfinite(got[:128, :128]).all()
+
+
+@pytest.mark.parametrize("kind", ["float", "power"])
+@pytest.mark.parametrize("shape", [(128, 128), (1, 1), (130, 70), (2, 300, 129)])
+def test_pack(shape, kind):
+    g = torch.Generator().manual_seed(shape[-1])
+    codes = torch.randint(0, 256, shape, generator=g, dtype=torch.uint8)
+    codes[codes & 127 == 127] = 5
+    codes = codes.view(torch.float8_e4m3fn)
+    blocks = (*shape[:-2], (shape[-2] + 127) // 128, (shape[-1] + 127) // 128)
+    scales = torch.rand(blocks, generator=g) + 0.1 if kind == "float" else torch.randint(100, 140, blocks, generator=g, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+    got = stk.ops.dequantize_8bit(stk.ops.pack_8bit(codes.to(DEV), scales.to(DEV)), torch.float32)
+    wide = torch.repeat_interleave(torch.repeat_interleave(scales.float(), 128, -2), 128, -1)[..., :shape[-2], :shape[-1]]
+    assert torch.equal(got.cpu(), codes.float() * wide)
+    for dtype in (torch.bfloat16, torch.float16):
+        assert torch.equal(stk.ops.dequantize_8bit(stk.ops.pack_8bit(codes.to(DEV), scales.to(DEV)), dtype).cpu(), (codes.float() * wide).to(dtype))
+
+
+# ---------------------------------------------------------------------------------------------------- products
+SIZES = [(1, 128, 128), (1, 4096, 4096), (16, 300, 200), (5, 1, 1), (7, 129, 65), (17, 256, 1000), (33, 1151, 96), (40, 640, 4096), (64, 128, 64), (65, 2000, 130),
+         (200, 513, 333), (129, 1024, 4096), (700, 384, 2050), (2500, 96, 1030), (1000, 4096, 513), (16, 512, 8190), (3, 4000, 16384), (5000, 256, 4100)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,inputs,outputs", SIZES)
+def test_whole_numbers(rows, inputs, outputs, dtype):
+    g = torch.Generator().manual_seed(rows + inputs)
+    x, w = _whole((rows, inputs), g), _whole((inputs, outputs), g)
+    want = (x.double() @ w.double()).float().to(dtype)
+    got = stk.ops.matmul_8bit(x.to(dtype).to(DEV), stk.ops.quantize_8bit(w.to(dtype).to(DEV)))
+    assert torch.equal(got.cpu(), want)
+    scales = 2.0 ** torch.randint(-1, 2, ((inputs + 127) // 128, (outputs + 127) // 128), generator=g).float()
+    packed = stk.ops.pack_8bit(w.to(torch.float8_e4m3fn).to(DEV), scales.to(DEV))
+    wide = torch.from_numpy(F.blocks_of(scales.numpy(), inputs, outputs)).double()
+    assert torch.equal(stk.ops.matmul_8bit(x.to(dtype).to(DEV), packed).cpu(), (x.double() @ (w.double() * wide)).float().to(dtype))
+    powers = stk.ops.pack_8bit(w.to(torch.float8_e4m3fn).to(DEV), scales.to(torch.float8_e8m0fnu).to(DEV))
+    assert torch.equal(stk.ops.matmul_8bit(x.to(dtype).to(DEV), powers).cpu(), (x.double() @ (w.double() * wide)).float().to(dtype))
+
+
+@pytest.mark.parametrize("activation", [None, "relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,inputs,outputs", [(3, 520, 200), (40, 300, 130), (300, 1000, 400)])
+def test_products(rows, inputs, outputs, dtype, activation):
+    g = torch.Generator().manual_seed(rows)
+    x = (torch.randn(rows, inputs, generator=g) * torch.exp(torch.randn(inputs, generator=g))).to(dtype)
+    codes = (torch.randn(inputs, outputs, generator=g) * 80).clamp(-448, 448).to(torch.float8_e4m3fn)
+    scales = (torch.rand((inputs + 127) // 128, (outputs + 127) // 128, generator=g) + 0.5) * inputs ** -0.5 / 80
+    xq = F.quantised(_n64(x), 1, 128)[0]
+    wq = _n64(codes.float()) * F.blocks_of(_n64(scales), inputs, outputs)
+    got = stk.ops.matmul_8bit(x.to(DEV), stk.ops.pack_8bit(codes.to(DEV), scales.to(DEV)), activation)
+    _check(got, xq @ wq, F.slack_of(xq, wq), dtype, activation)
+    w = (torch.randn(inputs, outputs, generator=g) * inputs ** -0.5).to(dtype)
+    wq = F.quantised(_n64(w), 128, 128)[0]
+    _check(stk.ops.matmul_8bit(x.to(DEV), stk.ops.quantize_8bit(w.to(DEV)), activation), xq @ wq, F.slack_of(xq, wq), dtype, activation)
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_rows_of_any_stride(rows):
+    g = torch.Generator().manual_seed(rows)
+    x, w = _whole((rows, 300), g), _whole((300, 70), g)
+    packed, want = stk.ops.quantize_8bit(w.bfloat16().to(DEV)), (x @ w).bfloat16()
+    wide = torch.zeros(rows, 311, dtype=torch.bfloat16, device=DEV)
+    wide[:, 5:305] = x.to(DEV)
+    assert torch.equal(stk.ops.matmul_8bit(wide[:, 5:305], packed).cpu(), want)
+    turned = x.t().contiguous().bfloat16().to(DEV).t()
+    assert torch.equal(stk.ops.matmul_8bit(turned, packed).cpu(), want)
+    assert torch.equal(stk.ops.matmul_8bit(wide[:1, 5:305].expand(rows, 300), packed).cpu(), want[:1].expand(rows, 70))
+    assert torch.equal(stk.ops.matmul_8bit(wide[:, 5:305].reshape(1, rows, 300), packed).cpu(), want[None])
+
+
+@pytest.mark.parametrize("rows", [4, 40, 300])
+@pytest.mark.parametrize("activation", [None, "relu", "silu"])
+def test_rows_that_are_not_numbers(rows, activation):
+    g = torch.Generator().manual_seed(1)
+    x, w = torch.randn(rows, 300, generator=g).bfloat16(), torch.randn(300, 140, generator=g).bfloat16()
+    x[1, 7], x[2, 299], x[3, 130] = float("inf"), float("nan"), -float("inf")
+    got = stk.ops.matmul_8bit(x.to(DEV), stk.ops.quantize_8bit(w.to(DEV)), activation).cpu()
+    assert got[1:4].isnan().all() and torch.isfinite(got[0]).all() and torch.isfinite(got[4:]).all()
+
+
+@pytest.mark.parametrize("rows", [4, 40, 300])
+def test_weights_that_are_not_numbers(rows):
+    x = torch.randn(rows, 300, generator=torch.Generator().manual_seed(1)).bfloat16().to(DEV)
+    w = torch.ones(300, 300)
+    w[130, 140] = float("nan")
+    got = stk.ops.matmul_8bit(x, stk.ops.quantize_8bit(w.to(DEV))).cpu()
+    assert got[:, 128:256].isnan().all() and torch.isfinite(got[:, :128]).all() and torch.isfinite(got[:, 256:]).all()
+    codes = torch.ones(300, 300).to(torch.float8_e4m3fn).to(DEV)
+    for scales in (torch.ones(3, 3, device=DEV), torch.ones(3, 3, device=DEV).to(torch.float8_e8m0fnu)):
+        scales.view(torch.uint8 if scales.dtype != torch.float32 else torch.int32)[1, 2] = 255 if scales.dtype != torch.float32 else 0x7fc00000
+        got = stk.ops.matmul_8bit(x, stk.ops.pack_8bit(codes, scales)).cpu()
+        assert got[:, 256:].isnan().all() and torch.isfinite(got[:, :256]).all()
+        assert stk.ops.dequantize_8bit(stk.ops.pack_8bit(codes, scales))[128:256, 256:].isnan().all()
+
+
+def test_large_and_small_scales():
+    """Rows and weights whose scales meet far from 1."""
+    x, w = torch.full((20, 256), 2.0 ** 100), torch.full((256, 64), 2.0 ** -90)
+    for rows in (4, 20):
+        got = stk.ops.matmul_8bit(x[:rows].bfloat16().to(DEV), stk.ops.quantize_8bit(w.bfloat16().to(DEV)))
+        assert torch.equal(got.cpu(), torch.full((rows, 64), 2.0 ** 18).bfloat16())
+
+
+# ---------------------------------------------------------------------------------------------------- routed
+def _route(tokens, experts, top_k, how, blocking, seed):
+    g = torch.Generator().manual_seed(seed)
+    if how == "one":
+        top = torch.zeros(tokens, top_k, dtype=torch.int32) + experts // 2
+    else:
+        top = torch.randint(0, experts if how == "any" else max(1, experts // 2), (tokens, top_k), generator=g, dtype=torch.int32)
+    return stk.ops.route(top.to(DEV), experts, blocking)
+
+
+ROUTED = [(1, 4, 1, 128, 16, "any", 1), (1, 64, 2, 256, 48, "any", 128), (3, 4, 4, 200, 33, "any", 1), (64, 64, 2, 256, 64, "any", 1), (100, 8, 2, 384, 100, "half", 1),
+          (50, 200, 1, 64, 16, "any", 1), (300, 4, 1, 130, 40, "one", 1), (33, 16, 3, 512, 80, "any", 64), (500, 6, 2, 256, 96, "half", 1), (17, 1, 1, 128, 20, "any", 1),
+          (40, 32, 8, 96, 24, "any", 1), (5, 1024, 2, 32, 16, "any", 1), (2000, 3, 1, 160, 144, "any", 128), (160, 64, 2, 136, 1120, "any", 1),
+          (600, 16, 2, 264, 528, "half", 1), (3000, 8, 2, 264, 1040, "any", 1), (2, 4, 2, 3200, 700, "any", 1), (900, 8, 1, 137, 1040, "half", 1), (4000, 64, 1, 256, 1100, "any", 1), (64, 64, 1, 257, 500, "any", 1)]
+
+
+@pytest.mark.parametrize("kind", ["power", "float"])
+@pytest.mark.parametrize("tokens,experts,top_k,inputs,outputs,how,blocking", ROUTED)
+def test_routed_products(tokens, experts, top_k, inputs, outputs, how, blocking, kind):
+    """Whole numbers: equal bits."""
+    g = torch.Generator().manual_seed(tokens + experts)
+    dtype = torch.float16 if tokens % 2 else torch.bfloat16
+    x, h, w = _whole((tokens, inputs), g), _whole((tokens * top_k, inputs), g), _whole((experts, inputs, outputs), g)
+    by = 2.0 ** torch.randint(-2, 2, (tokens, top_k), generator=g).float()
+    if kind == "power":
+        packed = stk.ops.quantize_8bit(w.to(dtype).to(DEV))
+    else:
+        packed = stk.ops.pack_8bit(w.to(torch.float8_e4m3fn).to(DEV), torch.ones(experts, (inputs + 127) // 128, (outputs + 127) // 128, device=DEV))
+    r = _route(tokens, experts, top_k, how, blocking, tokens)
+    indices, bins = r.indices.cpu().long(), r.bins.cpu()
+    expert = torch.searchsorted(bins, torch.arange(tokens * top_k, dtype=torch.int32), right=True)
+    sums, back = torch.empty(tokens * top_k, outputs).double(), torch.empty(tokens * top_k, outputs).double()
+    for e in expert.unique().tolist():
+        at = expert == e
+        sums[at], back[indices[at]] = x[indices[at] // top_k].double() @ w[e].double(), h[at].double() @ w[e].double()
+    for act in (None, "relu"):
+        assert torch.equal(stk.ops.gather_matmul_8bit(x.to(dtype).to(DEV), r, packed, act).cpu(), ACT[act](sums).float().to(dtype))
+    for weights in (by, None):
+        want = (back.view(tokens, top_k, outputs) * (1.0 if weights is None else weights.double().unsqueeze(2))).sum(1)
+        got = stk.ops.matmul_8bit_scatter(h.to(dtype).to(DEV), r, packed, None if weights is None else weights.to(DEV))
+        assert torch.equal(got.cpu(), want.float().to(dtype))
+
+
+def test_every_kernel_is_reached():
+    lib = _lib.load()
+    seen = {lib.stk_8bit_product_kernel(r, 1, i, o) for r, i, o in SIZES} | {lib.stk_8bit_product_kernel(c[0] * c[2], *c[1:2], *c[3:5]) for c in ROUTED}
+    possible = {lib.stk_8bit_product_kernel(r, e, i, o) for r in (1, 16, 17, 40, 65, 100, 300, 1000, 5000, 20000, 100000) for e in (1, 8, 64, 256)
+                for i in (64, 1024, 4096) for o in (16, 256, 1024, 4096)}
+    assert seen == possible
+
+
+def test_skewed_experts_of_many_rows():
+    """One expert with most of the rows, others with one or none."""
+    g = torch.Generator().manual_seed(9)
+    top = torch.zeros(3000, 1, dtype=torch.int32)
+    top[::100, 0] = torch.arange(30, dtype=torch.int32) % 8
+    x, w = _whole((3000, 256), g), _whole((8, 256, 512), g)
+    r = stk.ops.route(top.to(DEV), 8, 1)
+    packed = stk.ops.quantize_8bit(w.bfloat16().to(DEV))
+    want = torch.empty(3000, 512)
+    for p, s in enumerate(r.indices.cpu().tolist()):
+        want[p] = (x[s].double() @ w[int(top[s])].double()).float()
+    assert torch.equal(stk.ops.gather_matmul_8bit(x.bfloat16().to(DEV), r, packed).cpu(), want.bfloat16())
+
+
+def test_experts_without_rows_are_not_read():
+    w = torch.ones(8, 128, 32)
+    w[[0, 2, 3, 7]] = float("nan")
+    packed = stk.ops.quantize_8bit(w.to(DEV))
+    top = torch.tensor([[1, 4], [5, 6], [6, 1]], dtype=torch.int32, device=DEV)
+    for repeat in (1, 40):
+        r = stk.ops.route(top.repeat(repeat, 1), 8, 1)
+        x = torch.randn(3 * repeat, 128, generator=torch.Generator().manual_seed(2)).bfloat16().to(DEV)
+        assert torch.isfinite(stk.ops.gather_matmul_8bit(x, r, packed)).all()
+        assert torch.isfinite(stk.ops.matmul_8bit_scatter(x.repeat(2, 1), r, packed)).all()
+
+
+def test_no_rows():
+    packed = stk.ops.quantize_8bit(torch.ones(4, 128, 32, device=DEV))
+    r = stk.ops.route(torch.zeros(0, 2, dtype=torch.int32, device=DEV), 4, 1)
+    none = torch.empty(0, 128, device=DEV, dtype=torch.bfloat16)
+    assert stk.ops.gather_matmul_8bit(none, r, packed).shape == (0, 32) and stk.ops.matmul_8bit_scatter(none, r, packed).shape == (0, 32)
+    assert stk.ops.matmul_8bit(none, stk.ops.quantize_8bit(torch.ones(128, 32, device=DEV))).shape == (0, 32)
+
+
+@pytest.mark.parametrize("tokens", [40, 2000])
+def test_streams_and_graphs(tokens):
+    g = torch.Generator().manual_seed(3)
+    w1 = stk.ops.quantize_8bit(torch.randn(8, 512, 256, generator=g).to(DEV))
+    w2 = stk.ops.pack_8bit((torch.randn(8, 256, 512, generator=g) * 80).clamp(-448, 448).to(torch.float8_e4m3fn).to(DEV), torch.rand(8, 2, 4, generator=g).to(DEV))
+    x, by = torch.randn(tokens, 512, generator=g).bfloat16().to(DEV), torch.rand(tokens, 2, generator=g).to(DEV)
+    scores = torch.randn(tokens, 8, generator=g).to(DEV)
+
+    def layer():
+        top, weights = stk.ops.group_top_experts(scores, 2, groups=4, top_groups=2, bias=by[:8, 0].contiguous())
+        r = stk.ops.route(top, 8, 1, padded_rows=2 * tokens)
+        return stk.ops.matmul_8bit_scatter(stk.ops.gather_matmul_8bit(x, r, w1, "gelu"), r, w2, weights)
+
+    want = layer()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = layer()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = layer()
+    for replay in range(3):
+        x.copy_(torch.randn(x.shape, generator=g)), scores.copy_(torch.randn(scores.shape, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, layer()), replay
+
+
+def test_autocast():
+    g = torch.Generator().manual_seed(4)
+    x, w = _whole((5, 128), g).to(DEV), stk.ops.quantize_8bit(_whole((128, 64), g).to(DEV))
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert torch.equal(stk.ops.matmul_8bit(x, w), stk.ops.matmul_8bit(x.bfloat16(), w))
+
+
+def test_refusals():
+    w = stk.ops.quantize_8bit(torch.ones(128, 32, device=DEV))
+    experts = stk.ops.quantize_8bit(torch.ones(4, 128, 32, device=DEV))
+    x = torch.zeros(3, 128, dtype=torch.bfloat16, device=DEV)
+    r = stk.ops.route(torch.zeros(3, 1, dtype=torch.int32, device=DEV), 4, 1)
+    other = stk.ops.route(torch.zeros(3, 1, dtype=torch.int32, device=DEV), 5, 1)
+    codes, scales = torch.zeros(128, 32, device=DEV).to(torch.float8_e4m3fn), torch.ones(1, 1, device=DEV)
+    for call in (lambda: stk.ops.matmul_8bit(x[:, :127], w), lambda: stk.ops.matmul_8bit(x, experts), lambda: stk.ops.gather_matmul_8bit(x, r, w),
+                 lambda: stk.ops.gather_matmul_8bit(x[:2], r, experts), lambda: stk.ops.gather_matmul_8bit(x, other, experts),
+                 lambda: stk.ops.matmul_8bit_scatter(x[:2], r, experts), lambda: stk.ops.matmul_8bit_scatter(x, r, experts, torch.ones(4, 1, device=DEV)),
+                 lambda: stk.ops.pack_8bit(codes, scales[:0]), lambda: stk.ops.pack_8bit(codes, torch.ones(2, 1, device=DEV)),
+                 lambda: stk.ops.matmul_8bit(x, w._replace(outputs=65)), lambda: stk.ops.matmul_8bit(x, w._replace(scales=w.scales[:, 1:])),
+                 lambda: stk.ops.quantize_8bit(torch.ones(0, 32, device=DEV))):
+        with pytest.raises(AssertionError):
+            call()
+    for call in (lambda: stk.ops.matmul_8bit(x.float(), w), lambda: stk.ops.pack_8bit(codes.float(), scales), lambda: stk.ops.pack_8bit(codes, scales.half()),
+                 lambda: stk.ops.matmul_8bit(x.clone().requires_grad_(), w), lambda: stk.ops.quantize_8bit(torch.ones(128, 32, device=DEV, dtype=torch.float64)),
+                 lambda: stk.ops.matmul_8bit_scatter(x, r, experts, torch.ones(3, 1, device=DEV, requires_grad=True))):
+        with pytest.raises(NotImplementedError):
+            call()
+    with pytest.raises(ValueError):
+        stk.ops.matmul_8bit(x, w, "tanh")
+    with pytest.raises(RuntimeError):
+        stk.ops.matmul_8bit(x.cpu(), w)
