@@ -6,8 +6,8 @@
 //
 // Pieces: the operand that all rows share, 16 of its lines x 128 inputs in 2048 bytes, in the order of a wavefront's two 16-byte accesses:
 // access h, lane l has inputs 64 h + 16 (l / 16) .. + 15 of line l % 16.  (Which input goes where in v_mfma_scale_f32_16x16x128 does not
-// matter as long as both operands agree, and all inputs of a block have one scale.)  Pieces follow each other along the inputs, then along
-// the lines, then expert by expert.  Lines are dealt to the pieces of 64 so that the four sums that a lane has of each of four pieces belong to
+// matter as long as both operands agree, and all inputs of a block have one scale.)  The four pieces of 64 lines lie next to each other, then
+// follow those of the next block, of the next 64 lines, of the next expert.  Lines are dealt to the pieces of 64 so that the four sums that a lane has of each of four pieces belong to
 // 16 neighbouring lines: line 16 q + 4 t + r of the 64 is line 4 q + r of piece t.  Lines are padded to a multiple of 64 with zeros.
 // Scales of pieces: exponent bytes [place of the line][blocks rounded up to 4] ("power"), or fp32 [ceil(lines / 128)][blocks] ("float").
 #pragma once
@@ -21,6 +21,7 @@ enum Scales8 : int { kPowerScales = 0, kFloatScales = 1 };
 
 __host__ __device__ inline int64_t blocks8(int64_t size) { return (size + kBlock8 - 1) / kBlock8; }
 __host__ __device__ inline int64_t exponent_stride8(int64_t size) { return (blocks8(size) + 3) / 4 * 4; }
+__host__ __device__ inline int64_t row_stride8(int64_t size) { return blocks8(size) * kBlock8; }
 __host__ __device__ inline int64_t padded_lines8(int64_t lines) { return (lines + kGroupLines8 - 1) / kGroupLines8 * kGroupLines8; }
 __host__ __device__ inline int64_t piece_bytes8(int64_t lines, int64_t size) { return padded_lines8(lines) / kPieceLines8 * blocks8(size) * kPieceBytes8; }
 __host__ __device__ inline int64_t scale_bytes8(int64_t lines, int64_t size, int kind) {
@@ -28,9 +29,11 @@ __host__ __device__ inline int64_t scale_bytes8(int64_t lines, int64_t size, int
 }
 // Place of a line among those of its pieces.
 __host__ __device__ inline int64_t place8(int64_t line) { return (line & ~(int64_t)63) + ((line >> 2) & 3) * 16 + ((line >> 4) & 3) * 4 + (line & 3); }
+// Piece p (16 places) of a block, in pieces from the start of an operand.
+__host__ __device__ inline int64_t piece8(int64_t p, int64_t block, int64_t blocks) { return ((p >> 2) * blocks + block) * 4 + (p & 3); }
 // Byte of (place, input) from the start of an operand's pieces; `blocks` of them along the inputs.
 __host__ __device__ inline int64_t piece_at8(int64_t place, int64_t input, int64_t blocks) {
-  const int64_t piece = place / kPieceLines8 * blocks + input / kBlock8;
+  const int64_t piece = piece8(place / kPieceLines8, input / kBlock8, blocks);
   const int k = (int)(input % kBlock8);
   return piece * kPieceBytes8 + (k >> 6) * 1024 + ((int)(place & 15) + 16 * ((k & 63) >> 4)) * 16 + (k & 15);
 }

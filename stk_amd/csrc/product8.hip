@@ -11,137 +11,10 @@
 #include "common.h"
 #include "fp8.h"
 #include "gemm_core.h"
+#include "product8.h"
 #include "values.h"
-#include "wave_scan.h"
 
 namespace stk {
-
-bool sizes8(int64_t lines, int64_t size);
-int quantize_rows8(const char* who, const void* x, int64_t rows, int64_t size, int64_t stride, int dtype, uint8_t* codes, uint8_t* exponents, hipStream_t stream);
-
-typedef int i32x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
-
-// What a product is told.  Without routing: bins null, one expert.  With: row p of the sorted slots belongs to the first expert whose bin
-// ends behind p, and to the slot indices[p].
-struct Product8 {
-  const void* x;                             // 16-bit rows, ...
-  int64_t x_stride;
-  const uint8_t *codes, *exponents;          // ... or quantised ones
-  int64_t x_rows, rows;                      // rows there are; those multiplied (slots)
-  const uint8_t* packed;
-  const void* scales;
-  int64_t experts, inputs, outputs;
-  const int32_t *indices, *bins;
-  int top_k;                                 // gathered: row p reads token indices[p] / top_k; 0: row p itself
-  void* out;                                 // 16-bit rows in the order of the rows, or with `by_slot` of the slots, times `weights` of these, ...
-  int64_t out_stride;
-  bool by_slot;
-  const float* weights;
-  float* sums;                               // ... or, where given, fp32 rows [slot][outputs]
-  int activation;
-  bool bf16, zero_behind;                    // zero_behind: rows behind the last bin become zeros
-};
-
-// Which rows a tile of up to R rows of one expert is: tiles are numbered expert by expert, an expert of c rows has ceil(c / R).
-struct RowTile8 {
-  int expert, first, rows;   // (rows 0: no such tile, but the first-th behind them all)
-};
-template <int R>
-__device__ __forceinline__ RowTile8 row_tile8(const Product8& p, int tile, int lane) {
-  if (!p.bins) {
-    const int64_t first = (int64_t)tile * R, left = p.rows - first;
-    return {0, (int)first, left <= 0 ? 0 : left < R ? (int)left : R};
-  }
-  int before = 0;
-  for (int e0 = 0; e0 < p.experts; e0 += 64) {
-    const int e = e0 + lane;
-    const bool is = e < p.experts;
-    // (bins that do not ascend or leave the rows are kept inside them)
-    const int hi = is ? min(max(p.bins[e], 0), (int)p.rows) : 0, lo = is && e > 0 ? min(max(p.bins[e - 1], 0), (int)p.rows) : 0;
-    const int count = hi > lo ? hi - lo : 0, tiles = (count + R - 1) / R, upto = before + wave_inclusive_scan(tiles, lane);
-    const uint64_t mine = __ballot(upto > tile);
-    if (mine) {
-      const int at = __builtin_ctzll(mine);
-      const int inside = tile - __builtin_amdgcn_readlane(upto - tiles, at), c = __builtin_amdgcn_readlane(count, at);
-      return {e0 + at, __builtin_amdgcn_readlane(lo, at) + inside * R, min(c - inside * R, R)};
-    }
-    before = __builtin_amdgcn_readlane(upto, 63);
-  }
-  return {0, tile - before, 0};
-}
-
-__device__ __forceinline__ f32x4_t multiply8(i32x8_t weights, i32x8_t rows, f32x4_t sum, int weight_scale, int row_scale) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(weights, rows, sum, 0, 0, 0, weight_scale, 0, row_scale);
-}
-
-// total = activation(total); a NaN stays one (relu by the comparison from the other side would make 0 of it).
-template <int KIND, int N>
-__device__ __forceinline__ void activate_each8(f32x4_t (&total)[N]) {
-#pragma unroll
-  for (int n = 0; n < N; n++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float v = total[n][i];
-      total[n][i] = KIND == kRelu ? (v <= 0.f ? 0.f : v) : activate<KIND>(v);
-    }
-}
-template <int N>
-__device__ __forceinline__ void activate_sums8(f32x4_t (&total)[N], int kind) {
-  switch (kind) {
-    case kRelu: activate_each8<kRelu>(total); break;
-    case kGeluTanh: activate_each8<kGeluTanh>(total); break;
-    case kGeluErf: activate_each8<kGeluErf>(total); break;
-    case kSilu: activate_each8<kSilu>(total); break;
-    default: break;
-  }
-}
-__device__ __forceinline__ uint32_t pack8(float a, float b, bool bf16) { return bf16 ? pack2<true>(a, b) : pack2<false>(a, b); }
-
-// Where row r of a tile is stored, or false.
-__device__ __forceinline__ bool place_of_row8(const Product8& p, const RowTile8& t, int r, int64_t& to, float& by) {
-  if (r >= t.rows) return false;
-  to = t.first + r, by = 1.f;
-  if (p.sums || p.by_slot) {
-    to = p.indices[to];
-    if (to < 0 || to >= p.rows) return false;
-    if (!p.sums && p.weights) by = p.weights[to];
-  }
-  return true;
-}
-// N x 4 neighbouring outputs of a row from `first` on.
-template <int N>
-__device__ __forceinline__ void store8(const Product8& p, int64_t to, float by, int64_t first, const f32x4_t (&v)[N]) {
-  const int here = (int)min(p.outputs - first, (int64_t)(4 * N));
-  if (here <= 0) return;
-  if (p.sums) {
-    float* at = p.sums + to * p.outputs + first;
-    if (here == 4 * N) {
-#pragma unroll
-      for (int n = 0; n < N; n++) *reinterpret_cast<QuadAt4*>(at + 4 * n) = __builtin_bit_cast(Quad, v[n]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4 * N; i++)
-        if (i < here) at[i] = v[i / 4][i % 4];
-    }
-    return;
-  }
-  uint32_t two[2 * N];
-#pragma unroll
-  for (int i = 0; i < 2 * N; i++) two[i] = pack8(v[i / 2][2 * (i & 1)] * by, v[i / 2][2 * (i & 1) + 1] * by, p.bf16);
-  uint16_t* at = static_cast<uint16_t*>(p.out) + to * p.out_stride + first;
-  if (here == 4 * N) {
-    if constexpr (N == 1) *reinterpret_cast<PairAt2*>(at) = PairAt2{two[0], two[1]};
-    else {
-#pragma unroll
-      for (int n = 0; n < N; n += 2) *reinterpret_cast<QuadAt2*>(at + 4 * n) = QuadAt2{two[2 * n], two[2 * n + 1], two[2 * n + 2], two[2 * n + 3]};
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4 * N; i++)
-      if (i < here) at[i] = (uint16_t)(two[i / 2] >> (16 * (i & 1)));
-  }
-}
 
 // ------------------------------------------------------------------------------------------------ few rows
 // 128 values of a row, of which this lane has 64 h + 16 quarter .. + 15, quantised together with the lanes 16, 32 and 48 away.
@@ -221,8 +94,8 @@ __global__ __launch_bounds__(64 * KW * NW) void stream8_kernel(Product8 p) {
 #pragma unroll
   for (int n = 0; n < NT; n++) {
     tile[n] = ((int)blockIdx.x * NW + nw) * NT + n;
-    const int64_t at = (int64_t)t.expert * down + min(tile[n], down - 1);
-    weights[n] = reinterpret_cast<const u32x4*>(p.packed + at * along * kPieceBytes8) + lane;
+    const int64_t piece = min(tile[n], down - 1), at = (int64_t)t.expert * down + piece;
+    weights[n] = reinterpret_cast<const u32x4*>(p.packed + ((int64_t)t.expert * down * along + piece8(piece, 0, along)) * kPieceBytes8) + lane;
     // (the lines of a piece have one scale)
     if constexpr (KIND == kPowerScales) scales[n] = const_ints(static_cast<const uint8_t*>(p.scales) + at * kPieceLines8 * exponent_stride8(p.inputs));
     else scales[n] = const_ints(static_cast<const float*>(p.scales) + ((int64_t)t.expert * blocks8(p.outputs) + min(tile[n], down - 1) / 8) * along);
@@ -235,7 +108,7 @@ __global__ __launch_bounds__(64 * KW * NW) void stream8_kernel(Product8 p) {
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
-      for (int h = 0; h < 2; h++) g.w[n][h] = __builtin_nontemporal_load(weights[n] + (int64_t)block * (kPieceBytes8 / 16) + 64 * h);
+      for (int h = 0; h < 2; h++) g.w[n][h] = __builtin_nontemporal_load(weights[n] + (int64_t)block * (4 * kPieceBytes8 / 16) + 64 * h);
       if constexpr (KIND == kPowerScales) g.scale[n] = scales[n][block >> 2] >> (8 * (block & 3));
       else g.scale[n] = scales[n][block];
     }
@@ -303,19 +176,6 @@ __global__ __launch_bounds__(64 * KW * NW) void stream8_kernel(Product8 p) {
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
-// 16, or 4, bytes per lane from any addresses into the LDS bytes from lds_base on, lane after lane.
-__device__ __forceinline__ void dma16_from(const void* from, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(uniform((int)lds_base)), "v"((uint64_t)from) : "memory", "m0");
-}
-__device__ __forceinline__ void dma4_from(const void* from, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(uniform((int)lds_base)), "v"((uint64_t)from) : "memory", "m0");
-}
-
-// What the gradient of the weights is told beside: dw[e][i][o] = the sum over the rows r of expert e of xq[r][i] gq[r][o].  codes: the columns of x
-// (a line for each input, row blocks along it), packed: those of g as pieces; outputs, out: those of dw, x_rows its inputs, `inputs` the rows.
-// Otherwise a product of rows.
-enum What8 : int { kRows8 = 0, kGradient8 = 1 };
-
 // WM x WN wavefronts share 16 MT WM rows and 64 WN outputs, a block of 128 inputs at a time in two stages of LDS that are filled without
 // registers: pieces of weights as they lie in memory, rows 64 bytes at a time in the same order, so that every fragment is two
 // accesses of neighbouring lanes.  Exponents come four blocks at a time.
@@ -376,7 +236,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
 #pragma unroll
   for (int j = 0; j < kRowMoves; j++) {
     const int q = wave + T::kWaves * j;
-    row_from[j] = p.codes + source_row(16 * (q >> 1) + row) * ((int64_t)blocks * kBlock8) + 64 * (q & 1) + 16 * quarter;
+    row_from[j] = p.codes + source_row(16 * (q >> 1) + row) * row_stride8(p.inputs) + 64 * (q & 1) + 16 * quarter;
   }
   const int64_t matrix = WHAT == kGradient8 ? 0 : t.expert;
   gptr_t col_from[kColMoves];
@@ -384,7 +244,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
   for (int j = 0; j < kColMoves; j++) {
     const int q = wave + T::kWaves * j;
     const int64_t piece = min(col0 / kPieceLines8 + (q >> 1), places / kPieceLines8 - 1);
-    col_from[j] = uniform_global(p.packed + (matrix * (places / kPieceLines8) + piece) * blocks * kPieceBytes8 + 1024 * (q & 1));
+    col_from[j] = uniform_global(p.packed + (matrix * (places / kPieceLines8) * blocks + piece8(piece, 0, blocks)) * kPieceBytes8 + 1024 * (q & 1));
   }
   // exponents: 64 lines a transfer, first those of the rows
   constexpr int kScaleMoves = (kChunks + T::kWaves - 1) / T::kWaves;
@@ -396,14 +256,14 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
     else scale_from[j] = static_cast<const uint8_t*>(p.scales) + (matrix * places + min(col0 + 64 * (c - kRowChunks) + lane, places - 1)) * exponent_stride;
   }
   const uint32_t lds = (uint32_t)(uintptr_t)(STK_LDS char*)smem;
-  const auto issue = [&](int block, int stage) {
+  const auto issue = [&](int block, int stage, bool exponents_too, int place) {
     const uint32_t to = lds + stage * T::kStage;
 #pragma unroll
     for (int j = 0; j < kRowMoves; j++) dma16_from(row_from[j] + (int64_t)block * kBlock8, to + (wave + T::kWaves * j) * 1024);
 #pragma unroll
-    for (int j = 0; j < kColMoves; j++) dma16(col_from[j] + (int64_t)block * kPieceBytes8, lane * 16, to + T::kRowBytes + (wave + T::kWaves * j) * 1024);
-    if (block == begin || (block & 3) == 0) {
-      const uint32_t exponents = lds + 2 * T::kStage + ((block >> 2) & 1) * T::kExponents;
+    for (int j = 0; j < kColMoves; j++) dma16(col_from[j] + (int64_t)block * (4 * kPieceBytes8), lane * 16, to + T::kRowBytes + (wave + T::kWaves * j) * 1024);
+    if (exponents_too) {
+      const uint32_t exponents = lds + 2 * T::kStage + place * T::kExponents;
 #pragma unroll
       for (int j = 0; j < kScaleMoves; j++) {
         const int c = wave + T::kWaves * j;
@@ -420,16 +280,24 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
 #pragma unroll
     for (int n = 0; n < 4; n++) total[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   int row_scale[MT], col_scale[4] = {127, 127, 127, 127};
-  if (begin < end) issue(begin, 0);
-  for (int block = begin; block < end; block++) {
-    const int stage = (block - begin) & 1;
+  // this wavefront's rows are fragments wm, wm + WM, ... of 16, of which so many have any
+  const int fragments = ((t.rows + 15) / 16 - wm + WM - 1) / WM;
+  // Column tiles start at different blocks and go round: those of one block lie a fixed distance apart, which would all be in a few of the memory's channels.
+  const int count = end - begin;
+  int block = begin, place = 0;   // place: of the exponents in use
+  bool fresh = true;
+  if (count > 0) issue(block, 0, true, 0);
+  for (int step = 0; step < count; step++) {
+    const int stage = step & 1;
     wait_vmcnt<0>();
     __syncthreads();   // everybody's part of the block is there, and everybody is done with the one whose place is filled now
-    if (block + 1 < end) issue(block + 1, stage ^ 1);
-    if (block == begin || (block & 3) == 0) {
-      const int* exponents = reinterpret_cast<const int*>(smem + 2 * T::kStage + ((block >> 2) & 1) * T::kExponents);
+    const int next = block + 1 < end ? block + 1 : begin;
+    const bool next_fresh = next == begin || (next & 3) == 0;
+    if (step + 1 < count) issue(next, stage ^ 1, next_fresh, place ^ 1);
+    if (fresh) {
+      const int* exponents = reinterpret_cast<const int*>(smem + 2 * T::kStage + place * T::kExponents);
 #pragma unroll
-      for (int m = 0; m < MT; m++) row_scale[m] = exponents[16 * (wm * MT + m) + row] >> (8 * (block & 3));
+      for (int m = 0; m < MT; m++) row_scale[m] = exponents[16 * (m * WM + wm) + row] >> (8 * (block & 3));
       if constexpr (KIND == kPowerScales) {
 #pragma unroll
         for (int n = 0; n < 4; n++) col_scale[n] = exponents[T::kRows + 64 * wn + 16 * n + row] >> (8 * (block & 3));
@@ -443,7 +311,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
       }
     }
     const float by = KIND == kFloatScales ? __uint_as_float((uint32_t)const_ints(float_scales)[block]) : 1.f;
-    const u32x4* rows = reinterpret_cast<const u32x4*>(smem + stage * T::kStage) + wm * MT * (kPieceBytes8 / 16) + lane;
+    const u32x4* rows = reinterpret_cast<const u32x4*>(smem + stage * T::kStage) + wm * (kPieceBytes8 / 16) + lane;
     const u32x4* cols = reinterpret_cast<const u32x4*>(smem + stage * T::kStage + T::kRowBytes) + wn * 4 * (kPieceBytes8 / 16) + lane;
     const auto fragment = [&](const u32x4* from) {
       i32x8_t f;
@@ -452,22 +320,32 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
       for (int i = 0; i < 4; i++) f[i] = (int)a[i], f[4 + i] = (int)b[i];
       return f;
     };
-    i32x8_t w[4];
+    // The fragment of the next 16 rows is on its way while one is multiplied; with fp32 scales the sums of one are scaled while the next is.  What lies
+    // behind the last row of a tile is left out.
+    i32x8_t w[4], values[2];
+    values[0] = fragment(rows);
 #pragma unroll
     for (int n = 0; n < 4; n++) w[n] = fragment(cols + n * (kPieceBytes8 / 16));
 #pragma unroll
     for (int m = 0; m < MT; m++) {
-      const i32x8_t values = fragment(rows + m * (kPieceBytes8 / 16));
+      if (m >= fragments) break;
+      if (m + 1 < MT) values[(m + 1) & 1] = fragment(rows + (m + 1) * WM * (kPieceBytes8 / 16));
+      f32x4_t part[4];
 #pragma unroll
       for (int n = 0; n < 4; n++) {
-        if constexpr (KIND == kPowerScales) total[m][n] = multiply8(w[n], values, total[m][n], col_scale[n], row_scale[m]);
-        else {
-          const f32x4_t part = multiply8(w[n], values, f32x4_t{0.f, 0.f, 0.f, 0.f}, 127, row_scale[m]);
-#pragma unroll
-          for (int i = 0; i < 4; i++) total[m][n][i] = fmaf(part[i], by, total[m][n][i]);
-        }
+        if constexpr (KIND == kPowerScales) total[m][n] = multiply8(w[n], values[m & 1], total[m][n], col_scale[n], row_scale[m]);
+        else part[n] = multiply8(w[n], values[m & 1], f32x4_t{0.f, 0.f, 0.f, 0.f}, 127, row_scale[m]);
       }
+      if constexpr (KIND == kFloatScales) {
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) total[m][n][i] = fmaf(part[n][i], by, total[m][n][i]);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // (the accesses to LDS come first)
+      __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
     }
+    block = next, fresh = next_fresh, place ^= (int)next_fresh;
   }
   const int64_t first = col0 + 64 * wn + 16 * quarter;
   if constexpr (WHAT == kGradient8) p.out = static_cast<uint16_t*>(p.out) + (int64_t)expert * p.x_rows * p.out_stride;
@@ -476,7 +354,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
     if constexpr (WHAT == kRows8) activate_sums8(total[m], p.activation);
     int64_t to;
     float by;
-    if (place_of_row8(p, t, 16 * (wm * MT + m) + row, to, by)) store8<4>(p, to, by, first, total[m]);
+    if (place_of_row8(p, t, 16 * (m * WM + wm) + row, to, by)) store8<4>(p, to, by, first, total[m]);
   }
 }
 
@@ -574,7 +452,7 @@ static ProductKernel8 product_kernel8(int64_t rows, int64_t experts, int64_t inp
 }
 static int64_t workspace8(int64_t x_rows, int64_t rows, int64_t experts, int64_t inputs, int64_t outputs) {
   if (rows < 1 || product_kernel8(rows, experts, inputs, outputs) < kTile8_32) return 0;
-  return (x_rows * (blocks8(inputs) * kBlock8 + exponent_stride8(inputs)) + 255) / 256 * 256;
+  return (x_rows * (row_stride8(inputs) + exponent_stride8(inputs)) + 255) / 256 * 256;
 }
 template <int WHAT>
 static int launch_tiles8(const char* who, const Product8& p, int kind, ProductKernel8 kernel, hipStream_t stream) {
@@ -582,7 +460,7 @@ static int launch_tiles8(const char* who, const Product8& p, int kind, ProductKe
     case kTile8_32: return launch_tiles8<WHAT, 2, 2, 1>(who, p, kind, stream);
     case kTile8_64: return launch_tiles8<WHAT, 2, 2, 2>(who, p, kind, stream);
     case kTile8_128: return launch_tiles8<WHAT, 2, 2, 4>(who, p, kind, stream);
-    default: return launch_tiles8<WHAT, 2, 4, 8>(who, p, kind, stream);
+    default: return kind == kPowerScales ? launch_wide8<WHAT>(who, p, stream) : launch_tiles8<WHAT, 2, 4, 8>(who, p, kind, stream);
   }
 }
 // The product of 16-bit rows; the workspace holds them quantised where there are many.
@@ -590,7 +468,7 @@ static int launch_product8(const char* who, Product8 p, int kind, int dtype, voi
   const ProductKernel8 kernel = product_kernel8(p.rows, p.experts, p.inputs, p.outputs);
   if (kernel >= kTile8_32) {
     uint8_t* codes = static_cast<uint8_t*>(workspace);
-    uint8_t* exponents = codes + p.x_rows * blocks8(p.inputs) * kBlock8;
+    uint8_t* exponents = codes + p.x_rows * row_stride8(p.inputs);
     if (int rc = quantize_rows8(who, p.x, p.x_rows, p.inputs, p.x_stride, dtype, codes, exponents, stream)) return rc;
     p.codes = codes, p.exponents = exponents;
     return launch_tiles8<kRows8>(who, p, kind, kernel, stream);

@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const typename Value
     for (int j = 0; j < 8; j++) most = larger_bits(most, __float_as_uint(v[j]) & 0x7fffffffu);
     most = team16_larger(most);
     const int byte = exponent_byte8(most);
-    *reinterpret_cast<uint2*>(codes + row * (blocks * kBlock8) + first) = eight_codes(v, most, inverse_power8(byte));
+    *reinterpret_cast<uint2*>(codes + row * row_stride8(size) + first) = eight_codes(v, most, inverse_power8(byte));
     if (lane == 0) exponents[row * along + block] = (uint8_t)byte;
   }
 }
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(Quantize8 p) {
       if (row >= end) continue;
       const int byte = exponent_byte8(row_most[i]);
       const int64_t line = ALONG == kPieceForm ? place8(row) : row;
-      const int64_t to = ALONG == kPieceForm ? piece_at8(line, first, col_blocks) : row * (col_blocks * kBlock8) + first;
+      const int64_t to = ALONG == kPieceForm ? piece_at8(line, first, col_blocks) : row * row_stride8(p.cols) + first;
       *reinterpret_cast<uint2*>(codes + to) = eight_codes(v[i], row_most[i], inverse_power8(byte));
       if (eighth == 0) exponents[line * stride + blockIdx.x] = (uint8_t)byte;
     }
@@ -177,11 +177,11 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(Quantize8 p) {
         const int place = (piece & 3) * 16 + (lane & 15);               // of 64
         col = (piece >> 2) * 64 + ((place >> 2) & 3) * 16 + (place >> 4) * 4 + (place & 3), chunk = 4 * h + (lane >> 4);
         line = col0 + col;
-        to = ((col0 / kPieceLines8 + piece) * row_blocks + blockIdx.y) * kPieceBytes8 + h * 1024 + lane * 16;
+        to = piece8(col0 / kPieceLines8 + piece, blockIdx.y, row_blocks) * kPieceBytes8 + h * 1024 + lane * 16;
       } else {
         col = at >> 3, chunk = at & 7;
         line = col0 + col;
-        to = line * (row_blocks * kBlock8) + row0 + 16 * chunk;
+        to = line * row_stride8(p.rows) + row0 + 16 * chunk;
       }
       if (line >= end) continue;
       Quad q;
@@ -272,7 +272,7 @@ extern "C" int64_t stk_8bit_piece_bytes(int64_t experts, int64_t inputs, int64_t
 extern "C" int64_t stk_8bit_scale_bytes(int64_t experts, int64_t inputs, int64_t outputs, int float_scales) {
   return experts < 1 || inputs < 1 || outputs < 1 ? 0 : experts * scale_bytes8(outputs, inputs, float_scales ? kFloatScales : kPowerScales);
 }
-extern "C" int64_t stk_8bit_row_bytes(int64_t rows, int64_t size) { return rows < 1 || size < 1 ? 0 : rows * blocks8(size) * kBlock8; }
+extern "C" int64_t stk_8bit_row_bytes(int64_t rows, int64_t size) { return rows < 1 || size < 1 ? 0 : rows * row_stride8(size); }
 extern "C" int64_t stk_8bit_exponent_bytes(int64_t rows, int64_t size) { return rows < 1 || size < 1 ? 0 : rows * exponent_stride8(size); }
 
 static int weights_check8(const char* who, int64_t experts, int64_t inputs, int64_t outputs) {
