@@ -9,12 +9,15 @@
 //   softmax                ds_i = (u_j where i = chosen_j) - p_i sum u
 //
 // Which experts are chosen is to be a matter of the inputs, not of how exp is computed.  Everything is computed in fp32, whose error in c is below
-// 2^-19 of the largest p and |bias|; where two values that decide the choice or its order are closer than four times that, and are not of
-// equal inputs (which are equal whatever the precision), the token is done again in 64 bits.  That is one token in some hundred.
+// 2^-19 (softmax: the sum's error counts) or 2^-21 (sigmoid) of the largest p and |bias|, and keys (below) lose another 2^-19; where two values that decide
+// the choice or its order are closer than twice the error and that, 2^-17 or 2^-18, and are not of equal inputs (which are equal whatever the precision), the token is done again in 64 bits, by a whole wavefront.  That is one token in some
+// hundred, but a wavefront waits for the slowest of its four.  Where the order of c is that of the scores (no bias, and one expert decides for its group)
+// the groups are compared by these.
 //
 // A token belongs to a team of 16 or 64 lanes, and expert i to its lane i % LANES, place i / LANES.  A round of the choice is a maximum over
 // keys of 32 bits: the ordered bits of c with the place in the lowest four, so that a lane's maximum says whose it is; what that takes off c is
-// within the margin of the 64-bit check.
+// within the margin of the 64-bit check.  A lane remembers the last of its keys that was chosen, t, and the largest key below is t plus the largest
+// key - t modulo 2^32: an instruction and a half for each key and round.
 #include <type_traits>
 
 #include "common.h"
@@ -23,6 +26,7 @@
 
 namespace stk {
 
+constexpr int kFewTokens = 2048;
 constexpr int kGroupRouterExperts = 1024, kGroupRouterTopK = 32, kGroupRouterGroups = 64;
 
 struct GroupRouter {
@@ -37,8 +41,22 @@ struct GroupRouter {
   float* weights;
 };
 
+// Value of a lane of the team (of a whole wavefront: the same lane for all).
+template <class T, class Fn>
+__device__ __forceinline__ T by_words(T v, Fn&& move) {
+  constexpr int N = sizeof(T) / 4;
+  uint32_t w[N];
+  __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+  for (int i = 0; i < N; i++) w[i] = move(w[i]);
+  __builtin_memcpy(&v, w, sizeof(T));
+  return v;
+}
 template <int LANES, class T>
-__device__ __forceinline__ T from_lane(T v, int lane) { return __shfl(v, lane, LANES); }
+__device__ __forceinline__ T from_lane(T v, int lane) {
+  if constexpr (LANES == 64) return by_words(v, [&](uint32_t w) { return (uint32_t)__builtin_amdgcn_readlane((int)w, lane); });
+  else return __shfl(v, lane, LANES);
+}
 template <int LANES>
 __device__ __forceinline__ bool any_of_team(bool v) {
   const uint64_t all = __ballot(v);
@@ -51,14 +69,16 @@ __device__ __forceinline__ uint64_t ballot_of_team(bool v) {
   if constexpr (LANES == 64) return all;
   else return all >> (threadIdx.x & 48) & 0xffffu;
 }
-template <int LANES, class T, class Fn>
-__device__ __forceinline__ T reduce_team(T v, Fn&& fn) {
-#pragma unroll
-  for (int d = 1; d < LANES; d *= 2) v = fn(v, __shfl_xor(v, d, LANES));
-  return v;
-}
 template <int CONTROL>
 __device__ __forceinline__ uint32_t moved_key32(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, 0xf, 0xf, true); }
+// The same value for all lanes: pairs, quads, eights and sixteens meet by permutations that cost no trip to LDS, then the rows of a wavefront in their order.
+template <int LANES, class T, class Fn>
+__device__ __forceinline__ T reduce_team(T v, Fn&& fn) {
+  v = fn(v, by_words(v, moved_key32<0xb1>)), v = fn(v, by_words(v, moved_key32<0x4e>));
+  v = fn(v, by_words(v, moved_key32<0x141>)), v = fn(v, by_words(v, moved_key32<0x140>));
+  if constexpr (LANES == 64) v = fn(fn(from_lane<64>(v, 0), from_lane<64>(v, 16)), fn(from_lane<64>(v, 32), from_lane<64>(v, 48)));
+  return v;
+}
 template <int LANES>
 __device__ __forceinline__ uint32_t largest_key(uint32_t v) {
   v = max(v, moved_key32<0xb1>(v)), v = max(v, moved_key32<0x4e>(v)), v = max(v, moved_key32<0x141>(v)), v = max(v, moved_key32<0x140>(v));
@@ -76,6 +96,12 @@ __device__ __forceinline__ uint32_t ordered(float v) {
   const uint32_t u = __float_as_uint(v);
   return v != v ? 0xffffffffu : v == 0.f ? 0x80000000u : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+// No NaN, and the way back.
+__device__ __forceinline__ uint32_t ordered_number(float v) {
+  const int u = (int)__float_as_uint(v + 0.f);
+  return (uint32_t)u ^ ((uint32_t)(u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float number_of(uint32_t key) { return __uint_as_float(key ^ (~(uint32_t)((int)key >> 31) | 0x80000000u)); }
 __device__ __forceinline__ uint64_t ordered(double v) {
   const uint64_t u = (uint64_t)__double_as_longlong(v), sign = 1ull << 63;
   return v != v ? ~0ull : v == 0. ? sign : u & sign ? ~u : u | sign;
@@ -95,6 +121,11 @@ __device__ __forceinline__ F sigmoid_of(F s) {
   const F t = exponential_of(s < 0 ? s : -s);
   return (s < 0 ? t : F(1)) / (F(1) + t);
 }
+// The same for the choice, to within 2^-21.
+__device__ __forceinline__ float sigmoid_near(float s) {
+  const float t = exponential_of(-fabsf(s));
+  return (s < 0 ? t : 1.f) * __builtin_amdgcn_rcpf(1.f + t);
+}
 
 // The two largest of a group.
 template <class F>
@@ -111,47 +142,66 @@ __device__ __forceinline__ void put(Two<F>& t, F v) {
   t.first = top ? v : t.first;
 }
 
-// One token in the precision of F.  mine: the scores of this lane's experts lane + LANES j.  row: LDS of the team for the c of every expert,
+// One token in the precision of F.  from: its scores; mine: those of this lane's experts lane + LANES j.  row: LDS of the team for the c of every expert,
 // and the groups' values behind them.  at, p: the expert that lane k < top_k is to write and its p; sum: that of the chosen p.  false (F =
 // float only): two of the values that decide are too close for it.
 template <class F, int DTYPE, int LANES, int V>
-__device__ __forceinline__ bool choose(const GroupRouter& r, const float (&mine)[V], F* row, int lane, int& at, F& p_at, F& sum) {
+__device__ __forceinline__ bool choose(const GroupRouter& r, const typename Value<DTYPE>::stored* from, const float (&mine)[V], const float (&bias)[V], F* row, int lane, int& at, F& p_at, F& sum) {
   constexpr bool kFast = std::is_same<F, float>::value;
   const F kNone = -INFINITY;
   F c[V];
   F top = 0, total = 1, largest_p = 0, largest_b = 0;
   bool strange = false;
+  // (behind the last expert are scores of -infinity, whose share is 0)
   if (!r.sigmoid) {
     F most = kNone;
 #pragma unroll
-    for (int j = 0; j < V; j++)
-      if (lane + LANES * j < r.experts) most = in_front((F)mine[j], most) ? (F)mine[j] : most;
+    for (int j = 0; j < V; j++) most = in_front((F)mine[j], most) ? (F)mine[j] : most;
     top = reduce_team<LANES>(most, [](F a, F b) { return in_front(a, b) ? a : b; });
     total = 0;
+    const F shift = top == kNone ? F(0) : top;   // (a row of masked experts)
 #pragma unroll
-    for (int j = 0; j < V; j++)
-      if (lane + LANES * j < r.experts) total += top == kNone ? F(0) : exponential_of((F)mine[j] - top);   // (a row of masked experts)
+    for (int j = 0; j < V; j++) total += exponential_of((F)mine[j] - shift);
     total = reduce_team<LANES>(total, [](F a, F b) { return a + b; });
   }
   const auto share = [&](F s) {   // p of a score
     if (r.sigmoid) return sigmoid_of(s);
     return top == kNone ? F(0) : exponential_of(s - top) / total;
   };
+  // without a bias experts are in the order of the scores, in which sigmoids of 1 are told apart, and so are groups of which the best expert decides
+  const bool by_score = r.bias == nullptr, groups_by_score = by_score && r.best == 1;
+  if (groups_by_score) {
 #pragma unroll
-  for (int j = 0; j < V; j++) {
-    const int e = lane + LANES * j;
-    c[j] = kNone;
-    if (e < r.experts) {
-      const F s = (F)mine[j], p = share(s), b = r.bias ? (F)r.bias[e] : F(0);
-      c[j] = s == kNone ? kNone : p + b;
-      if constexpr (kFast) {
-        largest_p = fmaxf(largest_p, p);
-        if (fabsf(b) < INFINITY) largest_b = fmaxf(largest_b, fabsf(b));
-        else strange = true;
-        strange |= !(fabsf(c[j]) < INFINITY) && s != kNone;
-      }
-      row[e + (e >> 5)] = c[j];   // (groups of 32 start on different banks)
+    for (int j = 0; j < V; j++) {
+      c[j] = (F)mine[j];
+      if constexpr (kFast) strange |= !(mine[j] < INFINITY);
     }
+  } else {
+    if (r.sigmoid) {
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        if constexpr (kFast) c[j] = sigmoid_near(mine[j]);
+        else c[j] = sigmoid_of((F)mine[j]);
+      }
+    } else {
+      const F one_by = top == kNone ? F(0) : F(1) / total, shift = top == kNone ? F(0) : top;
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        if constexpr (kFast) c[j] = exponential_of(mine[j] - shift) * one_by;
+        else c[j] = share((F)mine[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      if constexpr (kFast) largest_p = fmaxf(largest_p, c[j]), largest_b = fmaxf(largest_b, fabsf(bias[j])), strange |= !(fabsf(bias[j]) < INFINITY) || !(mine[j] < INFINITY);
+      const F sum = c[j] + (F)bias[j];
+      c[j] = mine[j] == -INFINITY ? kNone : sum;
+    }
+    if constexpr (kFast) strange |= !(largest_p < INFINITY);
+  }
+  if (r.top_groups < r.groups) {
+#pragma unroll
+    for (int j = 0; j < V; j++) row[lane + LANES * j + ((lane + LANES * j) >> 5)] = c[j];   // (groups of 32 start on different banks)
   }
   asm volatile("" : : : "memory");   // (a team lies in one wavefront, whose LDS accesses are made in order)
   F margin = 0;
@@ -160,7 +210,7 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const float (&mine)
     if (any_of_team<LANES>(strange)) return false;
     largest_p = reduce_team<LANES>(largest_p, [](F a, F b) { return fmaxf(a, b); });
     if (r.bias) largest_b = reduce_team<LANES>(largest_b, [](F a, F b) { return fmaxf(a, b); });
-    margin = (largest_p + largest_b) * 0x1p-17f;
+    margin = (largest_p + largest_b) * (r.sigmoid ? 0x1p-18f : 0x1p-17f);
   }
   // ------------------------------------------------------------ groups
   uint64_t kept = ~0ull;
@@ -170,62 +220,89 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const float (&mine)
     while (2 * along * r.groups <= LANES) along *= 2;
     const int group = lane / along, size = (int)r.group_size;
     Two<F> two = {kNone, kNone};
-    if (group < r.groups)
+    if constexpr (kFast) {
+      // (no NaN here; four of them are on their way from LDS together)
+      const int base = min(group, r.groups - 1) * size, end = group < r.groups ? size : 0;
+      for (int i0 = lane % along; i0 < end; i0 += 4 * along) {
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const int i = i0 + q * along, e = base + min(i, size - 1);
+          v[q] = row[e + (e >> 5)];
+          if (i >= end) v[q] = kNone;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) two.second = fmaxf(two.second, fminf(two.first, v[q])), two.first = fmaxf(two.first, v[q]);
+      }
+    } else if (group < r.groups) {
       for (int i = lane % along; i < size; i += along) {
         const int e = group * size + i;
         put(two, row[e + (e >> 5)]);
       }
+    }
     for (int d = 1; d < along; d *= 2) {
       const Two<F> other = {__shfl_xor(two.first, d, LANES), __shfl_xor(two.second, d, LANES)};
       put(two, other.first), put(two, other.second);
     }
     const F value = group < r.groups ? r.best == 2 ? two.first + two.second : two.first : kNone;
-    int rank = 0;
-    uint64_t close = 0;
-    for (int g = 0; g < r.groups; g++) {
-      const F other = from_lane<LANES>(value, g * along);
-      rank += in_front(other, value) || ((other == value || (other != other && value != value)) && g < group) ? 1 : 0;
-      if constexpr (kFast) close |= (uint64_t)(fabsf(other - value) <= 2 * margin) << g;
-    }
-    const bool first_lane = lane % along == 0, is = group < r.groups && rank < r.top_groups;
-    // bits of the groups: those of their first lanes
-    const uint64_t bits = ballot_of_team<LANES>(is && first_lane);
+    const bool first_lane = lane % along == 0 && group < r.groups;
     kept = 0;
-    for (int g = 0; g < r.groups; g++) kept |= (bits >> (g * along) & 1ull) << g;
     if constexpr (kFast) {
-      const uint64_t all = r.groups < 64 ? (1ull << r.groups) - 1 : ~0ull;
-      if (any_of_team<LANES>(is && (close & all & ~kept) != 0)) return false;
+      // (ordered values of numbers are above 0, infinities below included)
+      uint32_t key = first_lane ? ordered(value) : 0u;
+      float last = kNone;
+      for (int k = 0; k < r.top_groups; k++) {
+        const uint32_t best = largest_key<LANES>(key);
+        const int who = __builtin_ctzll(ballot_of_team<LANES>(key == best));
+        kept |= 1ull << (who / along);
+        if (k == r.top_groups - 1) last = from_lane<LANES>(value, who);
+        if (lane == who) key = 0u;
+      }
+      // one that is not kept and may count as much
+      if (any_of_team<LANES>(!groups_by_score && key != 0u && last - value <= 2 * margin)) return false;
+    } else {
+      int rank = 0;
+      for (int g = 0; g < r.groups; g++) {
+        const F other = from_lane<LANES>(value, g * along);
+        rank += in_front(other, value) || ((other == value || (other != other && value != value)) && g < group) ? 1 : 0;
+      }
+      // bits of the groups: those of their first lanes
+      const uint64_t bits = ballot_of_team<LANES>(first_lane && rank < r.top_groups);
+      for (int g = 0; g < r.groups; g++) kept |= (bits >> (g * along) & 1ull) << g;
     }
   }
   // ------------------------------------------------------------ experts
-  // without a bias in the order of the scores, in which sigmoids of 1 are told apart
-  const bool by_score = r.bias == nullptr;
   typedef std::conditional_t<kFast, uint32_t, uint64_t> key_t;
   key_t key[V];
 #pragma unroll
   for (int j = 0; j < V; j++) {
     const uint32_t e = lane + LANES * j;
-    if (by_score) c[j] = (F)mine[j];
-    const bool in = (int)e < r.experts && (kept >> (r.group_size == 0 ? 0 : e * r.group_magic >> 22) & 1ull);
-    if constexpr (kFast) key[j] = in ? (ordered(c[j]) & ~15u) | (15u - j) : 0u;
-    else key[j] = in ? ordered(c[j]) : 0u;
-    if (!in) c[j] = kNone;
+    const F v = by_score ? (F)mine[j] : c[j];
+    if constexpr (kFast) key[j] = (ordered_number(v) & ~15u) | (15u - j);
+    else key[j] = ordered(v);
+    if ((int)e >= r.experts) key[j] = 0u;
+  }
+  if (r.top_groups < r.groups) {
+#pragma unroll
+    for (int j = 0; j < V; j++) key[j] = kept >> ((lane + LANES * j) * r.group_magic >> 22) & 1ull ? key[j] : 0u;
   }
   at = 0;
-  F c_last = 0, s_last = 0;
+  uint32_t mark = 0;   // the last of this lane's keys that was chosen
   for (int k = 0; k < r.top_k; k++) {
     key_t best = 0;
-#pragma unroll
-    for (int j = 0; j < V; j++) best = max(best, key[j]);
     int place = 0, who;
     if constexpr (kFast) {
+#pragma unroll
+      for (int j = 0; j < V; j++) best = max(best, key[j] - mark);
+      best += mark;
+      if (best - 1u >= mark - 1u) best = 0u;   // (none below: the largest of all came round)
       const key_t all = largest_key<LANES>(best);
       who = __builtin_ctzll(ballot_of_team<LANES>(best == all));
       place = 15 - (int)(all & 15u);
-      const key_t gone = lane == who ? all : 0u;
-#pragma unroll
-      for (int j = 0; j < V; j++) key[j] = key[j] == gone ? 0u : key[j];
+      if (lane == who) mark = all;
     } else {
+#pragma unroll
+      for (int j = 0; j < V; j++) best = max(best, key[j]);
       // of equal ones the lowest expert: the lowest place, then the lowest lane
       const key_t all = reduce_team<LANES>(best, [](key_t a, key_t b) { return a > b ? a : b; });
       int first = V;
@@ -238,29 +315,30 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const float (&mine)
     }
     if (lane == k) at = who + LANES * place;
   }
-  // the scores of the chosen: through LDS, where the lanes' experts are
-  asm volatile("" : : : "memory");
-#pragma unroll
-  for (int j = 0; j < V; j++) {
-    const int e = lane + LANES * j;
-    if (e < r.experts) row[e + (e >> 5)] = (F)mine[j];
-  }
-  asm volatile("" : : : "memory");
   const bool is = lane < r.top_k;
-  const F s_at = row[at + (at >> 5)];
+  const F s_at = is ? (F)Value<DTYPE>::widen(from[at]) : kNone;
   if constexpr (kFast) {
-    const F b_at = r.bias ? r.bias[at] : 0.f, c_at = by_score ? s_at : (s_at == kNone ? kNone : share(s_at) + b_at);
+    const float b_at = r.bias ? r.bias[at] : 0.f, c_at = by_score ? s_at : (s_at == kNone ? kNone : share(s_at) + b_at);
     // the order of the chosen
-    const F next_c = __shfl_down(c_at, 1, LANES), next_s = __shfl_down(s_at, 1, LANES), next_b = __shfl_down(b_at, 1, LANES);
-    const auto too_close = [&](F a, F b) { return fabsf(a - b) <= (by_score ? fminf(fabsf(a), fabsf(b)) * 0x1p-18f : margin); };
-    bool wrong = lane < r.top_k - 1 && too_close(c_at, next_c) && !(s_at == next_s && b_at == next_b);
-    // the last of them and those that are not chosen
-    c_last = from_lane<LANES>(c_at, r.top_k - 1), s_last = from_lane<LANES>(s_at, r.top_k - 1);
-    const F b_last = from_lane<LANES>(b_at, r.top_k - 1);
+    const float next_c = __shfl_down(c_at, 1, LANES), next_s = __shfl_down(s_at, 1, LANES), next_b = __shfl_down(b_at, 1, LANES);
+    const auto too_close = [&](float a, float b) { return fabsf(a - b) <= (by_score ? fminf(fabsf(a), fabsf(b)) * 0x1p-18f : margin); };
+    if (any_of_team<LANES>(lane < r.top_k - 1 && too_close(c_at, next_c) && !(s_at == next_s && b_at == next_b))) return false;
+    // the last of them and those that are not chosen (whose keys tell c to 2^-19 of it)
+    const float c_last = from_lane<LANES>(c_at, r.top_k - 1);
+    bool close = false;
 #pragma unroll
-    for (int j = 0; j < V; j++)
-      if (key[j] != 0 && too_close(c[j], c_last)) wrong |= !(mine[j] == s_last && (by_score || r.bias[lane + LANES * j] == b_last));
-    if (any_of_team<LANES>(wrong)) return false;
+    for (int j = 0; j < V; j++) close |= key[j] - 1u < mark - 1u && too_close(number_of(key[j] & ~15u), c_last);
+    if (any_of_team<LANES>(close)) {   // of equal inputs?
+      const float s_last = from_lane<LANES>(s_at, r.top_k - 1), b_last = from_lane<LANES>(b_at, r.top_k - 1);
+      bool wrong = false;
+#pragma unroll
+      for (int j = 0; j < V; j++)
+        if (key[j] - 1u < mark - 1u && too_close(number_of(key[j] & ~15u), c_last)) {
+          const int e = lane + LANES * j;
+          wrong |= !(Value<DTYPE>::widen(from[e]) == s_last && (by_score || r.bias[e] == b_last));
+        }
+      if (any_of_team<LANES>(wrong)) return false;
+    }
   }
   p_at = is ? share(s_at) : F(0);
   sum = reduce_team<LANES>(p_at, [](F a, F b) { return a + b; });
@@ -268,29 +346,59 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const float (&mine)
 }
 
 template <int DTYPE, int LANES, int V>
+__device__ __forceinline__ void load_scores(float (&mine)[V], const typename Value<DTYPE>::stored* from, int lane, int experts) {
+#pragma unroll
+  for (int j = 0; j < V; j++) mine[j] = Value<DTYPE>::widen(from[min(lane + LANES * j, experts - 1)]);   // (all on their way together)
+#pragma unroll
+  for (int j = 0; j < V; j++) mine[j] = lane + LANES * j < experts ? mine[j] : -INFINITY;
+}
+template <int LANES, int V>
+__device__ __forceinline__ void load_bias(float (&bias)[V], const GroupRouter& r, int lane) {
+#pragma unroll
+  for (int j = 0; j < V; j++) bias[j] = 0.f;
+  if (r.bias) {
+#pragma unroll
+    for (int j = 0; j < V; j++) bias[j] = r.bias[min(lane + LANES * j, r.experts - 1)];
+  }
+}
+__device__ __forceinline__ void write_choice(const GroupRouter& r, int64_t t, int lane, int at, float p, float sum) {
+  if (lane < r.top_k) {
+    r.chosen[t * r.top_k + lane] = at;
+    r.weights[t * r.top_k + lane] = !r.normalize ? r.scale * p : sum == 0.f ? 0.f : r.scale * (p / sum);
+  }
+}
+template <int DTYPE, int LANES, int V>
 __global__ __launch_bounds__(256) void group_top_experts_kernel(GroupRouter r) {
   typedef typename Value<DTYPE>::stored stored;
-  constexpr int kTeams = 256 / LANES, kRow = LANES * V + LANES * V / 32 + 1;
-  __shared__ double rows[kTeams][kRow];
-  const int lane = threadIdx.x % LANES;
-  double* row = rows[threadIdx.x / LANES];
-  for (int64_t t = (int64_t)blockIdx.x * kTeams + threadIdx.x / LANES; t < r.tokens; t += (int64_t)gridDim.x * kTeams) {
-    const stored* from = static_cast<const stored*>(r.scores) + t * r.stride;
-    float mine[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) mine[j] = lane + LANES * j < r.experts ? Value<DTYPE>::widen(from[lane + LANES * j]) : -INFINITY;
+  constexpr int kTeams = 256 / LANES, kExperts = LANES * V, kRow = kExperts + kExperts / 32 + 1, kWide = (kExperts + 63) / 64;
+  __shared__ union {
+    float fast[kTeams][kRow];
+    double wide[4][64 * kWide + 2 * kWide + 1];
+  } rows;
+  __shared__ int again[kTeams], agains;
+  const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES, wave = threadIdx.x / 64, place = threadIdx.x & 63;
+  const int64_t first = (int64_t)blockIdx.x * kTeams;   // (a grid for all tokens: what a loop keeps of the lanes' experts takes more registers than the choice)
+  if (threadIdx.x == 0) agains = 0;
+  __syncthreads();
+  if (first + team < r.tokens) {
+    const stored* from = static_cast<const stored*>(r.scores) + (first + team) * r.stride;
+    float mine[V], bias[V], p, sum;
     int at;
-    float p, sum;
-    if (!choose<float, DTYPE, LANES, V>(r, mine, reinterpret_cast<float*>(row), lane, at, p, sum)) {
-      double p64, sum64;
-      choose<double, DTYPE, LANES, V>(r, mine, row, lane, at, p64, sum64);
-      p = (float)p64, sum = (float)sum64;
-    }
-    if (lane < r.top_k) {
-      r.chosen[t * r.top_k + lane] = at;
-      r.weights[t * r.top_k + lane] = !r.normalize ? r.scale * p : sum == 0.f ? 0.f : r.scale * (p / sum);
-    }
-    asm volatile("" : : : "memory");
+    load_scores<DTYPE, LANES>(mine, from, lane, r.experts), load_bias<LANES>(bias, r, lane);
+    if (choose<float, DTYPE, LANES, V>(r, from, mine, bias, rows.fast[team], lane, at, p, sum)) write_choice(r, first + team, lane, at, p, sum);
+    else if (lane == 0) again[atomicAdd(&agains, 1)] = team;
+  }
+  __syncthreads();
+  for (int i = wave; i < agains; i += 4) {
+    const int64_t t = first + again[i];
+    const stored* from = static_cast<const stored*>(r.scores) + t * r.stride;
+    float mine[kWide], bias[kWide];
+    double p, sum;
+    int at;
+    load_scores<DTYPE, 64>(mine, from, place, r.experts), load_bias<64>(bias, r, place);
+    choose<double, DTYPE, 64, kWide>(r, from, mine, bias, rows.wide[wave], place, at, p, sum);
+    write_choice(r, t, place, at, (float)p, (float)sum);
+    asm volatile("" : : : "memory");   // (a team lies in one wavefront, whose LDS accesses are made in order)
   }
 }
 
@@ -303,57 +411,56 @@ __global__ __launch_bounds__(256) void group_top_experts_backward_kernel(GroupRo
   const int lane = threadIdx.x % LANES;
   float* row = rows[threadIdx.x / LANES];
   const auto add = [](float a, float b) { return a + b; };
-  for (int64_t t = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; t < r.tokens; t += (int64_t)gridDim.x * (256 / LANES)) {
-    const stored* from = static_cast<const stored*>(r.scores) + t * r.stride;
-    float w = 0.f, u = 0.f;
-    int at = -1;
-    if (lane < r.top_k) {
-      w = r.weights[t * r.top_k + lane], at = r.chosen[t * r.top_k + lane];
-      u = grad[t * r.top_k + lane] * w;
-    }
-    const float all = reduce_team<LANES>(u, add);
-    float mine[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) mine[j] = 0.f;
-    if (!r.sigmoid && !r.normalize) {
-      float most = -INFINITY, total = 0.f;
-#pragma unroll
-      for (int j = 0; j < V; j++) {
-        mine[j] = lane + LANES * j < r.experts ? Value<DTYPE>::widen(from[lane + LANES * j]) : -INFINITY;
-        most = in_front(mine[j], most) ? mine[j] : most;
-      }
-      most = reduce_team<LANES>(most, [](float a, float b) { return in_front(a, b) ? a : b; });
-#pragma unroll
-      for (int j = 0; j < V; j++) {
-        mine[j] = most == -INFINITY ? 0.f : exponential_of(mine[j] - most);
-        total += mine[j];
-      }
-      total = reduce_team<LANES>(total, add);
-#pragma unroll
-      for (int j = 0; j < V; j++) mine[j] = most == -INFINITY ? 0.f : -(mine[j] / total) * all;
-    }
-#pragma unroll
-    for (int j = 0; j < V; j++) row[lane + LANES * j] = mine[j];
-    asm volatile("" : : : "memory");   // (a team lies in one wavefront, whose LDS accesses are made in order)
-    if ((unsigned)at < (unsigned)r.experts) {
-      float own = r.normalize ? u - w / r.scale * all : u;
-      if (r.sigmoid) own *= sigmoid_of(-Value<DTYPE>::widen(from[at]));
-      row[at] += own;
-    }
-    asm volatile("" : : : "memory");
-#pragma unroll
-    for (int j = 0; j < V; j++)
-      if (lane + LANES * j < r.experts) out[t * out_stride + lane + LANES * j] = Value<DTYPE>::round(row[lane + LANES * j]);
-    asm volatile("" : : : "memory");
+  const int64_t t = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  if (t >= r.tokens) return;
+  const stored* from = static_cast<const stored*>(r.scores) + t * r.stride;
+  float w = 0.f, u = 0.f;
+  int at = -1;
+  if (lane < r.top_k) {
+    w = r.weights[t * r.top_k + lane], at = r.chosen[t * r.top_k + lane];
+    u = grad[t * r.top_k + lane] * w;
   }
+  const float all = reduce_team<LANES>(u, add);
+  float mine[V];
+#pragma unroll
+  for (int j = 0; j < V; j++) mine[j] = 0.f;
+  if (!r.sigmoid && !r.normalize) {
+    float most = -INFINITY, total = 0.f;
+    load_scores<DTYPE, LANES>(mine, from, lane, r.experts);
+#pragma unroll
+    for (int j = 0; j < V; j++) most = in_front(mine[j], most) ? mine[j] : most;
+    most = reduce_team<LANES>(most, [](float a, float b) { return in_front(a, b) ? a : b; });
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      mine[j] = most == -INFINITY ? 0.f : exponential_of(mine[j] - most);
+      total += mine[j];
+    }
+    total = reduce_team<LANES>(total, add);
+#pragma unroll
+    for (int j = 0; j < V; j++) mine[j] = most == -INFINITY ? 0.f : -(mine[j] / total) * all;
+  }
+#pragma unroll
+  for (int j = 0; j < V; j++) row[lane + LANES * j] = mine[j];
+  asm volatile("" : : : "memory");   // (a team lies in one wavefront, whose LDS accesses are made in order)
+  if ((unsigned)at < (unsigned)r.experts) {
+    float own = r.normalize ? u - w / r.scale * all : u;
+    if (r.sigmoid) own *= sigmoid_of(-Value<DTYPE>::widen(from[at]));
+    row[at] += own;
+  }
+  asm volatile("" : : : "memory");
+#pragma unroll
+  for (int j = 0; j < V; j++)
+    if (lane + LANES * j < r.experts) out[t * out_stride + lane + LANES * j] = Value<DTYPE>::round(row[lane + LANES * j]);
 }
 
-// Teams of 16 lanes have a lane for every choice, and for every group, where these are few.
+// Teams of 16 lanes have a lane for every choice, and for every group, where these are few.  Where there are few tokens a wavefront each is sooner done:
+// the top 8 of 256 in groups for 2048 tokens 12.5 us, with teams 14.1; for 16384 teams 22.8 (16.8 MB of scores are 3.4 us: bound by what the choice
+// executes, some 700 instructions a wavefront, and by the tokens that are done again).
 template <class Fn>
 static void for_team(const GroupRouter& r, Fn&& fn) {
   typedef std::integral_constant<int, 16> Sixteen;
   typedef std::integral_constant<int, 64> Wave;
-  if (r.top_k <= 16 && r.groups <= 16 && r.experts <= 256) {
+  if (r.top_k <= 16 && r.groups <= 16 && r.experts <= 256 && r.tokens > kFewTokens) {
     if (r.experts <= 64) fn(Sixteen(), std::integral_constant<int, 4>());
     else if (r.experts <= 128) fn(Sixteen(), std::integral_constant<int, 8>());
     else fn(Sixteen(), std::integral_constant<int, 16>());
@@ -361,10 +468,7 @@ static void for_team(const GroupRouter& r, Fn&& fn) {
   else if (r.experts <= 512) fn(Wave(), std::integral_constant<int, 8>());
   else fn(Wave(), std::integral_constant<int, 16>());
 }
-static dim3 group_router_grid(int64_t tokens, int lanes) {
-  const int64_t groups = (tokens + 256 / lanes - 1) / (256 / lanes);
-  return dim3((unsigned)(groups < 1 << 20 ? groups : 1 << 20));
-}
+static dim3 group_router_grid(int64_t tokens, int lanes) { return dim3((unsigned)((tokens + 256 / lanes - 1) / (256 / lanes))); }
 static int group_router_check(const char* who, GroupRouter& r, int64_t experts, int dtype) {
   if (!is_value_dtype(dtype)) return fail(STK_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
   if (r.tokens < 0 || experts < 1 || r.groups < 1 || experts % r.groups) return fail(STK_ERR_DIMS, "%s: %lld experts in %d groups", who, (long long)experts, r.groups);

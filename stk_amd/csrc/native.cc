@@ -937,6 +937,7 @@ struct GroupTopExperts : torch::autograd::Function<GroupTopExperts> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& scores, const OptTensor& bias, const GroupChoice& c) {
     auto [chosen, weights] = group_choice(scores, bias, c);
     ctx->save_for_backward({scores, chosen, weights});
+    ctx->set_materialize_grads(false);   // (chosen has none)
     ctx->saved_data["sigmoid"] = c.sigmoid, ctx->saved_data["normalize"] = c.normalize, ctx->saved_data["scale"] = c.scale;
     ctx->mark_non_differentiable({chosen});
     return {chosen, weights};

@@ -80,11 +80,14 @@ class _GroupTopExperts(torch.autograd.Function):
         _, _, _, sigmoid, _, normalize, scale = choice
         ctx.formula = sigmoid, normalize, scale
         ctx.mark_non_differentiable(chosen)
+        ctx.set_materialize_grads(False)
         return chosen, weights
 
     @staticmethod
     @once_differentiable
     def backward(ctx, _, grad):
+        if grad is None:
+            return (None,) * 9
         scores, chosen, weights = ctx.saved_tensors
         return hip_kernels.group_top_experts_backward(scores, chosen, weights, grad, *ctx.formula), *(None,) * 8
 
