@@ -30,27 +30,20 @@ __device__ __forceinline__ i32x8_t quantise_fragment(const u32x4 (&raw)[4], int&
       most2 = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most2), __builtin_bit_cast(u16x2, word & 0x7fff7fffu)));
     }
   uint32_t most = max(most2 >> 16, most2 & 0xffffu);
-  most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64)), most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
+  const auto by16 = __builtin_amdgcn_permlane16_swap(most, most, false, false);
+  most = max(by16[0], by16[1]);
+  const auto by32 = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+  most = max(by32[0], by32[1]);
   typedef std::conditional_t<BF16, Value<STK_BF16>, Value<STK_F16>> V;
   const uint32_t bits = __float_as_uint(V::widen(__builtin_bit_cast(typename V::stored, (uint16_t)most)));
   byte = exponent_byte8(bits);
-  const bool nan = bits >= 0x7f800000u;
-  const float inverse = inverse_power8(byte);
+  const float scale = __uint_as_float((uint32_t)byte << 23);
+  byte = bits >= 0x7f800000u ? 255 : byte;   // (a scale that is not a number)
   i32x8_t out;
 #pragma unroll
   for (int i = 0; i < 4; i++)
 #pragma unroll
-    for (int j = 0; j < 4; j += 2) {
-      const uint32_t lo = raw[i][j], hi = raw[i][j + 1];
-      float a, b, c, d;
-      if constexpr (BF16) a = __uint_as_float(lo << 16), b = __uint_as_float(lo & 0xffff0000u), c = __uint_as_float(hi << 16), d = __uint_as_float(hi & 0xffff0000u);
-      else {
-        const HalfPair p = __builtin_bit_cast(HalfPair, lo), q = __builtin_bit_cast(HalfPair, hi);
-        a = (float)p.x, b = (float)p.y, c = (float)q.x, d = (float)q.y;
-      }
-      const uint32_t four = codes8(a * inverse, b * inverse, c * inverse, d * inverse);
-      out[2 * i + j / 2] = (int)(nan ? kNan8 : four);
-    }
+    for (int j = 0; j < 4; j += 2) out[2 * i + j / 2] = (int)codes8_of_pairs<BF16>(raw[i][j], raw[i][j + 1], scale);
   return out;
 }
 
@@ -439,15 +432,21 @@ static ProductKernel8 product_kernel8(int64_t rows, int64_t experts, int64_t inp
   const int64_t along = blocks8(inputs), down = padded_lines8(outputs) / kPieceLines8;
   // as if the rows were spread evenly over the experts: where they really are only the device knows
   const int64_t hit = experts < rows ? experts : rows, each = (rows + hit - 1) / hit;
-  if (each > 16) {
+  // Streams read an expert's weights once for every 16 rows, behind the first time from the caches, at some 8 TB/s; tiles take a launch that quantises the
+  // rows, and a step of 0.6 us for every block where few of them are in the chip.  4096 x 4096, streams and the best tiles: 20 rows 9.5 and 23.4 us, 64
+  // rows 11.6 and 25.2, 128 rows 18.7 and 25.3; 1024 x 4096, 64 rows 5.8 and 10.0; 37 rows of 2944 x 1151 6.1 and 20.0; 8 experts of 1024 x 1024, 40
+  // rows each 8.3 and 11.5; 64 experts of 1024 x 4096, 20 rows each 77 and 68, 40 rows each 113 and 83.
+  const int64_t tiles = hit * ((each + 15) / 16) * down;
+  if (each > 16 && tiles > 2048 + 8192 / along) {
     if (each > 64 && hit * ((each + 255) / 256) * ((outputs + 255) / 256) >= 192) return kTile8_256;
     if (each > 64 && hit * ((each + 127) / 128) * ((outputs + 127) / 128) >= 192) return kTile8_128;
     return each > 32 ? kTile8_64 : kTile8_32;
   }
-  const int64_t tiles = hit * down;
+  // The fewer tiles there are the more wavefronts share the inputs of one: 1 row of 4096 x 4096 (256 tiles) 6.2, 8.8, 10.8 us by 8, 4 and 4 for two and four
+  // pieces; 20 rows (512) 10.8, 9.5, 11.2; 64 rows (1024) 21.5, 14.1, 11.6.
   if (tiles <= 320) return kStream8_811;
   if (tiles <= 640) return kStream8_412;
-  if (along >= 24) return kStream8_414;
+  if (along >= 24 || (along >= 8 && tiles <= 4096)) return kStream8_414;
   return tiles <= 4096 ? kStream8_222 : kStream8_144;
 }
 static int64_t workspace8(int64_t x_rows, int64_t rows, int64_t experts, int64_t inputs, int64_t outputs) {

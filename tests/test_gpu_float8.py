@@ -188,7 +188,8 @@ def _route(tokens, experts, top_k, how, blocking, seed):
 ROUTED = [(1, 4, 1, 128, 16, "any", 1), (1, 64, 2, 256, 48, "any", 128), (3, 4, 4, 200, 33, "any", 1), (64, 64, 2, 256, 64, "any", 1), (100, 8, 2, 384, 100, "half", 1),
           (50, 200, 1, 64, 16, "any", 1), (300, 4, 1, 130, 40, "one", 1), (33, 16, 3, 512, 80, "any", 64), (500, 6, 2, 256, 96, "half", 1), (17, 1, 1, 128, 20, "any", 1),
           (40, 32, 8, 96, 24, "any", 1), (5, 1024, 2, 32, 16, "any", 1), (2000, 3, 1, 160, 144, "any", 128), (160, 64, 2, 136, 1120, "any", 1),
-          (600, 16, 2, 264, 528, "half", 1), (3000, 8, 2, 264, 1040, "any", 1), (2, 4, 2, 3200, 700, "any", 1), (900, 8, 1, 137, 1040, "half", 1), (4000, 64, 1, 256, 1100, "any", 1), (64, 64, 1, 257, 500, "any", 1)]
+          (600, 16, 2, 264, 528, "half", 1), (3000, 8, 2, 264, 1040, "any", 1), (2, 4, 2, 3200, 700, "any", 1), (900, 8, 1, 137, 1040, "half", 1), (4000, 64, 1, 256, 1100, "any", 1), (64, 64, 1, 257, 500, "any", 1),
+          (1300, 64, 1, 256, 1100, "any", 1)]
 
 
 @pytest.mark.parametrize("kind", ["power", "float"])
