@@ -1,15 +1,16 @@
 // 8-bit floating-point values (e4m3: 4 bits of exponent, 3 of mantissa, at most 448, no infinities) with a scale for every block of 128, as
 // the products take them.
 //
-// Rows: codes [row][blocks x 128], zeros beyond the last input, and one exponent byte (2^(byte - 127)) for each row and block, [row][blocks
-// rounded up to 4], so that a dword holds those of four neighbouring blocks.
+// Rows: codes [row][blocks x 128], zeros beyond the last input, and an exponent byte (2^(byte - 127)) for each row and block, [block / 4][row][block % 4], so
+// that a dword holds those of four neighbouring blocks and neighbouring rows' dwords are neighbours.
 //
 // Pieces: the operand that all rows share, 16 of its lines x 128 inputs in 2048 bytes, in the order of a wavefront's two 16-byte accesses:
 // access h, lane l has inputs 64 h + 16 (l / 16) .. + 15 of line l % 16.  (Which input goes where in v_mfma_scale_f32_16x16x128 does not
 // matter as long as both operands agree, and all inputs of a block have one scale.)  The four pieces of 64 lines lie next to each other, then
-// follow those of the next block, of the next 64 lines, of the next expert.  Lines are dealt to the pieces of 64 so that the four sums that a lane has of each of four pieces belong to
-// 16 neighbouring lines: line 16 q + 4 t + r of the 64 is line 4 q + r of piece t.  Lines are padded to a multiple of 64 with zeros.
-// Scales of pieces: exponent bytes [place of the line][blocks rounded up to 4] ("power"), or fp32 [ceil(lines / 128)][blocks] ("float").
+// follow those of the next block, of the next 64 lines, of the next expert.  Lines are dealt to the pieces of 64 so that the four sums that each
+// of a row's four lanes has of two pieces make 64 neighbouring bytes of a 16-bit result: line 32 u + 8 q + 4 v + r of the 64 is line 4 q + r
+// of piece 2 u + v.  Lines are padded to a multiple of 64 with zeros.
+// Scales of pieces: exponent bytes [block / 4][place of the line][block % 4] ("power"), or fp32 [ceil(lines / 128)][blocks] ("float").
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -27,8 +28,11 @@ __host__ __device__ inline int64_t piece_bytes8(int64_t lines, int64_t size) { r
 __host__ __device__ inline int64_t scale_bytes8(int64_t lines, int64_t size, int kind) {
   return kind == kPowerScales ? padded_lines8(lines) * exponent_stride8(size) : blocks8(lines) * blocks8(size) * 4;
 }
-// Place of a line among those of its pieces.
-__host__ __device__ inline int64_t place8(int64_t line) { return (line & ~(int64_t)63) + ((line >> 2) & 3) * 16 + ((line >> 4) & 3) * 4 + (line & 3); }
+// Place of a line among those of its pieces, and the line of a place.
+__host__ __device__ inline int64_t place8(int64_t line) { return (line & ~(int64_t)63) + ((line >> 5) & 1) * 32 + ((line >> 2) & 1) * 16 + ((line >> 3) & 3) * 4 + (line & 3); }
+__host__ __device__ inline int line_of_place8(int place) { return (place & ~63) + ((place >> 5) & 1) * 32 + ((place >> 2) & 3) * 8 + ((place >> 4) & 1) * 4 + (place & 3); }
+// Byte of a line's exponent of a block, from the first of an operand of so many lines.
+__host__ __device__ inline int64_t exponent_at8(int64_t line, int64_t block, int64_t lines) { return ((block >> 2) * lines + line) * 4 + (block & 3); }
 // Piece p (16 places) of a block, in pieces from the start of an operand.
 __host__ __device__ inline int64_t piece8(int64_t p, int64_t block, int64_t blocks) { return ((p >> 2) * blocks + block) * 4 + (p & 3); }
 // Byte of (place, input) from the start of an operand's pieces; `blocks` of them along the inputs.

@@ -105,7 +105,7 @@ __device__ __forceinline__ bool place_of_row8(const Product8& p, const RowTile8&
   }
   return true;
 }
-// N x 4 neighbouring outputs of a row from `first` on.
+// 4 N neighbouring outputs of a row from `first` on.
 template <int N>
 __device__ __forceinline__ void store8(const Product8& p, int64_t to, float by, int64_t first, const f32x4_t (&v)[N]) {
   const int here = (int)min(p.outputs - first, (int64_t)(4 * N));
@@ -128,28 +128,49 @@ __device__ __forceinline__ void store8(const Product8& p, int64_t to, float by, 
   uint16_t* at = static_cast<uint16_t*>(p.out) + to * p.out_stride + first;
   if (here == 4 * N) {
     if constexpr (N == 1) *reinterpret_cast<PairAt2*>(at) = PairAt2{two[0], two[1]};
-    else {
-#pragma unroll
-      for (int n = 0; n < N; n += 2) *reinterpret_cast<QuadAt2*>(at + 4 * n) = QuadAt2{two[2 * n], two[2 * n + 1], two[2 * n + 2], two[2 * n + 3]};
-    }
+    else *reinterpret_cast<QuadAt2*>(at) = QuadAt2{two[0], two[1], two[2], two[3]};
   } else {
 #pragma unroll
     for (int i = 0; i < 4 * N; i++)
       if (i < here) at[i] = (uint16_t)(two[i / 2] >> (16 * (i & 1)));
   }
 }
+// The sums of a row's lane of the four pieces of 64 outputs, whose first is `first`.
+__device__ __forceinline__ void store_pieces8(const Product8& p, int64_t to, float by, int64_t first, int quarter, const f32x4_t (&v)[4]) {
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    const f32x4_t two[2] = {v[2 * u], v[2 * u + 1]};
+    store8<2>(p, to, by, first + 32 * u + 8 * quarter, two);
+  }
+}
+
+// Rows of a tile in LDS: eight of 128 bytes a transfer (1 KiB), whole lines of memory.  The 16-byte chunk c of row r is at slot c ^ (r / 2 % 8), which
+// spreads what the 16 rows of a fragment read at a time over all banks.  What lane l of a transfer takes is a matter of its address:
+__device__ __forceinline__ int row_of_transfer8(int lane) { return lane >> 3; }
+__device__ __forceinline__ int chunk_of_transfer8(int row, int lane) { return (lane & 7) ^ ((row >> 1) & 7); }
+// The first 16 bytes of a lane of a fragment of 16 rows; the other 16 are at this ^ 64.
+__device__ __forceinline__ int in_fragment8(int lane) { return (lane & 15) * kBlock8 + (((lane >> 4) ^ ((lane >> 1) & 7)) << 4); }
 
 // What the gradient of the weights is told beside: dw[e][i][o] = the sum over the rows r of expert e of xq[r][i] gq[r][o].  codes: the columns of x
 // (a line for each input, row blocks along it), packed: those of g as pieces; outputs, out: those of dw, x_rows its inputs, `inputs` the rows.
 // Otherwise a product of rows.
 enum What8 : int { kRows8 = 0, kGradient8 = 1 };
 
-// 16, or 4, bytes per lane from any addresses into the LDS bytes from lds_base on, lane after lane.
-__device__ __forceinline__ void dma16_from(const void* from, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(uniform((int)lds_base)), "v"((uint64_t)from) : "memory", "m0");
-}
+// 4 bytes per lane from any addresses into the LDS bytes from lds_base on, lane after lane.
 __device__ __forceinline__ void dma4_from(const void* from, uint32_t lds_base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(uniform((int)lds_base)), "v"((uint64_t)from) : "memory", "m0");
+}
+
+// 16, or 4, bytes from `offset` + `start` on in a buffer: everything from an address on, as far as 32 bits reach.  (The wait: a scalar register that the VALU
+// wrote may be read by a memory access five states later, and the compiler does not see that this is one.)
+__device__ __forceinline__ u32x4 buffer8(const uint8_t* from) {
+  const uint64_t a = (uint64_t)uniform_global(from);
+  return u32x4{(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
+}
+template <int BYTES>
+__device__ __forceinline__ void fetch8(u32x4 buffer, uint32_t offset, uint32_t start, uint32_t to) {
+  if constexpr (BYTES == 16) asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %0, %2 offen lds" : : "s"(buffer), "v"(offset), "s"(start), "s"(to) : "memory", "m0");
+  else asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dword %1, %0, %2 offen lds" : : "s"(buffer), "v"(offset), "s"(start), "s"(to) : "memory", "m0");
 }
 
 // Tiles of 256 x 256 with power-of-two scales (product8_wide.hip).

@@ -87,10 +87,10 @@ __global__ __launch_bounds__(64 * KW * NW) void stream8_kernel(Product8 p) {
 #pragma unroll
   for (int n = 0; n < NT; n++) {
     tile[n] = ((int)blockIdx.x * NW + nw) * NT + n;
-    const int64_t piece = min(tile[n], down - 1), at = (int64_t)t.expert * down + piece;
+    const int64_t piece = min(tile[n], down - 1);
     weights[n] = reinterpret_cast<const u32x4*>(p.packed + ((int64_t)t.expert * down * along + piece8(piece, 0, along)) * kPieceBytes8) + lane;
     // (the lines of a piece have one scale)
-    if constexpr (KIND == kPowerScales) scales[n] = const_ints(static_cast<const uint8_t*>(p.scales) + at * kPieceLines8 * exponent_stride8(p.inputs));
+    if constexpr (KIND == kPowerScales) scales[n] = const_ints(static_cast<const uint8_t*>(p.scales) + t.expert * scale_bytes8(p.outputs, p.inputs, KIND) + piece * kPieceLines8 * 4);
     else scales[n] = const_ints(static_cast<const float*>(p.scales) + ((int64_t)t.expert * blocks8(p.outputs) + min(tile[n], down - 1) / 8) * along);
   }
   f32x4_t total[NT];
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(64 * KW * NW) void stream8_kernel(Product8 p) {
     for (int n = 0; n < NT; n++) {
 #pragma unroll
       for (int h = 0; h < 2; h++) g.w[n][h] = __builtin_nontemporal_load(weights[n] + (int64_t)block * (4 * kPieceBytes8 / 16) + 64 * h);
-      if constexpr (KIND == kPowerScales) g.scale[n] = scales[n][block >> 2] >> (8 * (block & 3));
+      if constexpr (KIND == kPowerScales) g.scale[n] = scales[n][(int64_t)(block >> 2) * (down * kPieceLines8)] >> (8 * (block & 3));
       else g.scale[n] = scales[n][block];
     }
     const int first = block * kBlock8 + 16 * quarter;
@@ -157,21 +157,15 @@ __global__ __launch_bounds__(64 * KW * NW) void stream8_kernel(Product8 p) {
   int64_t to;
   float by;
   if (!place_of_row8(p, t, row, to, by)) return;
-  if constexpr (NT == 4) {
-    if (tile[0] < down) store8<4>(p, to, by, (int64_t)tile[0] * 16 + quarter * 16, total);
-  } else {
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-      const f32x4_t one[1] = {total[n]};
-      if (tile[n] < down) store8<1>(p, to, by, (int64_t)(tile[n] / 4) * 64 + quarter * 16 + tile[n] % 4 * 4, one);
-    }
-  }
+  const int64_t group = (int64_t)(tile[0] / 4) * 64;
+  if (tile[0] >= down) return;
+  if constexpr (NT == 4) store_pieces8(p, to, by, group, quarter, total);
+  else store8<NT>(p, to, by, group + tile[0] % 4 / 2 * 32 + quarter * 8 + (tile[0] & 1) * 4, total);
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
 // WM x WN wavefronts share 16 MT WM rows and 64 WN outputs, a block of 128 inputs at a time in two stages of LDS that are filled without
-// registers: pieces of weights as they lie in memory, rows 64 bytes at a time in the same order, so that every fragment is two
-// accesses of neighbouring lanes.  Exponents come four blocks at a time.
+// registers: pieces of weights as they lie in memory, rows by whole lines.  Exponents come four blocks at a time.
 template <int WM, int WN, int MT>
 struct Tile8 {
   static constexpr int kWaves = WM * WN, kRows = 16 * MT * WM, kCols = 64 * WN;
@@ -183,7 +177,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
   typedef Tile8<WM, WN, MT> T;
   extern __shared__ char smem[];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-  const int row = lane & 15, quarter = lane >> 4;
+  const int row = lane & 15, quarter = lane >> 4, in_fragment = in_fragment8(lane);
   // neighbouring tiles, which share rows or weights, go to one compute die: four row tiles by all columns, column after column
   constexpr int kPanel = 4;
   int at = xcd_chunked(blockIdx.x, gridDim.x), expert = 0;
@@ -214,22 +208,23 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
   }
   const int blocks = (int)blocks8(p.inputs), exponent_stride = (int)exponent_stride8(p.inputs);
   const int64_t places = padded_lines8(p.outputs), col0 = (int64_t)col_tile * T::kCols;
-  const auto source_row = [&](int r) {
-    int64_t from = t.first + (r < t.rows ? r : 0);
-    if (WHAT == kRows8 && p.top_k > 0) {
-      const int slot = p.indices[from];
-      from = (unsigned)slot < (unsigned)p.rows ? slot / p.top_k : 0;
-    }
-    return from;
+  const bool gathered = WHAT == kRows8 && p.top_k > 0;
+  const int64_t row_base = gathered ? 0 : t.first;
+  const auto source_row = [&](int r) {   // from row_base on
+    r = r < t.rows ? r : 0;
+    if (!gathered) return (uint32_t)r;
+    const int slot = p.indices[t.first + r];
+    return (unsigned)slot < (unsigned)p.rows ? (uint32_t)(slot / p.top_k) : 0u;
   };
-  // transfers of 1 KiB: half a piece; this wavefront's are number wave, wave + kWaves, ...
+  // transfers of 1 KiB: eight rows, half a piece; this wavefront's are number wave, wave + kWaves, ...
   constexpr int kRowMoves = T::kRows / 8 / T::kWaves, kColMoves = T::kCols / 8 / T::kWaves, kRowChunks = (T::kRows + 63) / 64, kChunks = kRowChunks + WN;
   static_assert(T::kRows / 8 % T::kWaves == 0 && T::kCols / 8 % T::kWaves == 0, "whole shares");
-  const uint8_t* row_from[kRowMoves];
+  const u32x4 row_buffer = buffer8(p.codes + row_base * row_stride8(p.inputs));
+  uint32_t row_offset[kRowMoves];
 #pragma unroll
   for (int j = 0; j < kRowMoves; j++) {
-    const int q = wave + T::kWaves * j;
-    row_from[j] = p.codes + source_row(16 * (q >> 1) + row) * row_stride8(p.inputs) + 64 * (q & 1) + 16 * quarter;
+    const int r = 8 * (wave + T::kWaves * j) + row_of_transfer8(lane);
+    row_offset[j] = source_row(r) * (uint32_t)row_stride8(p.inputs) + 16 * chunk_of_transfer8(r, lane);
   }
   const int64_t matrix = WHAT == kGradient8 ? 0 : t.expert;
   gptr_t col_from[kColMoves];
@@ -245,14 +240,14 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
 #pragma unroll
   for (int j = 0; j < kScaleMoves; j++) {
     const int c = wave + T::kWaves * j;
-    if (c < kRowChunks) scale_from[j] = p.exponents + source_row(64 * c + lane) * (int64_t)exponent_stride;
-    else scale_from[j] = static_cast<const uint8_t*>(p.scales) + (matrix * places + min(col0 + 64 * (c - kRowChunks) + lane, places - 1)) * exponent_stride;
+    if (c < kRowChunks) scale_from[j] = p.exponents + (row_base + source_row(64 * c + lane)) * 4;
+    else scale_from[j] = static_cast<const uint8_t*>(p.scales) + matrix * places * exponent_stride + min(col0 + 64 * (c - kRowChunks) + lane, places - 1) * 4;
   }
   const uint32_t lds = (uint32_t)(uintptr_t)(STK_LDS char*)smem;
   const auto issue = [&](int block, int stage, bool exponents_too, int place) {
     const uint32_t to = lds + stage * T::kStage;
 #pragma unroll
-    for (int j = 0; j < kRowMoves; j++) dma16_from(row_from[j] + (int64_t)block * kBlock8, to + (wave + T::kWaves * j) * 1024);
+    for (int j = 0; j < kRowMoves; j++) fetch8<16>(row_buffer, row_offset[j], block * kBlock8, to + (wave + T::kWaves * j) * 1024);
 #pragma unroll
     for (int j = 0; j < kColMoves; j++) dma16(col_from[j] + (int64_t)block * (4 * kPieceBytes8), lane * 16, to + T::kRowBytes + (wave + T::kWaves * j) * 1024);
     if (exponents_too) {
@@ -261,7 +256,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
       for (int j = 0; j < kScaleMoves; j++) {
         const int c = wave + T::kWaves * j;
         if (c < (KIND == kPowerScales ? kChunks : kRowChunks) && (T::kRows >= 64 || c >= kRowChunks || lane < T::kRows))
-          dma4_from(scale_from[j] + (block & ~3), exponents + (c < kRowChunks ? c * 256 : T::kRows * 4 + (c - kRowChunks) * 256));
+          dma4_from(scale_from[j] + (block >> 2) * (c < kRowChunks ? p.x_rows : places) * 4, exponents + (c < kRowChunks ? c * 256 : T::kRows * 4 + (c - kRowChunks) * 256));
       }
     }
   };
@@ -304,25 +299,26 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
       }
     }
     const float by = KIND == kFloatScales ? __uint_as_float((uint32_t)const_ints(float_scales)[block]) : 1.f;
-    const u32x4* rows = reinterpret_cast<const u32x4*>(smem + stage * T::kStage) + wm * (kPieceBytes8 / 16) + lane;
-    const u32x4* cols = reinterpret_cast<const u32x4*>(smem + stage * T::kStage + T::kRowBytes) + wn * 4 * (kPieceBytes8 / 16) + lane;
-    const auto fragment = [&](const u32x4* from) {
+    const char* rows = smem + stage * T::kStage + wm * kPieceBytes8;
+    const char* cols = smem + stage * T::kStage + T::kRowBytes + wn * 4 * kPieceBytes8 + lane * 16;
+    const auto fragment = [&](const char* first, const char* second) {
       i32x8_t f;
-      const u32x4 a = from[0], b = from[64];
+      const u32x4 a = *reinterpret_cast<const u32x4*>(first), b = *reinterpret_cast<const u32x4*>(second);
 #pragma unroll
       for (int i = 0; i < 4; i++) f[i] = (int)a[i], f[4 + i] = (int)b[i];
       return f;
     };
+    const auto row_fragment = [&](int m) { return fragment(rows + in_fragment + m * WM * kPieceBytes8, rows + (in_fragment ^ 64) + m * WM * kPieceBytes8); };
     // The fragment of the next 16 rows is on its way while one is multiplied; with fp32 scales the sums of one are scaled while the next is.  What lies
     // behind the last row of a tile is left out.
     i32x8_t w[4], values[2];
-    values[0] = fragment(rows);
+    values[0] = row_fragment(0);
 #pragma unroll
-    for (int n = 0; n < 4; n++) w[n] = fragment(cols + n * (kPieceBytes8 / 16));
+    for (int n = 0; n < 4; n++) w[n] = fragment(cols + n * kPieceBytes8, cols + n * kPieceBytes8 + 1024);
 #pragma unroll
     for (int m = 0; m < MT; m++) {
       if (m >= fragments) break;
-      if (m + 1 < MT) values[(m + 1) & 1] = fragment(rows + (m + 1) * WM * (kPieceBytes8 / 16));
+      if (m + 1 < MT) values[(m + 1) & 1] = row_fragment(m + 1);
       f32x4_t part[4];
 #pragma unroll
       for (int n = 0; n < 4; n++) {
@@ -340,14 +336,13 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
     }
     block = next, fresh = next_fresh, place ^= (int)next_fresh;
   }
-  const int64_t first = col0 + 64 * wn + 16 * quarter;
   if constexpr (WHAT == kGradient8) p.out = static_cast<uint16_t*>(p.out) + (int64_t)expert * p.x_rows * p.out_stride;
 #pragma unroll
   for (int m = 0; m < MT; m++) {
     if constexpr (WHAT == kRows8) activate_sums8(total[m], p.activation);
     int64_t to;
     float by;
-    if (place_of_row8(p, t, 16 * (m * WM + wm) + row, to, by)) store8<4>(p, to, by, first, total[m]);
+    if (place_of_row8(p, t, 16 * (m * WM + wm) + row, to, by)) store_pieces8(p, to, by, col0 + 64 * wn, quarter, total[m]);
   }
 }
 
@@ -459,7 +454,9 @@ static int launch_tiles8(const char* who, const Product8& p, int kind, ProductKe
     case kTile8_32: return launch_tiles8<WHAT, 2, 2, 1>(who, p, kind, stream);
     case kTile8_64: return launch_tiles8<WHAT, 2, 2, 2>(who, p, kind, stream);
     case kTile8_128: return launch_tiles8<WHAT, 2, 2, 4>(who, p, kind, stream);
-    default: return kind == kPowerScales ? launch_wide8<WHAT>(who, p, stream) : launch_tiles8<WHAT, 2, 4, 8>(who, p, kind, stream);
+    default:
+      if (kind == kPowerScales && p.activation != kGeluErf) return launch_wide8<WHAT>(who, p, stream);   // (erf's registers do not fit beside 256 sums)
+      return launch_tiles8<WHAT, 2, 4, 8>(who, p, kind, stream);
   }
 }
 // The product of 16-bit rows; the workspace holds them quantised where there are many.

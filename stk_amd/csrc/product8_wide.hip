@@ -24,37 +24,34 @@ constexpr int kWideTile = 256, kWideSide = kWideTile * kBlock8, kWideExponents =
 constexpr int kWideBytes = 4 * kWideSide + 2 * kWideExponents + kWideBins * 4;
 
 // sum += weights rows, the sum in accumulation registers.  As text, so that a sum stays in its registers: left to the compiler the 256 of them move
-// about and spill.  What the compiler does not see then is waited for by hand: settle8 between VALU writes and matrix instructions, and
-// finish8 between these and whatever reads their sums.
+// about and spill.  The compiler does not see into the text, so that waits for what may stand directly in front of it are part of it: two states between
+// a VALU write and a matrix instruction that reads the register, five between a VALU write of a scalar register (it may come back from a
+// spilled one) and a memory access that reads it, one between m0 and a transfer.  settle8 stands behind writes of the execution mask, and finish8 between
+// matrix instructions and whatever reads their sums.
 #define STK_SUM8 "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
 #define STK_SUM8_OPERANDS "v"(weights), "v"(rows), "v"(weight_scale), "v"(row_scale)
 __device__ __forceinline__ void accumulate8(f32x4_t& sum, const i32x8_t& weights, const i32x8_t& rows, int weight_scale, int row_scale) {
-  asm volatile(STK_SUM8 : "+a"(sum) : STK_SUM8_OPERANDS);
+  asm volatile("s_nop 1\n\t" STK_SUM8 : "+a"(sum) : STK_SUM8_OPERANDS);
 }
 // The same with a transfer into the LDS bytes from `to` + AT on: 16 or 4 bytes of each lane, from `offset` + `start` on in a buffer.
 template <int AT, int BYTES>
 __device__ __forceinline__ void accumulate8_fetch(f32x4_t& sum, const i32x8_t& weights, const i32x8_t& rows, int weight_scale, int row_scale, u32x4 buffer, uint32_t offset,
                                                   uint32_t start, uint32_t to) {
   if constexpr (BYTES == 16)
-    asm volatile("s_add_i32 m0, %8, %9\n\t" STK_SUM8 "\n\tbuffer_load_dwordx4 %6, %5, %7 offen lds"
+    asm volatile("s_add_i32 m0, %8, %9\n\ts_nop 2\n\t" STK_SUM8 "\n\tbuffer_load_dwordx4 %6, %5, %7 offen lds"
                  : "+a"(sum) : STK_SUM8_OPERANDS, "s"(buffer), "v"(offset), "s"(start), "s"(to), "n"(AT) : "memory", "m0", "scc");
   else
-    asm volatile("s_add_i32 m0, %8, %9\n\t" STK_SUM8 "\n\tbuffer_load_dword %6, %5, %7 offen lds"
+    asm volatile("s_add_i32 m0, %8, %9\n\ts_nop 2\n\t" STK_SUM8 "\n\tbuffer_load_dword %6, %5, %7 offen lds"
                  : "+a"(sum) : STK_SUM8_OPERANDS, "s"(buffer), "v"(offset), "s"(start), "s"(to), "n"(AT) : "memory", "m0", "scc");
-}
-template <int BYTES>
-__device__ __forceinline__ void fetch8(u32x4 buffer, uint32_t offset, uint32_t start, uint32_t to) {
-  if constexpr (BYTES == 16) asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %0, %2 offen lds" : : "s"(buffer), "v"(offset), "s"(start), "s"(to) : "memory", "m0");
-  else asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %1, %0, %2 offen lds" : : "s"(buffer), "v"(offset), "s"(start), "s"(to) : "memory", "m0");
 }
 __device__ __forceinline__ void settle8() { asm volatile("s_nop 4"); }
 __device__ __forceinline__ void finish8() { asm volatile("s_nop 15\n\ts_nop 15"); }
 // lgkmcnt(0), said so that the compiler knows: after a read through the scalar unit it would wait for all of LDS at the next step's first fragment.
 __device__ __forceinline__ void scalars_read8() { __builtin_amdgcn_s_waitcnt(0xc07f); }
-// Everything from an address on, as far as 32 bits reach.
-__device__ __forceinline__ u32x4 buffer8(const uint8_t* from) {
-  const uint64_t a = (uint64_t)uniform_global(from);
-  return u32x4{(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
+// Eight results to the buffer's byte `offset` + AT.  (As text, so that it is one instruction and the compiler does not wait for it.)
+template <int AT>
+__device__ __forceinline__ void store_eight8(u32x4 eight, uint32_t offset, u32x4 buffer) {
+  asm volatile("s_nop 4\n\tbuffer_store_dwordx4 %0, %1, %2, 0 offen offset:%3\n\ts_nop 0" : : "v"(eight), "v"(offset), "s"(buffer), "n"(AT) : "memory");
 }
 
 template <int WHAT, int ACTIVATION>
@@ -65,6 +62,7 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
   const int row = lane & 15, quarter = lane >> 4;
   const int blocks = (int)blocks8(p.inputs), exponent_stride = (int)exponent_stride8(p.inputs);
   const int64_t places = padded_lines8(p.outputs);
+  const uint32_t row_lines = (uint32_t)p.x_rows * 4, col_lines = (uint32_t)places * 4;   // bytes of the exponents of four blocks
   const uint32_t lds = (uint32_t)(uintptr_t)(STK_LDS char*)smem;
   typedef const STK_LDS int* lds_ints;
   const lds_ints near_bins = (lds_ints)(STK_LDS char*)(smem + kBinsAt);
@@ -136,17 +134,17 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
     };
     const int64_t matrix = WHAT == kGradient8 ? 0 : t.expert, col0 = (int64_t)next.col_tile * kWideTile;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {   // of the half fragments wave, wave + 4, ...
-      const int q = wave + 4 * j;
-      row_offset[j] = source(16 * (q >> 1) + row) * (uint32_t)line + 64 * (q & 1) + 16 * quarter;
+    for (int j = 0; j < 8; j++) {   // numbers wave, wave + 4, ...: eight rows, half a piece
+      const int r = 8 * (wave + 4 * j) + row_of_transfer8(lane);
+      row_offset[j] = source(r) * (uint32_t)line + 16 * chunk_of_transfer8(r, lane);
       const int64_t group = min(col0 + 64 * (j >> 1), places - 64) - col0;
       col_offset[j] = (uint32_t)(group / 64 * blocks * (4 * kPieceBytes8)) + (wave + 4 * (j & 1)) * 1024 + lane * 16;
     }
-    row_exponents = source(64 * wave + lane) * exponent_stride;
-    col_exponents = (uint32_t)(min(col0 + 64 * wave + lane, places - 1) - col0) * exponent_stride;
-    row_buffer = buffer8(p.codes + row_base * line), row_exponent_buffer = buffer8(p.exponents + row_base * exponent_stride);
+    row_exponents = source(64 * wave + lane) * 4;
+    col_exponents = (uint32_t)(min(col0 + 64 * wave + lane, places - 1) - col0) * 4;
+    row_buffer = buffer8(p.codes + row_base * line), row_exponent_buffer = buffer8(p.exponents + row_base * 4);
     col_buffer = buffer8(p.packed + (matrix * (places / kPieceLines8) * blocks + piece8(col0 / kPieceLines8, 0, blocks)) * kPieceBytes8);
-    col_exponent_buffer = buffer8(static_cast<const uint8_t*>(p.scales) + (matrix * places + col0) * exponent_stride);
+    col_exponent_buffer = buffer8(static_cast<const uint8_t*>(p.scales) + matrix * places * exponent_stride + col0 * 4);
   };
   const auto fetched = [&]() {   // everything of a block
     if (next.at < stretch_end && ++next_block == next.end) {
@@ -156,22 +154,30 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
     }
   };
   constexpr int kColsOf = 8, kExponentsOf = 2, kUpperOf = 4, kLowerOf = 4;   // transfers of a wavefront, in this order
-  constexpr int kAllOf = kColsOf + kExponentsOf + kUpperOf + kLowerOf;
+  constexpr int kAllOf = kColsOf + kExponentsOf + kUpperOf + kLowerOf, kStores = 32;
+  constexpr uint32_t kOutRange = 1u << 31;
 
   // ------------------------------------------------------------ one step
   f32x4_t total[8][8];
   i32x8_t weights[8], values[4];
   int row_scale[8], col_scale[8];
   int stage = 0;
-  const auto fragment = [&](const char* from) {
+  const auto fragment = [&](const char* first, const char* second) {
     i32x8_t f;
-    const u32x4 a = reinterpret_cast<const u32x4*>(from)[0], b = reinterpret_cast<const u32x4*>(from)[64];
+    const u32x4 a = *reinterpret_cast<const u32x4*>(first), b = *reinterpret_cast<const u32x4*>(second);
 #pragma unroll
     for (int i = 0; i < 4; i++) f[i] = (int)a[i], f[4 + i] = (int)b[i];
     return f;
   };
-  const auto row_fragment = [&](int of, int m) { return fragment(smem + of * kWideSide + lane * 16 + wm * kPieceBytes8 + 2 * m * kPieceBytes8); };
-  const auto col_fragment = [&](int of, int n) { return fragment(smem + 2 * kWideSide + of * kWideSide + lane * 16 + wn * 8 * kPieceBytes8 + n * kPieceBytes8); };
+  const int in_fragment = in_fragment8(lane) + wm * kPieceBytes8;
+  const auto row_fragment = [&](int of, int m) {
+    const char* from = smem + of * kWideSide + 2 * m * kPieceBytes8;
+    return fragment(from + in_fragment, from + (in_fragment ^ 64));
+  };
+  const auto col_fragment = [&](int of, int n) {
+    const char* from = smem + 2 * kWideSide + of * kWideSide + lane * 16 + wn * 8 * kPieceBytes8 + n * kPieceBytes8;
+    return fragment(from, from + 1024);
+  };
   const auto read_scales = [&](int of, int side) {   // as they are: of four blocks
     const int* from = reinterpret_cast<const int*>(smem + kExponentsAt + of * kWideExponents) + row;
 #pragma unroll
@@ -180,9 +186,11 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
       else col_scale[i] = (from + kWideTile + 128 * wn)[16 * i];
     }
   };
+  int stored = 2;   // steps since the last sums were stored by as many instructions as kStores, up to 2
   const auto step = [&](int block) {
     const uint32_t to_rows = lds + stage * kWideSide + wave * 1024, to_cols = to_rows + 2 * kWideSide, to_exponents = lds + kExponentsAt + stage * kWideExponents + wave * 256;
-    const uint32_t start = next_block * kBlock8, start_cols = next_block * (4 * kPieceBytes8), start_exponents = next_block & ~3;
+    const uint32_t start = next_block * kBlock8, start_cols = next_block * (4 * kPieceBytes8);
+    const uint32_t start_row_exponents = (next_block >> 2) * row_lines, start_col_exponents = (next_block >> 2) * col_lines;
     int by_row[8], by_col[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) by_row[i] = row_scale[i] >> (8 * (block & 3)), by_col[i] = col_scale[i] >> (8 * (block & 3));
@@ -191,14 +199,18 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
       constexpr int P = decltype(pair)::value;
       // 1: everybody has read the upper rows and, in the step before, the weights and exponents; the lower rows are there.
       // 3: everybody has read the lower rows; the next weights, exponents and upper rows are there.  Younger than these are as many transfers each time.
-      if constexpr (P == 1 || P == 3) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kAllOf) : "memory");
+      // The stores of a tile are younger than the transfers of the next two steps, but for the second step's last wait, and need not have ended.
+      if constexpr (P == 1 || P == 3) {
+        if (stored < (P == 1 ? 2 : 1)) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kAllOf + kStores) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kAllOf) : "memory");
+      }
       static_for<8>([&](auto at) {
         constexpr int N = decltype(at)::value, M = 2 * P;
         const i32x8_t &upper = values[2 * (P & 1)], &lower = values[2 * (P & 1) + 1];
         if constexpr (P == 1) accumulate8_fetch<4096 * N, 16>(total[M][N], weights[N], upper, by_col[N], by_row[M], col_buffer, col_offset[N], start_cols, to_cols);
         else if constexpr (P == 2 && N < 2)
           accumulate8_fetch<N * kWideTile * 4, 4>(total[M][N], weights[N], upper, by_col[N], by_row[M], N ? col_exponent_buffer : row_exponent_buffer,
-                                                  N ? col_exponents : row_exponents, start_exponents, to_exponents);
+                                                  N ? col_exponents : row_exponents, N ? start_col_exponents : start_row_exponents, to_exponents);
         else if constexpr (P == 2 && N >= 4)
           accumulate8_fetch<4096 * (N - 4), 16>(total[M][N], weights[N], upper, by_col[N], by_row[M], row_buffer, row_offset[N - 4], start, to_rows);
         else if constexpr (P == 3 && N >= 4)
@@ -214,6 +226,7 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
       });
     });
     stage ^= 1;
+    stored = min(stored + 1, 2);
     fetched();
   };
 
@@ -222,7 +235,8 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
     const uint32_t to = lds + s * kWideSide + wave * 1024, to_exponents = lds + kExponentsAt + s * kWideExponents + wave * 256;
 #pragma unroll
     for (int j = 0; j < 8; j++) fetch8<16>(col_buffer, col_offset[j], next_block * (4 * kPieceBytes8), to + 2 * kWideSide + 4096 * j);
-    fetch8<4>(row_exponent_buffer, row_exponents, next_block & ~3, to_exponents), fetch8<4>(col_exponent_buffer, col_exponents, next_block & ~3, to_exponents + kWideTile * 4);
+    fetch8<4>(row_exponent_buffer, row_exponents, (next_block >> 2) * row_lines, to_exponents);
+    fetch8<4>(col_exponent_buffer, col_exponents, (next_block >> 2) * col_lines, to_exponents + kWideTile * 4);
 #pragma unroll
     for (int j = 0; j < 8; j++) fetch8<16>(row_buffer, row_offset[j], next_block * kBlock8, to + 4096 * j);
     fetched();
@@ -233,6 +247,7 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
   for (int n = 0; n < 8; n++) weights[n] = col_fragment(0, n);
   read_scales(0, 0), read_scales(0, 1);
   values[0] = row_fragment(0, 0), values[1] = row_fragment(0, 1);
+  const bool even = !p.sums && !p.by_slot && (reinterpret_cast<uintptr_t>(p.out) & 3) == 0 && p.out_stride % 2 == 0 && p.out_stride <= 1 << 22;   // (256 rows of 8 MiB are kOutRange)
   for (; mine < stretch_end; mine += turn) {
     const Work w = mine == next.at ? next : work_of(mine);
 #pragma unroll
@@ -244,23 +259,40 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
     finish8();
     Product8 to_where = p;
     if constexpr (WHAT == kGradient8) to_where.out = static_cast<uint16_t*>(p.out) + (int64_t)w.t.expert * p.x_rows * p.out_stride;
-    const int64_t first = (int64_t)w.col_tile * kWideTile + 128 * wn + 16 * quarter;
+    const int64_t first = (int64_t)w.col_tile * kWideTile + 128 * wn;
+    // Whole lines of 64 outputs go out by 32-bit offsets, rows that are not there by one that is out of range, always kStores instructions.
+    const bool whole = first + 128 <= p.outputs && even;
+    uint16_t* rows_out = static_cast<uint16_t*>(to_where.out) + (int64_t)w.t.first * p.out_stride + first;
+    u32x4 out_buffer = buffer8(reinterpret_cast<const uint8_t*>(whole ? rows_out : static_cast<uint16_t*>(p.out)));
+    out_buffer[2] = kOutRange;
 #pragma unroll
     for (int m = 0; m < 8; m++) {
 #pragma unroll
       for (int n = 0; n < 8; n++) asm volatile("" : "+a"(total[m][n]));   // (16 rows at a time leave the accumulation registers)
-      int64_t to;
-      float by;
-      const bool is = place_of_row8(to_where, w.t, 16 * (2 * m + wm) + row, to, by);
+      const int r = 16 * (2 * m + wm) + row;
+      f32x4_t sums[2][4];
 #pragma unroll
       for (int g = 0; g < 2; g++) {
-        f32x4_t four[4];
 #pragma unroll
-        for (int n = 0; n < 4; n++) four[n] = total[m][4 * g + n];
-        if constexpr (ACTIVATION != kNoActivation) activate_each8<ACTIVATION>(four);
-        if (is) store8<4>(to_where, to, by, first + 64 * g, four);
+        for (int n = 0; n < 4; n++) sums[g][n] = total[m][4 * g + n];
+        if constexpr (ACTIVATION != kNoActivation) activate_each8<ACTIVATION>(sums[g]);
+      }
+      if (whole) {
+        const uint32_t offset = r < w.t.rows ? (uint32_t)(r * (int)p.out_stride + 8 * quarter) * 2 : kOutRange;
+        const auto store = [&](auto at) {
+          constexpr int I = decltype(at)::value;
+          const f32x4_t &a = sums[I >> 1][2 * (I & 1)], &b = sums[I >> 1][2 * (I & 1) + 1];
+          const u32x4 eight = {pack8(a[0], a[1], p.bf16), pack8(a[2], a[3], p.bf16), pack8(b[0], b[1], p.bf16), pack8(b[2], b[3], p.bf16)};
+          store_eight8<64 * I>(eight, offset, out_buffer);
+        };
+        static_for<4>(store);
+      } else {
+        int64_t to;
+        float by;
+        if (place_of_row8(to_where, w.t, r, to, by)) store_pieces8(to_where, to, by, first, quarter, sums[0]), store_pieces8(to_where, to, by, first + 64, quarter, sums[1]);
       }
     }
+    stored = whole ? 0 : 2;
   }
   wait_vmcnt<0>();
   // rows behind the last expert's
@@ -289,7 +321,6 @@ int launch_wide8(const char* who, const Product8& p, hipStream_t stream) {
     switch (p.activation) {
       case kRelu: launch(std::integral_constant<int, kRelu>()); break;
       case kGeluTanh: launch(std::integral_constant<int, kGeluTanh>()); break;
-      case kGeluErf: launch(std::integral_constant<int, kGeluErf>()); break;
       case kSilu: launch(std::integral_constant<int, kSilu>()); break;
       default: launch(std::integral_constant<int, kNoActivation>());
     }

@@ -32,7 +32,7 @@ template <int DTYPE>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const typename Value<DTYPE>::stored* __restrict__ x, int64_t rows, int64_t size, int64_t stride,
                                                             uint8_t* __restrict__ codes, uint8_t* __restrict__ exponents) {
   typedef typename Value<DTYPE>::stored stored;
-  const int64_t blocks = blocks8(size), along = exponent_stride8(size), teams = (int64_t)gridDim.x * 16;
+  const int64_t blocks = blocks8(size), teams = (int64_t)gridDim.x * 16;
   const int lane = threadIdx.x & 15;
   for (int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); at < rows * blocks; at += teams) {
     const int64_t row = at / blocks, block = at % blocks, first = block * kBlock8 + lane * 8;
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const typename Value
     most = team16_larger(most);
     const int byte = exponent_byte8(most);
     *reinterpret_cast<uint2*>(codes + row * row_stride8(size) + first) = eight_codes(v, most, inverse_power8(byte));
-    if (lane == 0) exponents[row * along + block] = (uint8_t)byte;
+    if (lane == 0) exponents[exponent_at8(row, block, rows)] = (uint8_t)byte;
   }
 }
 
@@ -127,7 +127,6 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(Quantize8 p) {
     }
   }
   if constexpr (ALONG != kNoForm) {
-    const int64_t stride = exponent_stride8(p.cols);
     uint8_t *codes = p.along, *exponents = p.along_exponents;
     if constexpr (ALONG == kPieceForm) {
       codes += (int64_t)blockIdx.z * piece_bytes8(p.rows, p.cols);
@@ -142,11 +141,10 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(Quantize8 p) {
       const int64_t line = ALONG == kPieceForm ? place8(row) : row;
       const int64_t to = ALONG == kPieceForm ? piece_at8(line, first, col_blocks) : row * row_stride8(p.cols) + first;
       *reinterpret_cast<uint2*>(codes + to) = eight_codes(v[i], row_most[i], inverse_power8(byte));
-      if (eighth == 0) exponents[line * stride + blockIdx.x] = (uint8_t)byte;
+      if (eighth == 0) exponents[exponent_at8(line, blockIdx.x, end)] = (uint8_t)byte;
     }
   }
   if constexpr (DOWN != kNoForm) {
-    const int64_t stride = exponent_stride8(p.rows);
     uint8_t *codes = p.down, *exponents = p.down_exponents;
     if constexpr (DOWN == kPieceForm) {
       codes += (int64_t)blockIdx.z * piece_bytes8(p.cols, p.rows);
@@ -163,7 +161,7 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(Quantize8 p) {
         const uint32_t four = codes8(v[4 * h][j] * inverse, v[4 * h + 1][j] * inverse, v[4 * h + 2][j] * inverse, v[4 * h + 3][j] * inverse);
         turned[(8 * eighth + j) * kPitch + 16 * h + quad] = nan ? kNan8 : four;
       }
-      if (quad == 0 && first + j < end) exponents[(DOWN == kPieceForm ? place8(first + j) : first + j) * stride + blockIdx.y] = (uint8_t)byte;
+      if (quad == 0 && first + j < end) exponents[exponent_at8(DOWN == kPieceForm ? place8(first + j) : first + j, blockIdx.y, end)] = (uint8_t)byte;
     }
     __syncthreads();
     // 16 bytes of a column a thread: neighbours within a column of rows, or in the order of a piece
@@ -174,8 +172,7 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(Quantize8 p) {
       int col, chunk;
       if constexpr (DOWN == kPieceForm) {
         const int piece = at >> 7, h = (at >> 6) & 1, lane = at & 63;   // piece of the eight, access, lane
-        const int place = (piece & 3) * 16 + (lane & 15);               // of 64
-        col = (piece >> 2) * 64 + ((place >> 2) & 3) * 16 + (place >> 4) * 4 + (place & 3), chunk = 4 * h + (lane >> 4);
+        col = line_of_place8(piece * 16 + (lane & 15)), chunk = 4 * h + (lane >> 4);
         line = col0 + col;
         to = piece8(col0 / kPieceLines8 + piece, blockIdx.y, row_blocks) * kPieceBytes8 + h * 1024 + lane * 16;
       } else {
@@ -210,7 +207,7 @@ __global__ __launch_bounds__(256) void pack8_scales_kernel(const void* __restric
   const int64_t count = experts * (kind == kPowerScales ? lines * stride : down * blocks), step = (int64_t)gridDim.x * 256;
   for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < count; at += step) {
     if (kind == kPowerScales) {
-      const int64_t e = at / (lines * stride), line = at / stride % lines, b = at % stride;   // (line and its place lie in the same 64, of one scale)
+      const int64_t e = at / (lines * stride), line = at / 4 % lines, b = at / (4 * lines) % (stride / 4) * 4 + at % 4;   // (line and its place lie in the same 64, of one scale)
       static_cast<uint8_t*>(packed)[at] = b < blocks && line / kBlock8 < down ? static_cast<const uint8_t*>(scales)[(e * blocks + b) * down + line / kBlock8] : (uint8_t)127;
     } else {
       const int64_t e = at / (down * blocks), o = at / blocks % down, b = at % blocks;
@@ -221,13 +218,13 @@ __global__ __launch_bounds__(256) void pack8_scales_kernel(const void* __restric
 template <int DTYPE>
 __global__ __launch_bounds__(256) void dequantize8_kernel(const uint8_t* __restrict__ packed, const void* __restrict__ scales, int kind, int64_t experts, int64_t inputs,
                                                           int64_t outputs, typename Value<DTYPE>::stored* __restrict__ out) {
-  const int64_t blocks = blocks8(inputs), stride = exponent_stride8(inputs), step = (int64_t)gridDim.x * 256;
+  const int64_t blocks = blocks8(inputs), step = (int64_t)gridDim.x * 256;
   for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < experts * inputs * outputs; at += step) {
     const int64_t o = at % outputs, i = at / outputs % inputs, e = at / outputs / inputs, place = place8(o);
     const float code = value8(packed[e * piece_bytes8(outputs, inputs) + piece_at8(place, i, blocks)]);
     float v;
     if (kind == kPowerScales) {
-      const int byte = static_cast<const uint8_t*>(scales)[e * scale_bytes8(outputs, inputs, kind) + place * stride + i / kBlock8];
+      const int byte = static_cast<const uint8_t*>(scales)[e * scale_bytes8(outputs, inputs, kind) + exponent_at8(place, i / kBlock8, padded_lines8(outputs))];
       v = byte == 255 ? NAN : ldexpf(code, byte - 127);
     } else {
       v = code * static_cast<const float*>(scales)[(e * blocks8(outputs) + o / kBlock8) * blocks + i / kBlock8];
