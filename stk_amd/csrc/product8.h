@@ -11,7 +11,7 @@
 namespace stk {
 
 bool sizes8(int64_t lines, int64_t size);
-int quantize_rows8(const char* who, const void* x, int64_t rows, int64_t size, int64_t stride, int dtype, uint8_t* codes, uint8_t* exponents, hipStream_t stream);
+int quantize_rows8(const char* who, const void* x, int64_t rows, int64_t size, int64_t stride, int dtype, uint8_t* codes, uint8_t* exponents, const int32_t* indices, int top_k, hipStream_t stream);
 
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -22,12 +22,12 @@ struct Product8 {
   const void* x;                             // 16-bit rows, ...
   int64_t x_stride;
   const uint8_t *codes, *exponents;          // ... or quantised ones
-  int64_t x_rows, rows;                      // rows there are; those multiplied (slots)
+  int64_t x_rows, rows;                      // rows there are (of quantised ones: lines); those multiplied (slots)
   const uint8_t* packed;
   const void* scales;
   int64_t experts, inputs, outputs;
   const int32_t *indices, *bins;
-  int top_k;                                 // gathered: row p reads token indices[p] / top_k; 0: row p itself
+  int top_k;                                 // 16-bit rows gathered: row p reads token indices[p] / top_k; 0, and quantised ones: row p itself
   void* out;                                 // 16-bit rows in the order of the rows, or with `by_slot` of the slots, times `weights` of these, ...
   int64_t out_stride;
   bool by_slot;

@@ -208,18 +208,11 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
   }
   const int blocks = (int)blocks8(p.inputs), exponent_stride = (int)exponent_stride8(p.inputs);
   const int64_t places = padded_lines8(p.outputs), col0 = (int64_t)col_tile * T::kCols;
-  const bool gathered = WHAT == kRows8 && p.top_k > 0;
-  const int64_t row_base = gathered ? 0 : t.first;
-  const auto source_row = [&](int r) {   // from row_base on
-    r = r < t.rows ? r : 0;
-    if (!gathered) return (uint32_t)r;
-    const int slot = p.indices[t.first + r];
-    return (unsigned)slot < (unsigned)p.rows ? (uint32_t)(slot / p.top_k) : 0u;
-  };
+  const auto source_row = [&](int r) { return r < t.rows ? r : 0; };   // of the tile
   // transfers of 1 KiB: eight rows, half a piece; this wavefront's are number wave, wave + kWaves, ...
   constexpr int kRowMoves = T::kRows / 8 / T::kWaves, kColMoves = T::kCols / 8 / T::kWaves, kRowChunks = (T::kRows + 63) / 64, kChunks = kRowChunks + WN;
   static_assert(T::kRows / 8 % T::kWaves == 0 && T::kCols / 8 % T::kWaves == 0, "whole shares");
-  const u32x4 row_buffer = buffer8(p.codes + row_base * row_stride8(p.inputs));
+  const u32x4 row_buffer = buffer8(p.codes + t.first * row_stride8(p.inputs));
   uint32_t row_offset[kRowMoves];
 #pragma unroll
   for (int j = 0; j < kRowMoves; j++) {
@@ -240,7 +233,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
 #pragma unroll
   for (int j = 0; j < kScaleMoves; j++) {
     const int c = wave + T::kWaves * j;
-    if (c < kRowChunks) scale_from[j] = p.exponents + (row_base + source_row(64 * c + lane)) * 4;
+    if (c < kRowChunks) scale_from[j] = p.exponents + ((int64_t)t.first + source_row(64 * c + lane)) * 4;
     else scale_from[j] = static_cast<const uint8_t*>(p.scales) + matrix * places * exponent_stride + min(col0 + 64 * (c - kRowChunks) + lane, places - 1) * 4;
   }
   const uint32_t lds = (uint32_t)(uintptr_t)(STK_LDS char*)smem;
@@ -444,9 +437,9 @@ static ProductKernel8 product_kernel8(int64_t rows, int64_t experts, int64_t inp
   if (along >= 24 || (along >= 8 && tiles <= 4096)) return kStream8_414;
   return tiles <= 4096 ? kStream8_222 : kStream8_144;
 }
-static int64_t workspace8(int64_t x_rows, int64_t rows, int64_t experts, int64_t inputs, int64_t outputs) {
+static int64_t workspace8(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs) {
   if (rows < 1 || product_kernel8(rows, experts, inputs, outputs) < kTile8_32) return 0;
-  return (x_rows * (row_stride8(inputs) + exponent_stride8(inputs)) + 255) / 256 * 256;
+  return (rows * (row_stride8(inputs) + exponent_stride8(inputs)) + 255) / 256 * 256;
 }
 template <int WHAT>
 static int launch_tiles8(const char* who, const Product8& p, int kind, ProductKernel8 kernel, hipStream_t stream) {
@@ -464,9 +457,10 @@ static int launch_product8(const char* who, Product8 p, int kind, int dtype, voi
   const ProductKernel8 kernel = product_kernel8(p.rows, p.experts, p.inputs, p.outputs);
   if (kernel >= kTile8_32) {
     uint8_t* codes = static_cast<uint8_t*>(workspace);
-    uint8_t* exponents = codes + p.x_rows * row_stride8(p.inputs);
-    if (int rc = quantize_rows8(who, p.x, p.x_rows, p.inputs, p.x_stride, dtype, codes, exponents, stream)) return rc;
-    p.codes = codes, p.exponents = exponents;
+    uint8_t* exponents = codes + p.rows * row_stride8(p.inputs);
+    // (gathered here: for one expert per token that costs nothing, and a tile's rows are neighbours)
+    if (int rc = quantize_rows8(who, p.x, p.rows, p.inputs, p.x_stride, dtype, codes, exponents, p.top_k > 0 ? p.indices : nullptr, p.top_k, stream)) return rc;
+    p.codes = codes, p.exponents = exponents, p.x_rows = p.rows, p.top_k = 0;
     return launch_tiles8<kRows8>(who, p, kind, kernel, stream);
   }
   if (most_tiles8(p, 16) > (int64_t)65535 * 65535) return fail(STK_ERR_UNSUPPORTED, "%s: %lld rows", who, (long long)p.rows);
@@ -500,7 +494,7 @@ extern "C" int stk_8bit_product_kernel(int64_t rows, int64_t experts, int64_t in
   return rows < 1 || experts < 1 || inputs < 1 || outputs < 1 ? -1 : (int)product_kernel8(rows, experts, inputs, outputs);
 }
 extern "C" size_t stk_matmul_8bit_workspace_bytes(int64_t x_rows, int64_t rows, int64_t experts, int64_t inputs, int64_t outputs) {
-  return x_rows < 1 || experts < 1 || inputs < 1 || outputs < 1 ? 0 : (size_t)workspace8(x_rows, rows, experts, inputs, outputs);
+  return x_rows < 1 || experts < 1 || inputs < 1 || outputs < 1 ? 0 : (size_t)workspace8(rows, experts, inputs, outputs);
 }
 extern "C" size_t stk_matmul_8bit_scatter_workspace_bytes(int64_t slots, int top_k, int64_t experts, int64_t inputs, int64_t outputs) {
   const size_t rows = stk_matmul_8bit_workspace_bytes(slots, slots, experts, inputs, outputs);

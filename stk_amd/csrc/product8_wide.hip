@@ -124,14 +124,8 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
     }
     next_block = next.begin;
     const RowTile8 t = next.t;
-    const bool gathered = WHAT == kRows8 && p.top_k > 0;
-    const int64_t row_base = gathered ? 0 : t.first, line = row_stride8(p.inputs);
-    const auto source = [&](int r) {   // from row_base on
-      r = r < t.rows ? r : 0;
-      if (!gathered) return (uint32_t)r;
-      const int slot = p.indices[t.first + r];
-      return (unsigned)slot < (unsigned)p.rows ? (uint32_t)(slot / p.top_k) : 0u;
-    };
+    const int64_t line = row_stride8(p.inputs);
+    const auto source = [&](int r) { return (uint32_t)(r < t.rows ? r : 0); };   // of the tile
     const int64_t matrix = WHAT == kGradient8 ? 0 : t.expert, col0 = (int64_t)next.col_tile * kWideTile;
 #pragma unroll
     for (int j = 0; j < 8; j++) {   // numbers wave, wave + 4, ...: eight rows, half a piece
@@ -142,7 +136,7 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
     }
     row_exponents = source(64 * wave + lane) * 4;
     col_exponents = (uint32_t)(min(col0 + 64 * wave + lane, places - 1) - col0) * 4;
-    row_buffer = buffer8(p.codes + row_base * line), row_exponent_buffer = buffer8(p.exponents + row_base * 4);
+    row_buffer = buffer8(p.codes + t.first * line), row_exponent_buffer = buffer8(p.exponents + (int64_t)t.first * 4);
     col_buffer = buffer8(p.packed + (matrix * (places / kPieceLines8) * blocks + piece8(col0 / kPieceLines8, 0, blocks)) * kPieceBytes8);
     col_exponent_buffer = buffer8(static_cast<const uint8_t*>(p.scales) + matrix * places * exponent_stride + col0 * 4);
   };
@@ -154,7 +148,7 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
     }
   };
   constexpr int kColsOf = 8, kExponentsOf = 2, kUpperOf = 4, kLowerOf = 4;   // transfers of a wavefront, in this order
-  constexpr int kAllOf = kColsOf + kExponentsOf + kUpperOf + kLowerOf, kStores = 32;
+  constexpr int kAllOf = kColsOf + kExponentsOf + kUpperOf + kLowerOf;
   constexpr uint32_t kOutRange = 1u << 31;
 
   // ------------------------------------------------------------ one step
@@ -186,7 +180,7 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
       else col_scale[i] = (from + kWideTile + 128 * wn)[16 * i];
     }
   };
-  int stored = 2;   // steps since the last sums were stored by as many instructions as kStores, up to 2
+  int stored = 2, stores = 0;   // steps since the last sums were stored, up to 2, and by at least how many instructions (0, 16 or 32)
   const auto step = [&](int block) {
     const uint32_t to_rows = lds + stage * kWideSide + wave * 1024, to_cols = to_rows + 2 * kWideSide, to_exponents = lds + kExponentsAt + stage * kWideExponents + wave * 256;
     const uint32_t start = next_block * kBlock8, start_cols = next_block * (4 * kPieceBytes8);
@@ -201,7 +195,9 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
       // 3: everybody has read the lower rows; the next weights, exponents and upper rows are there.  Younger than these are as many transfers each time.
       // The stores of a tile are younger than the transfers of the next two steps, but for the second step's last wait, and need not have ended.
       if constexpr (P == 1 || P == 3) {
-        if (stored < (P == 1 ? 2 : 1)) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kAllOf + kStores) : "memory");
+        const int young = stored < (P == 1 ? 2 : 1) ? stores : 0;
+        if (young == 32) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kAllOf + 32) : "memory");
+        else if (young == 16) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kAllOf + 16) : "memory");
         else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kAllOf) : "memory");
       }
       static_for<8>([&](auto at) {
@@ -260,7 +256,7 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
     Product8 to_where = p;
     if constexpr (WHAT == kGradient8) to_where.out = static_cast<uint16_t*>(p.out) + (int64_t)w.t.expert * p.x_rows * p.out_stride;
     const int64_t first = (int64_t)w.col_tile * kWideTile + 128 * wn;
-    // Whole lines of 64 outputs go out by 32-bit offsets, rows that are not there by one that is out of range, always kStores instructions.
+    // Whole lines of 64 outputs go out by 32-bit offsets, rows that are not there by one that is out of range, four instructions for 16 rows.
     const bool whole = first + 128 <= p.outputs && even;
     uint16_t* rows_out = static_cast<uint16_t*>(to_where.out) + (int64_t)w.t.first * p.out_stride + first;
     u32x4 out_buffer = buffer8(reinterpret_cast<const uint8_t*>(whole ? rows_out : static_cast<uint16_t*>(p.out)));
@@ -270,6 +266,7 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
 #pragma unroll
       for (int n = 0; n < 8; n++) asm volatile("" : "+a"(total[m][n]));   // (16 rows at a time leave the accumulation registers)
       const int r = 16 * (2 * m + wm) + row;
+      if (r - row >= w.t.rows) break;   // (none of the 16)
       f32x4_t sums[2][4];
 #pragma unroll
       for (int g = 0; g < 2; g++) {
@@ -292,7 +289,7 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
         if (place_of_row8(to_where, w.t, r, to, by)) store_pieces8(to_where, to, by, first, quarter, sums[0]), store_pieces8(to_where, to, by, first + 64, quarter, sums[1]);
       }
     }
-    stored = whole ? 0 : 2;
+    stored = 0, stores = !whole ? 0 : w.t.rows > 16 * (14 + wm) ? 32 : w.t.rows > 16 * (6 + wm) ? 16 : 0;   // (four for every 16 rows)
   }
   wait_vmcnt<0>();
   // rows behind the last expert's

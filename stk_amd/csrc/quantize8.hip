@@ -27,16 +27,21 @@ __device__ __forceinline__ uint2 eight_codes(const float (&v)[8], uint32_t most,
   return make_uint2(codes8(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse), codes8(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse));
 }
 
-// Rows alone: a team of 16 lanes takes 128 values of a row.
+// Rows alone: a team of 16 lanes takes 128 values of a row.  With indices: row r is that of the token indices[r] / top_k (there are rows / top_k).
 template <int DTYPE>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const typename Value<DTYPE>::stored* __restrict__ x, int64_t rows, int64_t size, int64_t stride,
-                                                            uint8_t* __restrict__ codes, uint8_t* __restrict__ exponents) {
+                                                            uint8_t* __restrict__ codes, uint8_t* __restrict__ exponents, const int32_t* __restrict__ indices, int top_k) {
   typedef typename Value<DTYPE>::stored stored;
   const int64_t blocks = blocks8(size), teams = (int64_t)gridDim.x * 16;
   const int lane = threadIdx.x & 15;
   for (int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); at < rows * blocks; at += teams) {
     const int64_t row = at / blocks, block = at % blocks, first = block * kBlock8 + lane * 8;
-    const stored* from = x + row * stride + first;
+    int64_t token = row;
+    if (indices) {
+      const int slot = indices[row];
+      token = (unsigned)slot < (unsigned)rows ? slot / top_k : 0;
+    }
+    const stored* from = x + token * stride + first;
     float v[8];
     if (first + 8 <= size) load8<DTYPE>(v, from);
     else {
@@ -241,11 +246,12 @@ static dim3 loop_grid8(int64_t count, int64_t each) {
 // What a tensor's sizes may be: positions within one are counted in 64 bits, blocks and lines in 32.
 bool sizes8(int64_t lines, int64_t size) { return lines <= INT32_MAX - 512 && size <= INT32_MAX - 512; }
 
-int quantize_rows8(const char* who, const void* x, int64_t rows, int64_t size, int64_t stride, int dtype, uint8_t* codes, uint8_t* exponents, hipStream_t stream) {
+int quantize_rows8(const char* who, const void* x, int64_t rows, int64_t size, int64_t stride, int dtype, uint8_t* codes, uint8_t* exponents, const int32_t* indices, int top_k,
+                   hipStream_t stream) {
   const dim3 grid = loop_grid8(rows * blocks8(size), 16);
   for_dtype(dtype, [&](auto d) {
     typedef typename Value<d()>::stored T;
-    hipLaunchKernelGGL((quantize_rows_kernel<d()>), grid, dim3(256), 0, stream, static_cast<const T*>(x), rows, size, stride, codes, exponents);
+    hipLaunchKernelGGL((quantize_rows_kernel<d()>), grid, dim3(256), 0, stream, static_cast<const T*>(x), rows, size, stride, codes, exponents, indices, top_k);
   });
   return check_launch(who);
 }
@@ -330,7 +336,7 @@ extern "C" int stk_quantize_rows_8bit(const void* x, int64_t rows, int64_t size,
   if (!x || !codes != !exponents || !columns != !column_exponents || (!codes && !columns)) return fail(STK_ERR_DIMS, "%s: missing pointer", who);
   if ((codes && !aligned16(codes)) || (columns && !aligned16(columns))) return fail(STK_ERR_UNSUPPORTED, "%s: codes at a multiple of 16 bytes", who);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (!columns) return quantize_rows8(who, x, rows, size, stride, dtype, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(exponents), s);
+  if (!columns) return quantize_rows8(who, x, rows, size, stride, dtype, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(exponents), nullptr, 1, s);
   const Quantize8 p = {x, 0, stride, 1, rows, size, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(exponents), static_cast<uint8_t*>(columns),
                        static_cast<uint8_t*>(column_exponents)};
   if (codes) return pieces ? quantize_blocks<kRowForm, kPieceForm, false>(who, p, 1, dtype, s) : quantize_blocks<kRowForm, kRowForm, false>(who, p, 1, dtype, s);
