@@ -80,12 +80,21 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(Quantize8 p) {
   const stored* x = static_cast<const stored*>(p.x) + (int64_t)blockIdx.z * p.stride_e;
   const int64_t first = col0 + 8 * eighth;
   float v[8][8];
+  if (first + 8 <= p.cols && p.stride_c == 1) {   // (all eight rows on their way together; behind the last one it once more, and then zeros)
+    decltype(fetch8<DTYPE>(x)) raw[8];
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const int64_t row = row0 + 64 * (i >> 2) + 4 * quad + (i & 3);
-    const stored* from = x + row * p.stride_r + first * p.stride_c;
-    if (row < p.rows && first + 8 <= p.cols && p.stride_c == 1) load8<DTYPE>(v[i], from);
-    else {
+    for (int i = 0; i < 8; i++) raw[i] = fetch8<DTYPE>(x + min(row0 + 64 * (i >> 2) + 4 * quad + (i & 3), p.rows - 1) * p.stride_r + first);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      widen8<DTYPE>(v[i], raw[i]);
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[i][j] = row0 + 64 * (i >> 2) + 4 * quad + (i & 3) < p.rows ? v[i][j] : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int64_t row = row0 + 64 * (i >> 2) + 4 * quad + (i & 3);
+      const stored* from = x + row * p.stride_r + first * p.stride_c;
 #pragma unroll
       for (int j = 0; j < 8; j++) v[i][j] = row < p.rows && first + j < p.cols ? Value<DTYPE>::widen(from[j * p.stride_c]) : 0.f;
     }
