@@ -164,17 +164,17 @@ __global__ __launch_bounds__(64 * KW * NW) void stream8_kernel(Product8 p) {
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
-// WM x WN wavefronts share 16 MT WM rows and 64 WN outputs, a block of 128 inputs at a time in two stages of LDS that are filled without
-// registers: pieces of weights as they lie in memory, rows by whole lines.  Exponents come four blocks at a time.
-template <int WM, int WN, int MT>
+// WM x WN wavefronts share 16 MT WM rows and 64 WN outputs, a block of 128 inputs at a time in stages of LDS that are filled without
+// registers: pieces of weights as they lie in memory, rows by whole lines, exponents of four blocks in a dword.
+template <int WM, int WN, int MT, int STAGES>
 struct Tile8 {
   static constexpr int kWaves = WM * WN, kRows = 16 * MT * WM, kCols = 64 * WN;
-  static constexpr int kRowBytes = kRows * kBlock8, kStage = (kRows + kCols) * kBlock8, kExponents = (kRows + kCols) * 4;
-  static constexpr int kBytes = 2 * (kStage + kExponents);
+  static constexpr int kRowBytes = kRows * kBlock8, kCodes = (kRows + kCols) * kBlock8, kStage = kCodes + (kRows + kCols) * 4;
+  static constexpr int kBytes = STAGES * kStage;
 };
-template <int KIND, int WHAT, int WM, int WN, int MT>
+template <int KIND, int WHAT, int WM, int WN, int MT, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row_tiles, int col_tiles) {
-  typedef Tile8<WM, WN, MT> T;
+  typedef Tile8<WM, WN, MT, STAGES> T;
   extern __shared__ char smem[];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   const int row = lane & 15, quarter = lane >> 4, in_fragment = in_fragment8(lane);
@@ -227,30 +227,28 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
     const int64_t piece = min(col0 / kPieceLines8 + (q >> 1), places / kPieceLines8 - 1);
     col_from[j] = uniform_global(p.packed + (matrix * (places / kPieceLines8) * blocks + piece8(piece, 0, blocks)) * kPieceBytes8 + 1024 * (q & 1));
   }
-  // exponents: 64 lines a transfer, first those of the rows
-  constexpr int kScaleMoves = (kChunks + T::kWaves - 1) / T::kWaves;
+  // exponents: 64 lines a transfer, first those of the rows; each wavefront makes as many (the last ones twice)
+  constexpr int kLines = KIND == kPowerScales ? kChunks : kRowChunks, kScaleMoves = (kLines + T::kWaves - 1) / T::kWaves;
+  constexpr int kMoves = kRowMoves + kColMoves + kScaleMoves;
   const uint8_t* scale_from[kScaleMoves];
 #pragma unroll
   for (int j = 0; j < kScaleMoves; j++) {
-    const int c = wave + T::kWaves * j;
+    const int c = min(wave + T::kWaves * j, kLines - 1);
     if (c < kRowChunks) scale_from[j] = p.exponents + ((int64_t)t.first + source_row(64 * c + lane)) * 4;
     else scale_from[j] = static_cast<const uint8_t*>(p.scales) + matrix * places * exponent_stride + min(col0 + 64 * (c - kRowChunks) + lane, places - 1) * 4;
   }
   const uint32_t lds = (uint32_t)(uintptr_t)(STK_LDS char*)smem;
-  const auto issue = [&](int block, int stage, bool exponents_too, int place) {
+  const auto issue = [&](int block, int stage) {
     const uint32_t to = lds + stage * T::kStage;
 #pragma unroll
     for (int j = 0; j < kRowMoves; j++) fetch8<16>(row_buffer, row_offset[j], block * kBlock8, to + (wave + T::kWaves * j) * 1024);
 #pragma unroll
     for (int j = 0; j < kColMoves; j++) dma16(col_from[j] + (int64_t)block * (4 * kPieceBytes8), lane * 16, to + T::kRowBytes + (wave + T::kWaves * j) * 1024);
-    if (exponents_too) {
-      const uint32_t exponents = lds + 2 * T::kStage + place * T::kExponents;
 #pragma unroll
-      for (int j = 0; j < kScaleMoves; j++) {
-        const int c = wave + T::kWaves * j;
-        if (c < (KIND == kPowerScales ? kChunks : kRowChunks) && (T::kRows >= 64 || c >= kRowChunks || lane < T::kRows))
-          dma4_from(scale_from[j] + (block >> 2) * (c < kRowChunks ? p.x_rows : places) * 4, exponents + (c < kRowChunks ? c * 256 : T::kRows * 4 + (c - kRowChunks) * 256));
-      }
+    for (int j = 0; j < kScaleMoves; j++) {
+      const int c = min(wave + T::kWaves * j, kLines - 1);
+      if (T::kRows >= 64 || c >= kRowChunks || lane < T::kRows)
+        dma4_from(scale_from[j] + (block >> 2) * (c < kRowChunks ? p.x_rows : places) * 4, to + T::kCodes + (c < kRowChunks ? c * 256 : T::kRows * 4 + (c - kRowChunks) * 256));
     }
   };
   const float* float_scales = static_cast<const float*>(p.scales) + (matrix * blocks8(p.outputs) + min((col0 + 64 * wn) / kBlock8, blocks8(p.outputs) - 1)) * blocks;
@@ -260,36 +258,27 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
   for (int m = 0; m < MT; m++)
 #pragma unroll
     for (int n = 0; n < 4; n++) total[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  int row_scale[MT], col_scale[4] = {127, 127, 127, 127};
   // this wavefront's rows are fragments wm, wm + WM, ... of 16, of which so many have any
   const int fragments = ((t.rows + 15) / 16 - wm + WM - 1) / WM;
-  // Column tiles start at different blocks and go round: those of one block lie a fixed distance apart, which would all be in a few of the memory's channels.
   const int count = end - begin;
-  int block = begin, place = 0;   // place: of the exponents in use
-  bool fresh = true;
-  if (count > 0) issue(block, 0, true, 0);
-  for (int step = 0; step < count; step++) {
-    const int stage = step & 1;
-    wait_vmcnt<0>();
-    __syncthreads();   // everybody's part of the block is there, and everybody is done with the one whose place is filled now
-    const int next = block + 1 < end ? block + 1 : begin;
-    const bool next_fresh = next == begin || (next & 3) == 0;
-    if (step + 1 < count) issue(next, stage ^ 1, next_fresh, place ^ 1);
-    if (fresh) {
-      const int* exponents = reinterpret_cast<const int*>(smem + 2 * T::kStage + place * T::kExponents);
 #pragma unroll
-      for (int m = 0; m < MT; m++) row_scale[m] = exponents[16 * (m * WM + wm) + row] >> (8 * (block & 3));
-      if constexpr (KIND == kPowerScales) {
+  for (int s = 0; s < STAGES - 1; s++)
+    if (s < count) issue(begin + s, s);
+  for (int step = 0, stage = 0; step < count; step++, stage = stage + 1 < STAGES ? stage + 1 : 0) {
+    const int block = begin + step;
+    // everybody's part of the block is there, and everybody is done with the one whose place is filled now
+    if (STAGES > 3 && step + 2 < count) wait_vmcnt<2 * kMoves>();
+    else if (STAGES > 2 && step + 1 < count) wait_vmcnt<kMoves>();
+    else wait_vmcnt<0>();
+    __syncthreads();
+    if (step + STAGES - 1 < count) issue(block + STAGES - 1, stage > 0 ? stage - 1 : STAGES - 1);
+    int row_scale[MT], col_scale[4] = {127, 127, 127, 127};
+    const int* exponents = reinterpret_cast<const int*>(smem + stage * T::kStage + T::kCodes);
 #pragma unroll
-        for (int n = 0; n < 4; n++) col_scale[n] = exponents[T::kRows + 64 * wn + 16 * n + row] >> (8 * (block & 3));
-      }
-    } else {
+    for (int m = 0; m < MT; m++) row_scale[m] = exponents[16 * (m * WM + wm) + row] >> (8 * (block & 3));
+    if constexpr (KIND == kPowerScales) {
 #pragma unroll
-      for (int m = 0; m < MT; m++) row_scale[m] >>= 8;
-      if constexpr (KIND == kPowerScales) {
-#pragma unroll
-        for (int n = 0; n < 4; n++) col_scale[n] >>= 8;
-      }
+      for (int n = 0; n < 4; n++) col_scale[n] = exponents[T::kRows + 64 * wn + 16 * n + row] >> (8 * (block & 3));
     }
     const float by = KIND == kFloatScales ? __uint_as_float((uint32_t)const_ints(float_scales)[block]) : 1.f;
     const char* rows = smem + stage * T::kStage + wm * kPieceBytes8;
@@ -327,7 +316,6 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // (the accesses to LDS come first)
       __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
     }
-    block = next, fresh = next_fresh, place ^= (int)next_fresh;
   }
   if constexpr (WHAT == kGradient8) p.out = static_cast<uint16_t*>(p.out) + (int64_t)expert * p.x_rows * p.out_stride;
 #pragma unroll
@@ -396,15 +384,15 @@ static void launch_stream8(const Product8& p, int kind, hipStream_t stream) {
   if (p.bf16) by_kind(std::true_type());
   else by_kind(std::false_type());
 }
-template <int WHAT, int WM, int WN, int MT>
+template <int WHAT, int WM, int WN, int MT, int STAGES>
 static int launch_tiles8(const char* who, const Product8& p, int kind, hipStream_t stream) {
-  typedef Tile8<WM, WN, MT> T;
+  typedef Tile8<WM, WN, MT, STAGES> T;
   const int64_t row_tiles = WHAT == kGradient8 ? (p.x_rows + T::kRows - 1) / T::kRows : most_tiles8(p, T::kRows), col_tiles = (p.outputs + T::kCols - 1) / T::kCols;
   const int64_t matrices = WHAT == kGradient8 ? p.experts : 1;
   if (row_tiles > INT32_MAX / col_tiles / matrices) return fail(STK_ERR_UNSUPPORTED, "%s: too many tiles", who);
   const dim3 grid((unsigned)(row_tiles * col_tiles * matrices));
   const auto launch = [&](auto k) {
-    const auto kernel = tile8_kernel<decltype(k)::value, WHAT, WM, WN, MT>;
+    const auto kernel = tile8_kernel<decltype(k)::value, WHAT, WM, WN, MT, STAGES>;
     set_lds_limit(kernel, T::kBytes);
     hipLaunchKernelGGL(kernel, grid, dim3(64 * T::kWaves), T::kBytes, stream, p, (int)row_tiles, (int)col_tiles);
   };
@@ -414,7 +402,8 @@ static int launch_tiles8(const char* who, const Product8& p, int kind, hipStream
   return check_launch(who);
 }
 
-// Which kernel.
+// Which kernel.  The tiles reach their rows by 32 bits.
+constexpr int64_t kMostTileInputs8 = 1 << 23;
 enum ProductKernel8 : int { kStream8_811 = 0, kStream8_412, kStream8_414, kStream8_222, kStream8_144, kTile8_32, kTile8_64, kTile8_128, kTile8_256 };
 static ProductKernel8 product_kernel8(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs) {
   const int64_t along = blocks8(inputs), down = padded_lines8(outputs) / kPieceLines8;
@@ -425,10 +414,13 @@ static ProductKernel8 product_kernel8(int64_t rows, int64_t experts, int64_t inp
   // rows 11.6 and 25.2, 128 rows 18.7 and 25.3; 1024 x 4096, 64 rows 5.8 and 10.0; 37 rows of 2944 x 1151 6.1 and 20.0; 8 experts of 1024 x 1024, 40
   // rows each 8.3 and 11.5; 64 experts of 1024 x 4096, 20 rows each 77 and 68, 40 rows each 113 and 83.
   const int64_t tiles = hit * ((each + 15) / 16) * down;
-  if (each > 16 && tiles > 2048 + 8192 / along) {
-    if (each > 64 && hit * ((each + 255) / 256) * ((outputs + 255) / 256) >= 192) return kTile8_256;
-    if (each > 64 && hit * ((each + 127) / 128) * ((outputs + 127) / 128) >= 192) return kTile8_128;
-    return each > 32 ? kTile8_64 : kTile8_32;
+  if (each > 16 && tiles > 2048 + 8192 / along && inputs <= kMostTileInputs8) {
+    // Larger tiles read less, smaller ones fill the chip.  4096 x 4096, tiles of 32, 64, 128, 256 rows: 256 rows 22, 28, 38, 57 us; 1024 rows 52, 35, 42, 60;
+    // 2048 rows 90, 65, 53, 65; 64 experts of 1024 x 4096, 20 rows each 76, 68, 73, 87, 64 rows each 109, 98, 101, 93, 128 rows each 165, 129, 141, 109.
+    const auto count = [&](int64_t high, int64_t wide) { return hit * ((each + high - 1) / high) * ((outputs + wide - 1) / wide); };
+    if (each > 64 && count(256, 256) >= 192) return kTile8_256;
+    if (each > 64 && count(128, 128) > 256) return kTile8_128;
+    return count(64, 128) > 256 ? kTile8_64 : kTile8_32;
   }
   // The fewer tiles there are the more wavefronts share the inputs of one: 1 row of 4096 x 4096 (256 tiles) 6.2, 8.8, 10.8 us by 8, 4 and 4 for two and four
   // pieces; 20 rows (512) 10.8, 9.5, 11.2; 64 rows (1024) 21.5, 14.1, 11.6.
@@ -444,12 +436,14 @@ static int64_t workspace8(int64_t rows, int64_t experts, int64_t inputs, int64_t
 template <int WHAT>
 static int launch_tiles8(const char* who, const Product8& p, int kind, ProductKernel8 kernel, hipStream_t stream) {
   switch (kernel) {
-    case kTile8_32: return launch_tiles8<WHAT, 2, 2, 1>(who, p, kind, stream);
-    case kTile8_64: return launch_tiles8<WHAT, 2, 2, 2>(who, p, kind, stream);
-    case kTile8_128: return launch_tiles8<WHAT, 2, 2, 4>(who, p, kind, stream);
+    case kTile8_32: return launch_tiles8<WHAT, 2, 2, 1, 3>(who, p, kind, stream);
+    case kTile8_64: return launch_tiles8<WHAT, 2, 2, 2, 2>(who, p, kind, stream);
+    case kTile8_128: return launch_tiles8<WHAT, 2, 2, 4, 2>(who, p, kind, stream);
     default:
-      if (kind == kPowerScales && p.activation != kGeluErf) return launch_wide8<WHAT>(who, p, stream);   // (erf's registers do not fit beside 256 sums)
-      return launch_tiles8<WHAT, 2, 4, 8>(who, p, kind, stream);
+      if constexpr (WHAT == kRows8) {
+        if (kind != kPowerScales || p.activation == kGeluErf) return launch_tiles8<WHAT, 2, 4, 8, 2>(who, p, kind, stream);   // (erf's registers do not fit beside 256 sums)
+      }
+      return launch_wide8<WHAT>(who, p, stream);
   }
 }
 // The product of 16-bit rows; the workspace holds them quantised where there are many.
@@ -568,6 +562,7 @@ extern "C" int stk_linear_8bit(const void* codes, const void* exponents, int64_t
   if (rows == 0) return STK_OK;
   if (!exponents || (!bins && experts > 1)) return fail(STK_ERR_DIMS, "%s: missing pointer", who);
   if (!aligned16(codes)) return fail(STK_ERR_UNSUPPORTED, "%s: codes at a multiple of 16 bytes", who);
+  if (inputs > kMostTileInputs8) return fail(STK_ERR_UNSUPPORTED, "%s: %lld inputs", who, (long long)inputs);
   const ProductKernel8 kernel = product_kernel8(rows, experts, inputs, outputs);
   return launch_tiles8<kRows8>(who, p, kPowerScales, kernel < kTile8_32 ? kTile8_32 : kernel, static_cast<hipStream_t>(stream));
 }
@@ -582,6 +577,8 @@ extern "C" int stk_weight_gradient_8bit(const void* columns, const void* exponen
   if (int rc = product_check8(who, p, dtype)) return rc;
   if (!exponents || (!bins && experts > 1)) return fail(STK_ERR_DIMS, "%s: missing pointer", who);
   if (!aligned16(columns)) return fail(STK_ERR_UNSUPPORTED, "%s: codes at a multiple of 16 bytes", who);
-  const ProductKernel8 kernel = experts * ((inputs + 255) / 256) * ((outputs + 255) / 256) >= 192 ? kTile8_256 : kTile8_128;
+  if (rows > kMostTileInputs8) return fail(STK_ERR_UNSUPPORTED, "%s: %lld rows", who, (long long)rows);
+  const auto count = [&](int64_t side) { return experts * ((inputs + side - 1) / side) * ((outputs + 127) / 128); };
+  const ProductKernel8 kernel = experts * ((inputs + 255) / 256) * ((outputs + 255) / 256) >= 192 ? kTile8_256 : count(128) >= 192 ? kTile8_128 : count(64) >= 192 ? kTile8_64 : kTile8_32;
   return launch_tiles8<kGradient8>(who, p, kPowerScales, kernel, static_cast<hipStream_t>(stream));
 }

@@ -177,3 +177,46 @@ def test_refusals():
         stk.ops.group_top_experts(s, 2, bias=torch.zeros(64))
     with pytest.raises(AssertionError):
         stk.ops.group_top_experts(s[0], 2)
+
+
+# more tokens than get a wavefront each
+MANY = [(2100, 256, 8, 4, 8, 2), (3000, 160, 8, 3, 6, 1), (2500, 64, 16, 3, 4, 2), (2049, 30, 3, 2, 10, 2), (4001, 8, 1, 1, 2, 1), (2300, 128, 2, 1, 16, 1), (2200, 100, 1, 1, 5, 1)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scoring,normalize,bias", [("sigmoid", True, True), ("softmax", False, False), ("softmax", True, True), ("sigmoid", False, False)])
+@pytest.mark.parametrize("tokens,experts,groups,top_groups,top_k,best", MANY)
+def test_many_tokens(tokens, experts, groups, top_groups, top_k, best, scoring, normalize, bias, dtype):
+    scores, b, g = _case(tokens, experts, dtype, tokens + experts, bias)
+    _check(scores, b, top_k, groups, top_groups, best, scoring, normalize, 2.5, torch.randn(tokens, top_k, generator=g))
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_many_tokens_that_fp32_does_not_tell_apart(scoring):
+    """Some of the tokens of a workgroup, or all."""
+    g = torch.Generator().manual_seed(8)
+    s = torch.randn(1, 256, generator=g)
+    n64 = s.double().numpy()[0]
+    p = 1 / (1 + np.exp(-n64)) if scoring == "sigmoid" else np.exp(n64 - n64.max()) / np.exp(n64 - n64.max()).sum()
+    level = torch.randint(1, 4, (256,), generator=g).double().numpy() / 4
+    bias = torch.from_numpy(level - p + 1e-8 * torch.randn(256, generator=g).double().numpy()).float()
+    scores = s.repeat(2100, 1)
+    scores[1000:] += (torch.rand(1100, 1, generator=g) < 0.7) * torch.randn(1100, 256, generator=g)
+    _check(scores, bias, 8, 8, 4, 2, scoring, True, 1.0)
+    _check(scores, bias, 8, 1, 1, 1, scoring, False, 1.0)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("bias", [None, "some"])
+def test_many_tokens_of_ties_and_masks(scoring, bias):
+    g = torch.Generator().manual_seed(3)
+    s = torch.randint(-2, 3, (2200, 128), generator=g).float()
+    s[500:1500][torch.rand(1000, 128, generator=g) < 0.5] = -float("inf")
+    s[700], s[701, 3:], s[702, :64], s[703, 1:] = -float("inf"), -float("inf"), -float("inf"), torch.finfo(torch.float32).min
+    b = None if bias is None else torch.randint(0, 3, (128,), generator=g) * 0.25
+    grad = torch.randn(2200, 9, generator=g)
+    for groups, top_groups, best in ((1, 1, 1), (8, 3, 1), (8, 3, 2)):
+        _check(s, b, 9, groups, top_groups, best, scoring, True, 1.0, grad, (groups, best))
+    s[::7, 17] = float("nan")
+    got, weights = stk.ops.group_top_experts(s.to(DEV), 9, 8, 3, scoring, None if b is None else b.to(DEV))
+    assert all(len(set(row)) == 9 and 0 <= min(row) and max(row) < 128 for row in got[::7].cpu().tolist()) and weights[::7].isnan().any(1).any()
