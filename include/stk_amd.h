@@ -750,8 +750,8 @@ int stk_quantize_rows_8bit(const void* x, int64_t rows, int64_t size, int64_t st
  * way as above, a scale for every row and 128 inputs.  What is written, `activation`, indices, bins, top_k and weights as for the 4-bit products; out
  * is of x's type.  Sums are fp32 from the matrix units, which add the (exact) products of a block of 128 with 13 bits below the largest of them.
  * A row with an infinity or a NaN gives NaN throughout its result (in the scatter: in its token's).  Weights of experts without rows are not read.
- * workspace: as many bytes as the functions say (0: may be NULL), 16-byte aligned, nothing in it is read before it is written; x_rows: rows of x, rows:
- * those multiplied (with routing tokens * top_k).
+ * workspace: as many bytes as the functions say (0: may be NULL), 16-byte aligned, nothing in it is read before it is written; x_rows: rows of x (they
+ * do not count at present), rows: those multiplied (with routing tokens * top_k).
  */
 size_t stk_matmul_8bit_workspace_bytes(int64_t x_rows, int64_t rows, int64_t experts, int64_t inputs, int64_t outputs);
 int stk_matmul_8bit(const void* x, int64_t rows, int64_t x_stride, const void* packed, const void* scales, int float_scales, int64_t inputs,
@@ -774,7 +774,7 @@ int stk_8bit_product_kernel(int64_t rows, int64_t experts, int64_t inputs, int64
  *   stk_linear_8bit           out[r] = rows[r] w[expert of r], zeros in rows behind the last bin; with the gradient's rows and packed_t: dx
  *   stk_weight_gradient_8bit  dw[e][i][o] = sum over the rows of e of x[r][i] g[r][o]; columns, exponents: x's as rows of [inputs, rows], grad_pieces: g's
  *                             as pieces; zeros for an expert without rows.  rows at least 1.
- * Sums as above; results are 16-bit (dtype), rounded once.
+ * Sums as above; results are 16-bit (dtype), rounded once.  At most 8388608 inputs, or rows that a gradient adds up.
  */
 int stk_linear_8bit(const void* codes, const void* exponents, int64_t rows, const int32_t* bins, const void* packed, const void* weight_exponents,
                     int64_t experts, int64_t inputs, int64_t outputs, void* out, int64_t out_stride, int dtype, stk_stream_t stream);

@@ -73,13 +73,15 @@ def test_refusals_of_the_c_abi():
         (dims, lambda l: l.stk_matmul_8bit(at, 4, 128, at, at, 0, 128, 128, at, 127, 0, bf16, None, 0, None)),
         (dims, lambda l: l.stk_matmul_8bit(at, -4, 128, at, at, 0, 128, 128, at, 128, 0, bf16, None, 0, None)),
         (dims, lambda l: l.stk_matmul_8bit(at, 4, 128, None, at, 0, 128, 128, at, 128, 0, bf16, None, 0, None)),
-        (workspace, lambda l: l.stk_matmul_8bit(at, 400, 128, at, at, 0, 128, 128, at, 128, 0, bf16, None, 0, None)),
-        (workspace, lambda l: l.stk_matmul_8bit(at, 400, 128, at, at, 0, 128, 128, at, 128, 0, bf16, odd, 1 << 30, None)),
+        (workspace, lambda l: l.stk_matmul_8bit(at, 400000, 128, at, at, 0, 128, 128, at, 128, 0, bf16, None, 0, None)),
+        (workspace, lambda l: l.stk_matmul_8bit(at, 400000, 128, at, at, 0, 128, 128, at, 128, 0, bf16, odd, 1 << 30, None)),
         (dims, lambda l: l.stk_gather_matmul_8bit(at, 4, 128, None, at, 1, at, at, 0, 2, 128, 128, at, 128, 0, bf16, None, 0, None)),
         (dims, lambda l: l.stk_gather_matmul_8bit(at, huge, 128, at, at, 2, at, at, 0, 2, 128, 128, at, 128, 0, bf16, None, 0, None)),
         (workspace, lambda l: l.stk_matmul_8bit_scatter(at, 128, at, at, 2, 4, None, at, at, 0, 2, 128, 128, at, 128, bf16, None, 0, None)),
         (dims, lambda l: l.stk_linear_8bit(at, at, 128, None, at, at, 2, 128, 128, at, 128, bf16, None)),
         (dims, lambda l: l.stk_linear_8bit(at, None, 128, None, at, at, 1, 128, 128, at, 128, bf16, None)),
+        (unsupported, lambda l: l.stk_linear_8bit(at, at, 128, None, at, at, 1, 2 ** 23 + 1, 128, at, 128, bf16, None)),
+        (unsupported, lambda l: l.stk_weight_gradient_8bit(at, at, at, at, 2 ** 23 + 1, None, 1, 128, 128, at, bf16, None)),
         (dims, lambda l: l.stk_weight_gradient_8bit(at, at, at, at, 0, None, 1, 128, 128, at, bf16, None)),
         (dims, lambda l: l.stk_weight_gradient_8bit(at, at, at, at, 128, None, 2, 128, 128, at, bf16, None)),
         (dims, lambda l: l.stk_group_top_experts(at, 4, 30, 30, 4, 2, 1, 2, 0, None, 0, 1.0, at, at, f32, None)),

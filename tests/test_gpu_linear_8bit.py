@@ -189,3 +189,32 @@ def test_refusals():
     dx, = torch.autograd.grad(stk.ops.linear_8bit(xs, w).sum(), xs, create_graph=True)
     with pytest.raises(RuntimeError):
         dx.sum().backward()
+
+
+@pytest.mark.parametrize("tokens,experts,hidden,ffn", [(300, 8, 96, 200), (6000, 16, 1032, 1544)])
+def test_a_routed_layer(tokens, experts, hidden, ffn):
+    """A router's choice among groups, the padded layout, both products and the way back, trained, against the same layer with every expert's products by
+    themselves: blocks are the same, so that results and gradients differ by what sums in another order differ, 2^-8 of the largest."""
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(tokens, hidden, generator=g).bfloat16().to(DEV)
+    scores, bias = torch.randn(tokens, experts, generator=g).to(DEV), (torch.randn(experts, generator=g) * 0.1).to(DEV)
+    w1 = (torch.randn(experts, hidden, ffn, generator=g) * hidden ** -0.5).bfloat16().to(DEV)
+    w2 = (torch.randn(experts, ffn, hidden, generator=g) * ffn ** -0.5).bfloat16().to(DEV)
+    grad = torch.randn(tokens, hidden, generator=g).bfloat16().to(DEV)
+
+    def layer(product):
+        leaves = [t.detach().clone().requires_grad_() for t in (x, scores, w1, w2)]
+        a, s, u, v = leaves
+        chosen, weights = stk.ops.group_top_experts(s, 2, groups=4, top_groups=2, bias=bias)
+        r = stk.ops.route(chosen, experts, 128)
+        h = torch.relu(product(stk.ops.padded_gather(a, r), u, r))
+        out = stk.ops.padded_scatter(product(h, v, r), r, weights)
+        return (out.detach(), *torch.autograd.grad(out, leaves, grad))
+
+    def apart(rows, w, r):
+        ends = [0] + r.padded_bins.tolist()
+        parts = [stk.ops.linear_8bit(rows[ends[e]:ends[e + 1]], w[e]) for e in range(experts)]
+        return torch.cat(parts + [rows.new_zeros(rows.size(0) - ends[-1], w.size(2))])
+
+    for got, want in zip(layer(stk.ops.linear_8bit), layer(apart)):
+        assert (got.double() - want.double()).abs().max() <= 2.0 ** -8 * want.double().abs().max()
