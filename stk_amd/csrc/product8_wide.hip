@@ -147,8 +147,8 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
       scalars_read8();
     }
   };
-  constexpr int kColsOf = 8, kExponentsOf = 2, kUpperOf = 4, kLowerOf = 4;   // transfers of a wavefront, in this order
-  constexpr int kAllOf = kColsOf + kExponentsOf + kUpperOf + kLowerOf;
+  // Transfers of a wavefront: weights, exponents and upper rows of a block during a step, its lower rows at the start of the next.
+  constexpr int kColsOf = 8, kExponentsOf = 2, kUpperOf = 4, kLowerOf = 4, kFirstOf = kColsOf + kExponentsOf + kUpperOf;
   constexpr uint32_t kOutRange = 1u << 31;
 
   // ------------------------------------------------------------ one step
@@ -180,37 +180,37 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
       else col_scale[i] = (from + kWideTile + 128 * wn)[16 * i];
     }
   };
-  int stored = 2, stores = 0;   // steps since the last sums were stored, up to 2, and by at least how many instructions (0, 16 or 32)
+  int stores = 0;   // by at least how many instructions the sums were stored in front of a step (0, 16 or 32)
   const auto step = [&](int block) {
-    const uint32_t to_rows = lds + stage * kWideSide + wave * 1024, to_cols = to_rows + 2 * kWideSide, to_exponents = lds + kExponentsAt + stage * kWideExponents + wave * 256;
-    const uint32_t start = next_block * kBlock8, start_cols = next_block * (4 * kPieceBytes8);
-    const uint32_t start_row_exponents = (next_block >> 2) * row_lines, start_col_exponents = (next_block >> 2) * col_lines;
     int by_row[8], by_col[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) by_row[i] = row_scale[i] >> (8 * (block & 3)), by_col[i] = col_scale[i] >> (8 * (block & 3));
     settle8();
+    uint32_t to_rows = lds + (stage ^ 1) * kWideSide + wave * 1024, start = next_block * kBlock8;   // of the next step's lower rows
+    uint32_t to_cols = 0, to_exponents = 0, start_cols = 0, start_row_exponents = 0, start_col_exponents = 0;
     static_for<4>([&](auto pair) {
       constexpr int P = decltype(pair)::value;
       // 1: everybody has read the upper rows and, in the step before, the weights and exponents; the lower rows are there.
-      // 3: everybody has read the lower rows; the next weights, exponents and upper rows are there.  Younger than these are as many transfers each time.
-      // The stores of a tile are younger than the transfers of the next two steps, but for the second step's last wait, and need not have ended.
+      // 3: everybody has read the lower rows; the next weights, exponents and upper rows are there.
+      // Younger than these are as many transfers each time, and in the first step of a tile the stores of the last one, which need not have ended.
       if constexpr (P == 1 || P == 3) {
-        const int young = stored < (P == 1 ? 2 : 1) ? stores : 0;
-        if (young == 32) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kAllOf + 32) : "memory");
-        else if (young == 16) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kAllOf + 16) : "memory");
-        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kAllOf) : "memory");
+        constexpr int kYounger = P == 1 ? kFirstOf + kLowerOf : kLowerOf + kColsOf + kExponentsOf;
+        if (stores == 32) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kYounger + 32) : "memory");
+        else if (stores == 16) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kYounger + 16) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kYounger) : "memory");
       }
       static_for<8>([&](auto at) {
         constexpr int N = decltype(at)::value, M = 2 * P;
         const i32x8_t &upper = values[2 * (P & 1)], &lower = values[2 * (P & 1) + 1];
-        if constexpr (P == 1) accumulate8_fetch<4096 * N, 16>(total[M][N], weights[N], upper, by_col[N], by_row[M], col_buffer, col_offset[N], start_cols, to_cols);
-        else if constexpr (P == 2 && N < 2)
-          accumulate8_fetch<N * kWideTile * 4, 4>(total[M][N], weights[N], upper, by_col[N], by_row[M], N ? col_exponent_buffer : row_exponent_buffer,
-                                                  N ? col_exponents : row_exponents, N ? start_col_exponents : start_row_exponents, to_exponents);
-        else if constexpr (P == 2 && N >= 4)
-          accumulate8_fetch<4096 * (N - 4), 16>(total[M][N], weights[N], upper, by_col[N], by_row[M], row_buffer, row_offset[N - 4], start, to_rows);
-        else if constexpr (P == 3 && N >= 4)
-          accumulate8_fetch<4096 * N, 16>(total[M][N], weights[N], upper, by_col[N], by_row[M], row_buffer, row_offset[N], start, to_rows);
+        // (as many transfers to each pair of fragments as the next has: more at a time wait for each other)
+        constexpr int kCol = P == 1 && N < 5 ? N : P == 2 && N < 3 ? 5 + N : -1, kRow = P == 3 && N >= 4 ? N - 4 : P == 0 && N >= 4 ? N : -1;
+        if constexpr (kCol >= 0)
+          accumulate8_fetch<4096 * kCol, 16>(total[M][N], weights[N], upper, by_col[N], by_row[M], col_buffer, col_offset[kCol], start_cols, to_cols);
+        else if constexpr (kRow >= 0)
+          accumulate8_fetch<4096 * kRow, 16>(total[M][N], weights[N], upper, by_col[N], by_row[M], row_buffer, row_offset[kRow], start, to_rows);
+        else if constexpr (P == 2 && (N == 4 || N == 6))
+          accumulate8_fetch<N / 6 * kWideTile * 4, 4>(total[M][N], weights[N], upper, by_col[N], by_row[M], N == 6 ? col_exponent_buffer : row_exponent_buffer,
+                                                      N == 6 ? col_exponents : row_exponents, N == 6 ? start_col_exponents : start_row_exponents, to_exponents);
         else accumulate8(total[M][N], weights[N], upper, by_col[N], by_row[M]);
         if constexpr (N < 2) values[2 * (~P & 1) + N] = P < 3 ? row_fragment(stage, M + 2 + N) : row_fragment(stage ^ 1, N);
         accumulate8(total[M + 1][N], weights[N], lower, by_col[N], by_row[M + 1]);
@@ -220,10 +220,14 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
         }
         __builtin_amdgcn_sched_barrier(0);
       });
+      if constexpr (P == 0) {
+        fetched();
+        to_rows = lds + stage * kWideSide + wave * 1024, to_cols = to_rows + 2 * kWideSide, to_exponents = lds + kExponentsAt + stage * kWideExponents + wave * 256;
+        start = next_block * kBlock8, start_cols = next_block * (4 * kPieceBytes8);
+        start_row_exponents = (next_block >> 2) * row_lines, start_col_exponents = (next_block >> 2) * col_lines;
+      }
     });
-    stage ^= 1;
-    stored = min(stored + 1, 2);
-    fetched();
+    stage ^= 1, stores = 0;
   };
 
   aim(mine);
@@ -234,10 +238,13 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
     fetch8<4>(row_exponent_buffer, row_exponents, (next_block >> 2) * row_lines, to_exponents);
     fetch8<4>(col_exponent_buffer, col_exponents, (next_block >> 2) * col_lines, to_exponents + kWideTile * 4);
 #pragma unroll
-    for (int j = 0; j < 8; j++) fetch8<16>(row_buffer, row_offset[j], next_block * kBlock8, to + 4096 * j);
+    for (int j = 0; j < 4; j++) fetch8<16>(row_buffer, row_offset[j], next_block * kBlock8, to + 4096 * j);
+    if (s == 1) break;   // (the lower rows of the second block: in the first step)
+#pragma unroll
+    for (int j = 4; j < 8; j++) fetch8<16>(row_buffer, row_offset[j], next_block * kBlock8, to + 4096 * j);
     fetched();
   }
-  wait_vmcnt<kLowerOf + kAllOf>();
+  wait_vmcnt<kLowerOf + kFirstOf>();
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < 8; n++) weights[n] = col_fragment(0, n);
@@ -289,7 +296,7 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
         if (place_of_row8(to_where, w.t, r, to, by)) store_pieces8(to_where, to, by, first, quarter, sums[0]), store_pieces8(to_where, to, by, first + 64, quarter, sums[1]);
       }
     }
-    stored = 0, stores = !whole ? 0 : w.t.rows > 16 * (14 + wm) ? 32 : w.t.rows > 16 * (6 + wm) ? 16 : 0;   // (four for every 16 rows)
+    stores = !whole ? 0 : w.t.rows > 16 * (14 + wm) ? 32 : w.t.rows > 16 * (6 + wm) ? 16 : 0;   // (four for every 16 rows)
   }
   wait_vmcnt<0>();
   // rows behind the last expert's
