@@ -284,7 +284,7 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const typename Valu
   }
   if (r.top_groups < r.groups) {
 #pragma unroll
-    for (int j = 0; j < V; j++) key[j] = kept >> ((lane + LANES * j) * r.group_magic >> 22) & 1ull ? key[j] : 0u;
+    for (int j = 0; j < V; j++) key[j] = kept >> (((lane + LANES * j) * r.group_magic >> 22) & 63u) & 1ull ? key[j] : 0u;   // (behind the last expert it is 0 already)
   }
   at = 0;
   uint32_t mark = 0;   // the last of this lane's keys that was chosen

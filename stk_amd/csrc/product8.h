@@ -168,7 +168,7 @@ __device__ __forceinline__ u32x4 buffer8(const uint8_t* from) {
   return u32x4{(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
 }
 template <int BYTES>
-__device__ __forceinline__ void fetch8(u32x4 buffer, uint32_t offset, uint32_t start, uint32_t to) {
+__device__ __forceinline__ void transfer8(u32x4 buffer, uint32_t offset, uint32_t start, uint32_t to) {
   if constexpr (BYTES == 16) asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %0, %2 offen lds" : : "s"(buffer), "v"(offset), "s"(start), "s"(to) : "memory", "m0");
   else asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dword %1, %0, %2 offen lds" : : "s"(buffer), "v"(offset), "s"(start), "s"(to) : "memory", "m0");
 }

@@ -60,7 +60,10 @@ __device__ __forceinline__ u32x4 row_values8(const uint16_t* row, int i, int inp
 }
 
 // Few rows: KW wavefronts share the inputs of NW x NT pieces and up to 16 rows of one expert, a block at a time; their sums meet in LDS.
-// Codes go from memory into registers as the matrix instruction takes them; the rows are quantised on the way.
+// Codes go from memory into registers as the matrix instruction takes them; the rows are quantised on the way, some 75 instructions for 16 x 128 of them.
+// Bound by the bytes of the weights where there are many: 64 rows to the top 2 of 64 experts of 1024 x 4096 (233 MB) 42 us, 5.5 TB/s; by a launch and one trip to
+// memory where there are few: 1 row of 4096 x 4096 6 us.  More rows of a tile in one wavefront (32, 64) were slower than tiles of 16 that read the
+// weights from the caches again.
 template <int NT>
 struct Stage8 {
   u32x4 w[NT][2], v[4];
@@ -166,6 +169,9 @@ __global__ __launch_bounds__(64 * KW * NW) void stream8_kernel(Product8 p) {
 // ------------------------------------------------------------------------------------------------ many rows
 // WM x WN wavefronts share 16 MT WM rows and 64 WN outputs, a block of 128 inputs at a time in stages of LDS that are filled without
 // registers: pieces of weights as they lie in memory, rows by whole lines, exponents of four blocks in a dword.
+// With fp32 scales every matrix instruction is followed by four additions to sums that lie in vector registers: 8192 x 4096 x 4096 in tiles of 256 x 256
+// 144 us, 1.9 PFLOP/s, matrix units busy 37 % of the time, three waves of four waiting at a barrier or for LDS.  Smaller tiles are for problems that do not
+// fill the chip; a step of theirs takes 0.5 - 1 us whatever the depth of the stages (two, three and four were the same but for the smallest tile).
 template <int WM, int WN, int MT, int STAGES>
 struct Tile8 {
   static constexpr int kWaves = WM * WN, kRows = 16 * MT * WM, kCols = 64 * WN;
@@ -241,7 +247,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
   const auto issue = [&](int block, int stage) {
     const uint32_t to = lds + stage * T::kStage;
 #pragma unroll
-    for (int j = 0; j < kRowMoves; j++) fetch8<16>(row_buffer, row_offset[j], block * kBlock8, to + (wave + T::kWaves * j) * 1024);
+    for (int j = 0; j < kRowMoves; j++) transfer8<16>(row_buffer, row_offset[j], block * kBlock8, to + (wave + T::kWaves * j) * 1024);
 #pragma unroll
     for (int j = 0; j < kColMoves; j++) dma16(col_from[j] + (int64_t)block * (4 * kPieceBytes8), lane * 16, to + T::kRowBytes + (wave + T::kWaves * j) * 1024);
 #pragma unroll

@@ -10,6 +10,12 @@
 //
 // Workgroups stay: each takes tile after tile, and the transfers of the next tile's first blocks run during the last steps of one and while its sums
 // are stored.
+//
+// Measured (MI355X): the gradient of 4096 x 4096 weights from 16384 rows 217 - 237 us on different machines, 2.3 - 2.5 PFLOP/s, where the library's product without
+// block scales takes 230; the matrix units are busy for 59 % of the clocks, which fall to 2.1 GHz under them (alone, out of registers, they reach
+// 3.5 PFLOP/s at 1.7).  With the transfers cut off a step takes two thirds of that: what bounds it is their way through the caches into LDS, 66 KiB
+// a step and unit, 9 TB/s.  The product of the same sizes, four tiles for each workgroup, takes 243 - 270 us: all of them store at the same time.  With
+// eight blocks of inputs (64 experts of 1024 x 4096, 256 rows each) storing and applying gelu takes a third of 175 us.
 #include <type_traits>
 
 #include "common.h"
@@ -234,14 +240,14 @@ __global__ __launch_bounds__(256, 1) void wide8_kernel(Product8 p, int row_tiles
   for (int s = 0; s < 2; s++) {
     const uint32_t to = lds + s * kWideSide + wave * 1024, to_exponents = lds + kExponentsAt + s * kWideExponents + wave * 256;
 #pragma unroll
-    for (int j = 0; j < 8; j++) fetch8<16>(col_buffer, col_offset[j], next_block * (4 * kPieceBytes8), to + 2 * kWideSide + 4096 * j);
-    fetch8<4>(row_exponent_buffer, row_exponents, (next_block >> 2) * row_lines, to_exponents);
-    fetch8<4>(col_exponent_buffer, col_exponents, (next_block >> 2) * col_lines, to_exponents + kWideTile * 4);
+    for (int j = 0; j < 8; j++) transfer8<16>(col_buffer, col_offset[j], next_block * (4 * kPieceBytes8), to + 2 * kWideSide + 4096 * j);
+    transfer8<4>(row_exponent_buffer, row_exponents, (next_block >> 2) * row_lines, to_exponents);
+    transfer8<4>(col_exponent_buffer, col_exponents, (next_block >> 2) * col_lines, to_exponents + kWideTile * 4);
 #pragma unroll
-    for (int j = 0; j < 4; j++) fetch8<16>(row_buffer, row_offset[j], next_block * kBlock8, to + 4096 * j);
+    for (int j = 0; j < 4; j++) transfer8<16>(row_buffer, row_offset[j], next_block * kBlock8, to + 4096 * j);
     if (s == 1) break;   // (the lower rows of the second block: in the first step)
 #pragma unroll
-    for (int j = 4; j < 8; j++) fetch8<16>(row_buffer, row_offset[j], next_block * kBlock8, to + 4096 * j);
+    for (int j = 4; j < 8; j++) transfer8<16>(row_buffer, row_offset[j], next_block * kBlock8, to + 4096 * j);
     fetched();
   }
   wait_vmcnt<kLowerOf + kFirstOf>();
