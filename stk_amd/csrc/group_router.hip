@@ -191,13 +191,14 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const typename Valu
         else c[j] = share((F)mine[j]);
       }
     }
+    uint32_t most_p = 0, most_b = 0;   // as bits: of magnitudes, NaN and infinities are the largest
 #pragma unroll
     for (int j = 0; j < V; j++) {
-      if constexpr (kFast) largest_p = fmaxf(largest_p, c[j]), largest_b = fmaxf(largest_b, fabsf(bias[j])), strange |= !(fabsf(bias[j]) < INFINITY) || !(mine[j] < INFINITY);
+      if constexpr (kFast) most_p = max(most_p, __float_as_uint(c[j])), most_b = max(most_b, __float_as_uint(bias[j]) & 0x7fffffffu);
       const F sum = c[j] + (F)bias[j];
       c[j] = mine[j] == -INFINITY ? kNone : sum;
     }
-    if constexpr (kFast) strange |= !(largest_p < INFINITY);
+    if constexpr (kFast) strange = max(most_p, most_b) >= 0x7f800000u, largest_p = __uint_as_float(most_p), largest_b = __uint_as_float(most_b);
   }
   if (r.top_groups < r.groups) {
 #pragma unroll
@@ -284,7 +285,11 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const typename Valu
   }
   if (r.top_groups < r.groups) {
 #pragma unroll
-    for (int j = 0; j < V; j++) key[j] = kept >> (((lane + LANES * j) * r.group_magic >> 22) & 63u) & 1ull ? key[j] : 0u;   // (behind the last expert it is 0 already)
+    for (int j = 0; j < V; j++) {   // (behind the last expert it is 0 already)
+      const uint32_t g = (lane + LANES * j) * r.group_magic >> 22;
+      if constexpr (kFast && LANES == 16) key[j] &= (uint32_t)__builtin_amdgcn_sbfe((int)kept, g, 1);   // (at most 16 groups)
+      else key[j] = kept >> (g & 63u) & 1ull ? key[j] : 0u;
+    }
   }
   at = 0;
   uint32_t mark = 0;   // the last of this lane's keys that was chosen
@@ -303,12 +308,13 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const typename Valu
     } else {
 #pragma unroll
       for (int j = 0; j < V; j++) best = max(best, key[j]);
-      // of equal ones the lowest expert: the lowest place, then the lowest lane
-      const key_t all = reduce_team<LANES>(best, [](key_t a, key_t b) { return a > b ? a : b; });
+      // the largest by halves of 32 bits; of equal ones the lowest expert: the lowest place, then the lowest lane
+      const uint32_t high = largest_key<LANES>((uint32_t)(best >> 32)), low = largest_key<LANES>((uint32_t)(best >> 32) == high ? (uint32_t)best : 0u);
+      const key_t all = (key_t)high << 32 | low;
       int first = V;
 #pragma unroll
       for (int j = V - 1; j >= 0; j--) first = key[j] == all ? j : first;
-      place = reduce_team<LANES>(first, [](int a, int b) { return a < b ? a : b; });
+      place = 16 - (int)largest_key<LANES>(first < V ? 16u - first : 0u);
       who = __builtin_ctzll(ballot_of_team<LANES>(first == place));
 #pragma unroll
       for (int j = 0; j < V; j++) key[j] = lane == who && j == place ? 0u : key[j];
@@ -325,10 +331,11 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const typename Valu
     if (any_of_team<LANES>(lane < r.top_k - 1 && too_close(c_at, next_c) && !(s_at == next_s && b_at == next_b))) return false;
     // the last of them and those that are not chosen (whose keys tell c to 2^-19 of it)
     const float c_last = from_lane<LANES>(c_at, r.top_k - 1);
-    bool close = false;
+    uint32_t rest = 0;   // the lane's largest that is not chosen
 #pragma unroll
-    for (int j = 0; j < V; j++) close |= key[j] - 1u < mark - 1u && too_close(number_of(key[j] & ~15u), c_last);
-    if (any_of_team<LANES>(close)) {   // of equal inputs?
+    for (int j = 0; j < V; j++) rest = max(rest, key[j] - mark);
+    rest += mark;
+    if (any_of_team<LANES>(rest - 1u < mark - 1u && too_close(number_of(rest & ~15u), c_last))) {   // of equal inputs?
       const float s_last = from_lane<LANES>(s_at, r.top_k - 1), b_last = from_lane<LANES>(b_at, r.top_k - 1);
       bool wrong = false;
 #pragma unroll
@@ -454,8 +461,8 @@ __global__ __launch_bounds__(256) void group_top_experts_backward_kernel(GroupRo
 }
 
 // Teams of 16 lanes have a lane for every choice, and for every group, where these are few.  Where there are few tokens a wavefront each is sooner done:
-// the top 8 of 256 in groups for 2048 tokens 12.5 us, with teams 14.1; for 16384 teams 22.8 (16.8 MB of scores are 3.4 us: bound by what the choice
-// executes, some 700 instructions a wavefront, and by the tokens that are done again).
+// the top 8 of 256 in groups for 2048 tokens 12.1 us, with teams 13.1; for 16384 teams 21 (16.8 MB of scores are 3.4 us: bound by what the choice
+// executes, some 1500 instructions for a wavefront's four tokens, and by the tokens that are done again, 7 us where a workgroup has one).
 template <class Fn>
 static void for_team(const GroupRouter& r, Fn&& fn) {
   typedef std::integral_constant<int, 16> Sixteen;
@@ -463,6 +470,7 @@ static void for_team(const GroupRouter& r, Fn&& fn) {
   if (r.top_k <= 16 && r.groups <= 16 && r.experts <= 256 && r.tokens > kFewTokens) {
     if (r.experts <= 64) fn(Sixteen(), std::integral_constant<int, 4>());
     else if (r.experts <= 128) fn(Sixteen(), std::integral_constant<int, 8>());
+    else if (r.experts <= 192) fn(Sixteen(), std::integral_constant<int, 12>());
     else fn(Sixteen(), std::integral_constant<int, 16>());
   } else if (r.experts <= 256) fn(Wave(), std::integral_constant<int, 4>());
   else if (r.experts <= 512) fn(Wave(), std::integral_constant<int, 8>());
