@@ -179,7 +179,7 @@ struct Tile8 {
   static constexpr int kBytes = STAGES * kStage;
 };
 template <int KIND, int WHAT, int WM, int WN, int MT, int STAGES>
-__global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row_tiles, int col_tiles) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void tile8_kernel(Product8 p, int row_tiles, int col_tiles) {
   typedef Tile8<WM, WN, MT, STAGES> T;
   extern __shared__ char smem[];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
@@ -264,8 +264,6 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
   for (int m = 0; m < MT; m++)
 #pragma unroll
     for (int n = 0; n < 4; n++) total[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  // this wavefront's rows are fragments wm, wm + WM, ... of 16, of which so many have any
-  const int fragments = ((t.rows + 15) / 16 - wm + WM - 1) / WM;
   const int count = end - begin;
 #pragma unroll
   for (int s = 0; s < STAGES - 1; s++)
@@ -297,15 +295,14 @@ __global__ __launch_bounds__(64 * WM * WN) void tile8_kernel(Product8 p, int row
       return f;
     };
     const auto row_fragment = [&](int m) { return fragment(rows + in_fragment + m * WM * kPieceBytes8, rows + (in_fragment ^ 64) + m * WM * kPieceBytes8); };
-    // The fragment of the next 16 rows is on its way while one is multiplied; with fp32 scales the sums of one are scaled while the next is.  What lies
-    // behind the last row of a tile is left out.
+    // The fragment of the next 16 rows is on its way while one is multiplied; with fp32 scales the sums of one are scaled while the next is.  (Leaving out what
+    // lies behind the last row of a tile would need branches, around which the sums move between registers: twice the instructions.)
     i32x8_t w[4], values[2];
     values[0] = row_fragment(0);
 #pragma unroll
     for (int n = 0; n < 4; n++) w[n] = fragment(cols + n * kPieceBytes8, cols + n * kPieceBytes8 + 1024);
 #pragma unroll
     for (int m = 0; m < MT; m++) {
-      if (m >= fragments) break;
       if (m + 1 < MT) values[(m + 1) & 1] = row_fragment(m + 1);
       f32x4_t part[4];
 #pragma unroll
@@ -415,14 +412,14 @@ static ProductKernel8 product_kernel8(int64_t rows, int64_t experts, int64_t inp
   const int64_t along = blocks8(inputs), down = padded_lines8(outputs) / kPieceLines8;
   // as if the rows were spread evenly over the experts: where they really are only the device knows
   const int64_t hit = experts < rows ? experts : rows, each = (rows + hit - 1) / hit;
-  // Streams read an expert's weights once for every 16 rows, behind the first time from the caches, at some 8 TB/s; tiles take a launch that quantises the
-  // rows, and a step of 0.6 us for every block where few of them are in the chip.  4096 x 4096, streams and the best tiles: 20 rows 9.5 and 23.4 us, 64
-  // rows 11.6 and 25.2, 128 rows 18.7 and 25.3; 1024 x 4096, 64 rows 5.8 and 10.0; 37 rows of 2944 x 1151 6.1 and 20.0; 8 experts of 1024 x 1024, 40
-  // rows each 8.3 and 11.5; 64 experts of 1024 x 4096, 20 rows each 77 and 68, 40 rows each 113 and 83.
+  // Streams read an expert's weights once for every 16 rows, behind the first time from the caches, and quantise the rows for every piece; tiles take a launch
+  // that quantises the rows, and 0.4 us for every block where few of them are in the chip.  Rows that are no whole 16-byte pieces cost the streams twice.
+  // Streams and the best tiles: 4096 x 4096, 64 rows (1024 units) 11.4 and 18.5 us, 128 rows 18.9 and 18.7, 256 rows 35 and 20.7; 8 experts of 1024 x 1024, 40 rows each
+  // (1536) 8.4 and 10.0; 100 rows of 1151 x 2944 (1288) 13.7 and 9.4; 64 experts of 1024 x 4096, 20 rows each 81 and 66.
   const int64_t tiles = hit * ((each + 15) / 16) * down;
-  if (each > 16 && tiles > 2048 + 8192 / along && inputs <= kMostTileInputs8) {
-    // Larger tiles read less, smaller ones fill the chip.  4096 x 4096, tiles of 32, 64, 128, 256 rows: 256 rows 22, 28, 38, 57 us; 1024 rows 52, 35, 42, 60;
-    // 2048 rows 90, 65, 53, 65; 64 experts of 1024 x 4096, 20 rows each 76, 68, 73, 87, 64 rows each 109, 98, 101, 93, 128 rows each 165, 129, 141, 109.
+  if (each > 16 && tiles > (inputs % 8 ? 896 : 1792) && inputs <= kMostTileInputs8) {
+    // Larger tiles read less, smaller ones fill the chip.  4096 x 4096, tiles of 32, 64, 128, 256 rows: 256 rows 21, 24, 29, 55 us; 1024 rows 44, 30, 34, 59;
+    // 2048 rows 78, 57, 43, 62; 64 experts of 1024 x 4096, 20 rows each 72, 67, 72, 83, 64 rows each 105, 95, 97, 92, 128 rows each 162, 128, 131, 108.
     const auto count = [&](int64_t high, int64_t wide) { return hit * ((each + high - 1) / high) * ((outputs + wide - 1) / wide); };
     if (each > 64 && count(256, 256) >= 192) return kTile8_256;
     if (each > 64 && count(128, 128) > 256) return kTile8_128;
