@@ -47,16 +47,27 @@ __device__ __forceinline__ i32x8_t quantise_fragment(const u32x4 (&raw)[4], int&
   return out;
 }
 
-// Eight values of a row from input i on, zeros beyond the last input.
+// Eight values of a row from input i on, zeros beyond the last input: the eight that end with the row, moved down.  (No branch stands between loads, which
+// would wait for each of them.)
 __device__ __forceinline__ u32x4 row_values8(const uint16_t* row, int i, int inputs) {
-  if (i + 8 <= inputs) return __builtin_bit_cast(u32x4, *reinterpret_cast<const QuadAt2*>(row + i));
-  u32x4 v = {0u, 0u, 0u, 0u};
+  u32x4 v;
+  int down;
+  if (inputs >= 8) {
+    const int from = min(i, inputs - 8);
+    v = __builtin_bit_cast(u32x4, *reinterpret_cast<const QuadAt2*>(row + from));
+    down = i - from;
+  } else {
+    uint32_t one[8];
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const uint32_t one = i + j < inputs ? row[i + j] : 0u;
-    v[j / 2] |= one << (16 * (j & 1));
+    for (int j = 0; j < 8; j++) one[j] = row[min(j, inputs - 1)];
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = (2 * j < inputs ? one[2 * j] : 0u) | (2 * j + 1 < inputs ? one[2 * j + 1] << 16 : 0u);
+    down = i;
   }
-  return v;
+  if (down & 1) v = u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+  if (down & 2) v = u32x4{v[1], v[2], v[3], 0u};
+  if (down & 4) v = u32x4{v[2], v[3], 0u, 0u};
+  return down >= 8 ? u32x4{0u, 0u, 0u, 0u} : v;
 }
 
 // Few rows: KW wavefronts share the inputs of NW x NT pieces and up to 16 rows of one expert, a block at a time; their sums meet in LDS.
@@ -70,7 +81,7 @@ struct Stage8 {
   int scale[NT];
 };
 template <bool BF16, int KIND, int KW, int NW, int NT>
-__global__ __launch_bounds__(64 * KW * NW) void stream8_kernel(Product8 p) {
+__global__ __launch_bounds__(64 * KW * NW, 2) void stream8_kernel(Product8 p) {
   __shared__ f32x4_t shared[KW > 1 ? (KW - 1) * NW * NT * 64 : 1];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), kw = wave / NW, nw = wave % NW;
   const RowTile8 t = row_tile8<16>(p, (int)(blockIdx.z * gridDim.y + blockIdx.y), lane);
@@ -415,9 +426,9 @@ static ProductKernel8 product_kernel8(int64_t rows, int64_t experts, int64_t inp
   // Streams read an expert's weights once for every 16 rows, behind the first time from the caches, and quantise the rows for every piece; tiles take a launch
   // that quantises the rows, and 0.4 us for every block where few of them are in the chip.  Rows that are no whole 16-byte pieces cost the streams twice.
   // Streams and the best tiles: 4096 x 4096, 64 rows (1024 units) 11.4 and 18.5 us, 128 rows 18.9 and 18.7, 256 rows 35 and 20.7; 8 experts of 1024 x 1024, 40 rows each
-  // (1536) 8.4 and 10.0; 100 rows of 1151 x 2944 (1288) 13.7 and 9.4; 64 experts of 1024 x 4096, 20 rows each 81 and 66.
+  // (1536) 8.4 and 10.0; 37, 64, 100 rows of 1151 x 2944 (552, 736, 1288) 9.1, 10.0, 13.3 and 9.1, 9.1, 9.3; 64 experts of 1024 x 4096, 20 rows each 81 and 66.
   const int64_t tiles = hit * ((each + 15) / 16) * down;
-  if (each > 16 && tiles > (inputs % 8 ? 896 : 1792) && inputs <= kMostTileInputs8) {
+  if (each > 16 && tiles > (inputs % 8 ? 640 : 1792) && inputs <= kMostTileInputs8) {
     // Larger tiles read less, smaller ones fill the chip.  4096 x 4096, tiles of 32, 64, 128, 256 rows: 256 rows 21, 24, 29, 55 us; 1024 rows 44, 30, 34, 59;
     // 2048 rows 78, 57, 43, 62; 64 experts of 1024 x 4096, 20 rows each 72, 67, 72, 83, 64 rows each 105, 95, 97, 92, 128 rows each 162, 128, 131, 108.
     const auto count = [&](int64_t high, int64_t wide) { return hit * ((each + high - 1) / high) * ((outputs + wide - 1) / wide); };
@@ -426,11 +437,12 @@ static ProductKernel8 product_kernel8(int64_t rows, int64_t experts, int64_t inp
     return count(64, 128) > 256 ? kTile8_64 : kTile8_32;
   }
   // The fewer tiles there are the more wavefronts share the inputs of one: 1 row of 4096 x 4096 (256 tiles) 6.2, 8.8, 10.8 us by 8, 4 and 4 for two and four
-  // pieces; 20 rows (512) 10.8, 9.5, 11.2; 64 rows (1024) 21.5, 14.1, 11.6.
+  // pieces; 20 rows (512) 10.8, 9.5, 11.2; 64 rows (1024) 21.9, 13.8, 11.2.  Where every unit has a workgroup of four wavefronts with four pieces each they share
+  // nothing: 64 rows to the top 2 of 64 experts of 4096 x 1024 (4096) 40.1 us and 43.4 with shared inputs.
   if (tiles <= 320) return kStream8_811;
   if (tiles <= 640) return kStream8_412;
-  if (along >= 24 || (along >= 8 && tiles <= 4096)) return kStream8_414;
-  return tiles <= 4096 ? kStream8_222 : kStream8_144;
+  if (tiles >= 4096) return kStream8_144;
+  return along >= 8 ? kStream8_414 : kStream8_222;
 }
 static int64_t workspace8(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs) {
   if (rows < 1 || product_kernel8(rows, experts, inputs, outputs) < kTile8_32) return 0;
