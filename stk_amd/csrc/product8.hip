@@ -181,8 +181,9 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void stream8_kernel(Product8 p) {
 // WM x WN wavefronts share 16 MT WM rows and 64 WN outputs, a block of 128 inputs at a time in stages of LDS that are filled without
 // registers: pieces of weights as they lie in memory, rows by whole lines, exponents of four blocks in a dword.
 // With fp32 scales every matrix instruction is followed by four additions to sums that lie in vector registers: 8192 x 4096 x 4096 in tiles of 256 x 256
-// 144 us, 1.9 PFLOP/s, matrix units busy 37 % of the time, three waves of four waiting at a barrier or for LDS.  Smaller tiles are for problems that do not
-// fill the chip; a step of theirs takes 0.5 - 1 us whatever the depth of the stages (two, three and four were the same but for the smallest tile).
+// 144 us, 1.9 PFLOP/s, matrix units busy 37 % of the time, wavefronts waiting at barriers, for LDS or for a transfer 42 % of it.  Smaller tiles are for problems
+// that do not fill the chip: a step of theirs takes 0.4 - 0.7 us, of which a third or less are matrix instructions.  Three stages were faster than two only for
+// tiles of 32 rows, which few units have (4096 x 4096, 256 rows 20.7 and 24.0 us).
 template <int WM, int WN, int MT, int STAGES>
 struct Tile8 {
   static constexpr int kWaves = WM * WN, kRows = 16 * MT * WM, kCols = 64 * WN;
