@@ -181,9 +181,10 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void stream8_kernel(Product8 p) {
 // WM x WN wavefronts share 16 MT WM rows and 64 WN outputs, a block of 128 inputs at a time in stages of LDS that are filled without
 // registers: pieces of weights as they lie in memory, rows by whole lines, exponents of four blocks in a dword.
 // With fp32 scales every matrix instruction is followed by four additions to sums that lie in vector registers: 8192 x 4096 x 4096 in tiles of 256 x 256
-// 144 us, 1.9 PFLOP/s, matrix units busy 37 % of the time, wavefronts waiting at barriers, for LDS or for a transfer 42 % of it.  Smaller tiles are for problems
-// that do not fill the chip: a step of theirs takes 0.4 - 0.7 us, of which a third or less are matrix instructions.  Three stages were faster than two only for
-// tiles of 32 rows, which few units have (4096 x 4096, 256 rows 20.7 and 24.0 us).
+// 144 us, 1.9 PFLOP/s, matrix units busy 39 % of the time, wavefronts waiting at barriers, for LDS or for a transfer 47 % of it.  Smaller tiles are for problems
+// that do not fill the chip.  By the depth of the inputs, with 4096 outputs, a block costs 0.40 us in 256 tiles of 32 rows, 0.68 in 512 of 64 and 1.0 in 512 of
+// 128; where there are few blocks (2501 rows, 1151 x 2944 and its gradients) the matrix units are busy 13 - 15 % of the time.  Three stages are for tiles of 32
+// rows, which few units have: 256 rows of 4096 x 4096, quantising included, 20.3 us, and 23.1 by two.
 template <int WM, int WN, int MT, int STAGES>
 struct Tile8 {
   static constexpr int kWaves = WM * WN, kRows = 16 * MT * WM, kCols = 64 * WN;
