@@ -115,6 +115,15 @@ __device__ __forceinline__ float exponential_of(float x) {
   return t < -149.f ? 0.f : fmaf(y, rest * kLn2, y);
 }
 __device__ __forceinline__ double exponential_of(double x) { return exp(x); }
+// exp(a - b), a - b <= 0, in the range of 64 bits: what a - b rounds away and what the exponent of fp32 has no room for are kept.
+__device__ __forceinline__ double exponential_of_difference(float a, float b) {
+#pragma clang fp contract(off)   // (t - whole is to be that of the rounded t)
+  constexpr float kLog2e = 1.44269504088896341f, kLog2eRest = 1.92596299112661746887e-8f, kLn2 = 0.693147180559945309f;
+  const float x = a - b, was = x - a, lost = (a - (x - was)) - (b + was);
+  const float t = x * kLog2e, rest = fmaf(lost, kLog2e, fmaf(x, kLog2eRest, fmaf(x, kLog2e, -t))), whole = rintf(t), y = __builtin_amdgcn_exp2f(t - whole);
+  return t < -1080.f ? 0. : ldexp((double)fmaf(y, rest * kLn2, y), (int)whole);
+}
+__device__ __forceinline__ double exponential_of_difference(double a, double b) { return exp(a - b); }
 // 1 / (1 + exp(-s)) from the exponential of -|s|.
 template <class F>
 __device__ __forceinline__ F sigmoid_of(F s) {
@@ -143,10 +152,10 @@ __device__ __forceinline__ void put(Two<F>& t, F v) {
 }
 
 // One token in the precision of F.  from: its scores; mine: those of this lane's experts lane + LANES j.  row: LDS of the team for the c of every expert,
-// and the groups' values behind them.  at, p: the expert that lane k < top_k is to write and its p; sum: that of the chosen p.  false (F =
-// float only): two of the values that decide are too close for it.
+// and the groups' values behind them.  at, weight: what lane k < top_k is to write.  false (F = float only): two of the values that decide are too
+// close for it.
 template <class F, int DTYPE, int LANES, int V>
-__device__ __forceinline__ bool choose(const GroupRouter& r, const typename Value<DTYPE>::stored* from, const float (&mine)[V], const float (&bias)[V], F* row, int lane, int& at, F& p_at, F& sum) {
+__device__ __forceinline__ bool choose(const GroupRouter& r, const typename Value<DTYPE>::stored* from, const float (&mine)[V], const float (&bias)[V], F* row, int lane, int& at, float& weight) {
   constexpr bool kFast = std::is_same<F, float>::value;
   const F kNone = -INFINITY;
   F c[V];
@@ -164,10 +173,7 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const typename Valu
     for (int j = 0; j < V; j++) total += exponential_of((F)mine[j] - shift);
     total = reduce_team<LANES>(total, [](F a, F b) { return a + b; });
   }
-  const auto share = [&](F s) {   // p of a score
-    if (r.sigmoid) return sigmoid_of(s);
-    return top == kNone ? F(0) : exponential_of(s - top) / total;
-  };
+  const auto share = [&](F s) { return top == kNone ? F(0) : exponential_of(s - top) / total; };   // a softmax's p of a score
   // without a bias experts are in the order of the scores, in which sigmoids of 1 are told apart, and so are groups of which the best expert decides
   const bool by_score = r.bias == nullptr, groups_by_score = by_score && r.best == 1;
   if (groups_by_score) {
@@ -323,8 +329,10 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const typename Valu
   }
   const bool is = lane < r.top_k;
   const F s_at = is ? (F)Value<DTYPE>::widen(from[at]) : kNone;
+  F share_of_one = 1, t_at = 1;   // sigmoid: 1 / (1 + t), t = exp(-|s|)
+  if (r.sigmoid) t_at = exponential_of(s_at < 0 ? s_at : -s_at), share_of_one = F(1) / (F(1) + t_at);
   if constexpr (kFast) {
-    const float b_at = r.bias ? r.bias[at] : 0.f, c_at = by_score ? s_at : (s_at == kNone ? kNone : share(s_at) + b_at);
+    const float b_at = r.bias ? r.bias[at] : 0.f, c_at = by_score ? s_at : s_at == kNone ? kNone : (r.sigmoid ? (s_at < 0 ? t_at : 1.f) * share_of_one : share(s_at)) + b_at;
     // the order of the chosen
     const float next_c = __shfl_down(c_at, 1, LANES), next_s = __shfl_down(s_at, 1, LANES), next_b = __shfl_down(b_at, 1, LANES);
     const auto too_close = [&](float a, float b) { return fabsf(a - b) <= (by_score ? fminf(fabsf(a), fabsf(b)) * 0x1p-18f : margin); };
@@ -347,8 +355,29 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const typename Valu
       if (any_of_team<LANES>(wrong)) return false;
     }
   }
-  p_at = is ? share(s_at) : F(0);
-  sum = reduce_team<LANES>(p_at, [](F a, F b) { return a + b; });
+  // The weights.  p leaves fp32 at scores of -87 (of a softmax: below the largest), and a sum of such p with it; p / exp(base), with the largest of the
+  // chosen scores (of sigmoids: or 0) as base, has the same shares and does not.  A row whose chosen p are 0 in 64 bits has no weights.
+  constexpr float kNothing = -745.14f;   // exp of less rounds to 0 in 64 bits
+  const auto add = [](F a, F b) { return a + b; };
+  F base = r.sigmoid ? F(0) : top;
+  bool nothing = false;
+  if (r.normalize) {
+    const F most = reduce_team<LANES>(s_at, [](F a, F b) { return in_front(a, b) ? a : b; });
+    nothing = (r.sigmoid ? most : most - top) < kNothing;
+    base = !r.sigmoid || most < 0 ? most : F(0);
+  }
+  nothing = (nothing || base == kNone) && total == total;   // (masked experts; a softmax with a NaN or +infinity in its row is NaN throughout)
+  const F from_base = r.sigmoid && !(s_at < 0) ? F(0) : s_at;
+  const double power = exponential_of_difference(from_base, base);
+  F whole = r.sigmoid ? F(1) : total;
+  if (r.normalize) {
+    const F sum = reduce_team<LANES>((F)power * share_of_one, add);
+    whole = total == total ? sum : total;
+  }
+  F by;   // (1 / whole, in fp32 to one unit in the last place)
+  if constexpr (kFast) by = share_of_one * __builtin_amdgcn_rcpf(whole);
+  else by = share_of_one / whole;
+  weight = nothing ? 0.f : (float)(power * ((double)by * (double)r.scale));
   return true;
 }
 
@@ -368,11 +397,8 @@ __device__ __forceinline__ void load_bias(float (&bias)[V], const GroupRouter& r
     for (int j = 0; j < V; j++) bias[j] = r.bias[min(lane + LANES * j, r.experts - 1)];
   }
 }
-__device__ __forceinline__ void write_choice(const GroupRouter& r, int64_t t, int lane, int at, float p, float sum) {
-  if (lane < r.top_k) {
-    r.chosen[t * r.top_k + lane] = at;
-    r.weights[t * r.top_k + lane] = !r.normalize ? r.scale * p : sum == 0.f ? 0.f : r.scale * (p / sum);
-  }
+__device__ __forceinline__ void write_choice(const GroupRouter& r, int64_t t, int lane, int at, float weight) {
+  if (lane < r.top_k) r.chosen[t * r.top_k + lane] = at, r.weights[t * r.top_k + lane] = weight;
 }
 template <int DTYPE, int LANES, int V>
 __global__ __launch_bounds__(256) void group_top_experts_kernel(GroupRouter r) {
@@ -389,22 +415,21 @@ __global__ __launch_bounds__(256) void group_top_experts_kernel(GroupRouter r) {
   __syncthreads();
   if (first + team < r.tokens) {
     const stored* from = static_cast<const stored*>(r.scores) + (first + team) * r.stride;
-    float mine[V], bias[V], p, sum;
+    float mine[V], bias[V], weight;
     int at;
     load_scores<DTYPE, LANES>(mine, from, lane, r.experts), load_bias<LANES>(bias, r, lane);
-    if (choose<float, DTYPE, LANES, V>(r, from, mine, bias, rows.fast[team], lane, at, p, sum)) write_choice(r, first + team, lane, at, p, sum);
+    if (choose<float, DTYPE, LANES, V>(r, from, mine, bias, rows.fast[team], lane, at, weight)) write_choice(r, first + team, lane, at, weight);
     else if (lane == 0) again[atomicAdd(&agains, 1)] = team;
   }
   __syncthreads();
   for (int i = wave; i < agains; i += 4) {
     const int64_t t = first + again[i];
     const stored* from = static_cast<const stored*>(r.scores) + t * r.stride;
-    float mine[kWide], bias[kWide];
-    double p, sum;
+    float mine[kWide], bias[kWide], weight;
     int at;
     load_scores<DTYPE, 64>(mine, from, place, r.experts), load_bias<64>(bias, r, place);
-    choose<double, DTYPE, 64, kWide>(r, from, mine, bias, rows.wide[wave], place, at, p, sum);
-    write_choice(r, t, place, at, (float)p, (float)sum);
+    choose<double, DTYPE, 64, kWide>(r, from, mine, bias, rows.wide[wave], place, at, weight);
+    write_choice(r, t, place, at, weight);
     asm volatile("" : : : "memory");   // (a team lies in one wavefront, whose LDS accesses are made in order)
   }
 }

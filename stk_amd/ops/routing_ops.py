@@ -105,8 +105,8 @@ def group_top_experts(scores, top_k, groups=1, top_groups=1, scoring="sigmoid", 
 
     scores float16, bfloat16 or float32, at most 1024 experts, 64 groups, the top 32.  Which experts are chosen does not depend on how p is rounded: what fp32 does
     not tell apart is compared in 64 bits.  A score of -infinity masks an expert: it is chosen only where the kept groups have too few
-    others, and its weight is 0 (as every weight is where the sum of a normalised row is 0).  In a row with a NaN (softmax: or +infinity) the experts are valid
-    and distinct, and weights that it enters are NaN."""
+    others, and its weight is 0 (as every weight of a normalised row is where the chosen p are all 0 in 64 bits: a sigmoid below -745).  In a row
+    with a NaN (softmax: or +infinity) the experts are valid and distinct, and weights that it enters are NaN."""
     if scoring not in ("softmax", "sigmoid"):
         raise ValueError(f"unknown scoring {scoring!r}; one of ['sigmoid', 'softmax']")
     best = group_best if top_groups < groups else 1
