@@ -335,7 +335,8 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const typename Valu
     const float b_at = r.bias ? r.bias[at] : 0.f, c_at = by_score ? s_at : s_at == kNone ? kNone : (r.sigmoid ? (s_at < 0 ? t_at : 1.f) * share_of_one : share(s_at)) + b_at;
     // the order of the chosen
     const float next_c = __shfl_down(c_at, 1, LANES), next_s = __shfl_down(s_at, 1, LANES), next_b = __shfl_down(b_at, 1, LANES);
-    const auto too_close = [&](float a, float b) { return fabsf(a - b) <= (by_score ? fminf(fabsf(a), fabsf(b)) * 0x1p-18f : margin); };
+    // (16 numbers share a key: of scores below the normal numbers these are 2^-145 apart at most, whatever their size)
+    const auto too_close = [&](float a, float b) { return fabsf(a - b) <= (by_score ? fmaf(fminf(fabsf(a), fabsf(b)), 0x1p-18f, 0x1p-145f) : margin); };
     if (any_of_team<LANES>(lane < r.top_k - 1 && too_close(c_at, next_c) && !(s_at == next_s && b_at == next_b))) return false;
     // the last of them and those that are not chosen (whose keys tell c to 2^-19 of it)
     const float c_last = from_lane<LANES>(c_at, r.top_k - 1);
