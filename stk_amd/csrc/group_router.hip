@@ -217,7 +217,8 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const typename Valu
     if (any_of_team<LANES>(strange)) return false;
     largest_p = reduce_team<LANES>(largest_p, [](F a, F b) { return fmaxf(a, b); });
     if (r.bias) largest_b = reduce_team<LANES>(largest_b, [](F a, F b) { return fmaxf(a, b); });
-    margin = (largest_p + largest_b) * (r.sigmoid ? 0x1p-18f : 0x1p-17f);
+    // (the absolute part: a p below the normal numbers counts as 0 here, off by up to 2^-126, and a group has two)
+    margin = fmaf(largest_p + largest_b, r.sigmoid ? 0x1p-18f : 0x1p-17f, 0x1p-125f);
   }
   // ------------------------------------------------------------ groups
   uint64_t kept = ~0ull;

@@ -32,3 +32,14 @@ def test_subnormal_scores(tokens, scoring, unit):
     for groups, top_groups, best in ((1, 1, 1), (8, 3, 1), (8, 3, 2)):
         _same(scores, None, 8, groups, top_groups, best, scoring)
         _same(scores, None, 1, groups, top_groups, best, scoring)
+
+
+@pytest.mark.parametrize("tokens", [200, 2100])
+@pytest.mark.parametrize("bias", [False, True])
+def test_sums_of_sigmoids_below_the_normal_numbers(tokens, bias):
+    """A group's two best around 2^-126, where one of them may have no normal number and the other one."""
+    g = torch.Generator().manual_seed(3)
+    scores = torch.randn(tokens, 64, generator=g) * 0.7 - 87.3
+    b = torch.randn(64, generator=g) * 2.0 ** -127 if bias else None
+    _same(scores, b, 8, 8, 3, 2, "sigmoid")
+    _same(scores, b, 8, 8, 3, 1, "sigmoid")
