@@ -204,7 +204,8 @@ __device__ __forceinline__ bool choose(const GroupRouter& r, const typename Valu
       const F sum = c[j] + (F)bias[j];
       c[j] = mine[j] == -INFINITY ? kNone : sum;
     }
-    if constexpr (kFast) strange = max(most_p, most_b) >= 0x7f800000u, largest_p = __uint_as_float(most_p), largest_b = __uint_as_float(most_b);
+    // (from 2^126 on a group's sum may leave fp32)
+    if constexpr (kFast) strange = max(most_p, most_b) >= 0x7e800000u, largest_p = __uint_as_float(most_p), largest_b = __uint_as_float(most_b);
   }
   if (r.top_groups < r.groups) {
 #pragma unroll

@@ -43,3 +43,15 @@ def test_sums_of_sigmoids_below_the_normal_numbers(tokens, bias):
     b = torch.randn(64, generator=g) * 2.0 ** -127 if bias else None
     _same(scores, b, 8, 8, 3, 2, "sigmoid")
     _same(scores, b, 8, 8, 3, 1, "sigmoid")
+
+
+@pytest.mark.parametrize("tokens", [60, 2100])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_biases_whose_sum_leaves_fp32(tokens, scoring):
+    """Groups whose two best add up to more than fp32 has, above and below."""
+    scores = torch.randn(tokens, 16, generator=torch.Generator().manual_seed(4))
+    bias = torch.tensor([3.2, 3.0, -1.0, -2.0, 3.3, 3.1, -1.1, -2.2, 2.0, 1.0, 0.5, -2.5, 1.5, 0.7, 0.2, -2.6]) * 1e38
+    _same(scores, bias, 2, 4, 1, 2, scoring)
+    below = torch.tensor([-3.0, -3.3, -3.31, -3.32, 0.0, 1.0, 2.0, 3.0, -2.9, -3.1, -3.2, -3.25, -2.7, -2.8, -3.3, -3.32]) * 1e38
+    _same(scores, below, 1, 4, 3, 2, scoring)
+    _same(scores, below, 12, 4, 3, 2, scoring)
