@@ -18,6 +18,7 @@
 // keys of 32 bits: the ordered bits of c with the place in the lowest four, so that a lane's maximum says whose it is; what that takes off c is
 // within the margin of the 64-bit check.  A lane remembers the last of its keys that was chosen, t, and the largest key below is t plus the largest
 // key - t modulo 2^32: an instruction and a half for each key and round.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -504,7 +505,22 @@ static void for_team(const GroupRouter& r, Fn&& fn) {
   else if (r.experts <= 512) fn(Wave(), std::integral_constant<int, 8>());
   else fn(Wave(), std::integral_constant<int, 16>());
 }
-static dim3 group_router_grid(int64_t tokens, int lanes) { return dim3((unsigned)((tokens + 256 / lanes - 1) / (256 / lanes))); }
+// fn(first token, how many, grid): as many launches as it takes, since one may have less than 2^32 threads.
+constexpr int64_t kTokensOfLaunch = 1 << 24;
+template <class Fn>
+static void for_launches(int64_t tokens, int lanes, Fn&& fn) {
+  for (int64_t first = 0; first < tokens; first += kTokensOfLaunch) {
+    const int64_t here = std::min(tokens - first, kTokensOfLaunch);
+    fn(first, here, dim3((unsigned)((here + 256 / lanes - 1) / (256 / lanes))));
+  }
+}
+// r without its first tokens.
+template <class T>
+static GroupRouter part_of(GroupRouter r, int64_t first, int64_t here) {
+  r.scores = static_cast<const T*>(r.scores) + first * r.stride, r.tokens = here;
+  r.chosen += first * r.top_k, r.weights += first * r.top_k;
+  return r;
+}
 static int group_router_check(const char* who, GroupRouter& r, int64_t experts, int dtype) {
   if (!is_value_dtype(dtype)) return fail(STK_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
   if (r.tokens < 0 || experts < 1 || r.groups < 1 || experts % r.groups) return fail(STK_ERR_DIMS, "%s: %lld experts in %d groups", who, (long long)experts, r.groups);
@@ -533,9 +549,12 @@ extern "C" int stk_group_top_experts(const void* scores, int64_t tokens, int64_t
   if (!scores || !chosen || !weights) return fail(STK_ERR_DIMS, "%s: missing pointer", who);
   if (stride < 0) return fail(STK_ERR_DIMS, "%s: stride %lld", who, (long long)stride);
   for_dtype(dtype, [&](auto d) {
+    typedef typename Value<d()>::stored T;
     for_team(r, [&](auto lanes, auto v) {
       constexpr int D = decltype(d)::value, L = decltype(lanes)::value, V = decltype(v)::value;
-      hipLaunchKernelGGL((group_top_experts_kernel<D, L, V>), group_router_grid(tokens, L), dim3(256), 0, static_cast<hipStream_t>(stream), r);
+      for_launches(tokens, L, [&](int64_t first, int64_t here, dim3 grid) {
+        hipLaunchKernelGGL((group_top_experts_kernel<D, L, V>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), part_of<T>(r, first, here));
+      });
     });
   });
   return check_launch(who);
@@ -554,8 +573,10 @@ extern "C" int stk_group_top_experts_backward(const void* scores, int64_t stride
     typedef typename Value<d()>::stored T;
     for_team(r, [&](auto lanes, auto v) {
       constexpr int D = decltype(d)::value, L = decltype(lanes)::value, V = decltype(v)::value;
-      hipLaunchKernelGGL((group_top_experts_backward_kernel<D, L, V>), group_router_grid(tokens, L), dim3(256), 0, static_cast<hipStream_t>(stream), r, grad,
-                         static_cast<T*>(dscores), dscores_stride);
+      for_launches(tokens, L, [&](int64_t first, int64_t here, dim3 grid) {
+        hipLaunchKernelGGL((group_top_experts_backward_kernel<D, L, V>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), part_of<T>(r, first, here),
+                           grad + first * r.top_k, static_cast<T*>(dscores) + first * dscores_stride, dscores_stride);
+      });
     });
   });
   return check_launch(who);
