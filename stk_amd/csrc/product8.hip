@@ -1,7 +1,7 @@
 // Products of rows with 8-bit floating-point weights that have a scale for every block of 128 x 128, and the gradient of such weights.
 //   out = act(sum over blocks b of (sum over the inputs i of b of xq[i] wq[i][o]) sx[b] sw[b][o / 128])
 // xq, sx: the rows quantised as fp8.h says.  Powers of two go into the matrix instruction's own scale operands, one byte a line and block;
-// a weight's fp32 scale multiplies the fp32 sum of a block.
+// so does that of a weight's fp32 scale, whose mantissa multiplies the fp32 sum of a block.
 //
 // The matrix units multiply e4m3 values exactly and add the products of one instruction with some 13 bits below the largest of them (measured on
 // an MI355X, all fp8 instructions alike: products below 2^-13 of the largest lose bits, 2e-6 of the sum of magnitudes in the root mean square for
@@ -15,6 +15,19 @@
 #include "values.h"
 
 namespace stk {
+
+// A weight's fp32 scale as mantissa 2^(byte - 127): the power goes into the matrix instruction beside that of the rows, so that only a block's scaled sum has
+// to have a place in fp32, not the sum under the scale of the rows alone; the mantissa, in [1, 2) (below 2 for scales below the normal numbers), multiplies
+// it.  An infinity or a NaN stays mantissa.
+struct FloatScale8 {
+  int byte;
+  float mantissa;
+};
+__device__ __forceinline__ FloatScale8 float_scale8(float scale) {
+  const uint32_t u = __float_as_uint(scale), byte = u >> 23 & 255u;
+  if (byte == 255u) return {127, scale};
+  return {(int)byte, byte == 0u ? scale * 0x1p127f : __uint_as_float((u & 0x807fffffu) | 0x3f800000u)};
+}
 
 // ------------------------------------------------------------------------------------------------ few rows
 // 128 values of a row, of which this lane has 64 h + 16 quarter .. + 15, quantised together with the lanes 16, 32 and 48 away.
@@ -138,10 +151,10 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void stream8_kernel(Product8 p) {
       for (int i = 0; i < 8; i++) w[i] = (int)g.w[n][i / 4][i % 4];
       if constexpr (KIND == kPowerScales) total[n] = multiply8(w, values, total[n], g.scale[n], byte);
       else {
-        const f32x4_t part = multiply8(w, values, f32x4_t{0.f, 0.f, 0.f, 0.f}, 127, byte);
-        const float by = __uint_as_float((uint32_t)g.scale[n]);
+        const FloatScale8 by = float_scale8(__uint_as_float((uint32_t)g.scale[n]));
+        const f32x4_t part = multiply8(w, values, f32x4_t{0.f, 0.f, 0.f, 0.f}, by.byte, byte);
 #pragma unroll
-        for (int i = 0; i < 4; i++) total[n][i] = fmaf(part[i], by, total[n][i]);
+        for (int i = 0; i < 4; i++) total[n][i] = fmaf(part[i], by.mantissa, total[n][i]);
       }
     }
   };
@@ -289,7 +302,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile8_kernel(Product8 p, int 
     else wait_vmcnt<0>();
     __syncthreads();
     if (step + STAGES - 1 < count) issue(block + STAGES - 1, stage > 0 ? stage - 1 : STAGES - 1);
-    int row_scale[MT], col_scale[4] = {127, 127, 127, 127};
+    int row_scale[MT], col_scale[4];
     const int* exponents = reinterpret_cast<const int*>(smem + stage * T::kStage + T::kCodes);
 #pragma unroll
     for (int m = 0; m < MT; m++) row_scale[m] = exponents[16 * (m * WM + wm) + row] >> (8 * (block & 3));
@@ -297,7 +310,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile8_kernel(Product8 p, int 
 #pragma unroll
       for (int n = 0; n < 4; n++) col_scale[n] = exponents[T::kRows + 64 * wn + 16 * n + row] >> (8 * (block & 3));
     }
-    const float by = KIND == kFloatScales ? __uint_as_float((uint32_t)const_ints(float_scales)[block]) : 1.f;
+    const FloatScale8 by = float_scale8(KIND == kFloatScales ? __uint_as_float((uint32_t)const_ints(float_scales)[block]) : 1.f);
     const char* rows = smem + stage * T::kStage + wm * kPieceBytes8;
     const char* cols = smem + stage * T::kStage + T::kRowBytes + wn * 4 * kPieceBytes8 + lane * 16;
     const auto fragment = [&](const char* first, const char* second) {
@@ -321,13 +334,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile8_kernel(Product8 p, int 
 #pragma unroll
       for (int n = 0; n < 4; n++) {
         if constexpr (KIND == kPowerScales) total[m][n] = multiply8(w[n], values[m & 1], total[m][n], col_scale[n], row_scale[m]);
-        else part[n] = multiply8(w[n], values[m & 1], f32x4_t{0.f, 0.f, 0.f, 0.f}, 127, row_scale[m]);
+        else part[n] = multiply8(w[n], values[m & 1], f32x4_t{0.f, 0.f, 0.f, 0.f}, by.byte, row_scale[m]);
       }
       if constexpr (KIND == kFloatScales) {
 #pragma unroll
         for (int n = 0; n < 4; n++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) total[m][n][i] = fmaf(part[n][i], by, total[m][n][i]);
+          for (int i = 0; i < 4; i++) total[m][n][i] = fmaf(part[n][i], by.mantissa, total[m][n][i]);
       }
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // (the accesses to LDS come first)
       __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
