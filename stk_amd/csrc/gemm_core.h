@@ -169,16 +169,20 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 // in M0).  The load is tracked by vmcnt only; the caller waits for it.
 // STREAM: non-temporal hint for data that is read once, so that it does not
 // displace operands and results that are read again from the caches.
+// The base goes through a scalar move: where the vector unit has written it (readfirstlane, a spilled register coming back)
+// an access may read it five states later only, and the compiler does not see that this text is one; the scalar
+// unit waits by itself, and the move is the state that m0 wants in front of the access.
 template <bool STREAM = false>
 __device__ __forceinline__ void dma16(gptr_t base, uint32_t lane_offset, uint32_t lds_base) {
+  uint64_t from;
   if constexpr (STREAM)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
-                 :
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0 nt"
+                 : "=&s"(from)
                  : "s"(lds_base), "v"(lane_offset), "s"(base)
                  : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
+                 : "=&s"(from)
                  : "s"(lds_base), "v"(lane_offset), "s"(base)
                  : "memory", "m0");
 }
