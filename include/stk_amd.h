@@ -704,7 +704,7 @@ int stk_4bit_product_kernel(int64_t rows, int64_t experts, int64_t inputs, int64
  * largest scores - are chosen, in descending order, ties to the lower expert.
  *   weights[t][j] = scale * p[chosen[t][j]]        normalize: divided by the sum of p over the chosen ones; 0 where all of these
  *                                              are 0 in 64 bits (scores below -745, for softmax below the row's largest)
- * The choice is that of exact arithmetic: values closer than fp32 tells apart are compared in 64 bits.  scores as for stk_top_experts; at most 1024
+ * The choice is that of 64-bit arithmetic, in which values closer than fp32 tells apart are compared (what is equal there is a tie).  scores as for stk_top_experts; at most 1024
  * experts, 64 groups, the top 32.  A score of -infinity masks an expert: its weight is 0, and it is chosen only where the kept groups have too few
  * others.  In a row with a NaN (softmax: or +infinity) the chosen experts are valid and distinct and weights that depend on it are NaN.
  * Backward: the gradient with respect to the scores, every element of it, given that of the weights (grad [tokens, top_k], fp32).  The bias decides

@@ -10,9 +10,9 @@
 //
 // Which experts are chosen is to be a matter of the inputs, not of how exp is computed.  Everything is computed in fp32, whose error in c is below
 // 2^-19 (softmax: the sum's error counts) or 2^-21 (sigmoid) of the largest p and |bias|, and keys (below) lose another 2^-19; where two values that decide
-// the choice or its order are closer than twice the error and that, 2^-17 or 2^-18, and are not of equal inputs (which are equal whatever the precision), the token is done again in 64 bits, by a whole wavefront.  That is one token in some
-// hundred, but a wavefront waits for the slowest of its four.  Where the order of c is that of the scores (no bias, and one expert decides for its group)
-// the groups are compared by these.
+// the choice or its order are closer than twice the error and that, 2^-17 or 2^-18, and are not of equal inputs (which are equal whatever the precision), the
+// token is done again in 64 bits: one token in some hundred.  A workgroup collects its own and a wavefront takes each.  Where the order of c is that of
+// the scores (no bias, and one expert decides for its group) the groups are compared by these.
 //
 // A token belongs to a team of 16 or 64 lanes, and expert i to its lane i % LANES, place i / LANES.  A round of the choice is a maximum over
 // keys of 32 bits: the ordered bits of c with the place in the lowest four, so that a lane's maximum says whose it is; what that takes off c is

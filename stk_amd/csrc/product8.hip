@@ -207,6 +207,7 @@ struct Tile8 {
 template <int KIND, int WHAT, int WM, int WN, int MT, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile8_kernel(Product8 p, int row_tiles, int col_tiles) {
   typedef Tile8<WM, WN, MT, STAGES> T;
+  static_assert(STAGES == 2 || STAGES == 3, "what the waits below count");
   extern __shared__ char smem[];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   const int row = lane & 15, quarter = lane >> 4, in_fragment = in_fragment8(lane);
@@ -297,8 +298,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile8_kernel(Product8 p, int 
   for (int step = 0, stage = 0; step < count; step++, stage = stage + 1 < STAGES ? stage + 1 : 0) {
     const int block = begin + step;
     // everybody's part of the block is there, and everybody is done with the one whose place is filled now
-    if (STAGES > 3 && step + 2 < count) wait_vmcnt<2 * kMoves>();
-    else if (STAGES > 2 && step + 1 < count) wait_vmcnt<kMoves>();
+    if (STAGES > 2 && step + 1 < count) wait_vmcnt<kMoves>();
     else wait_vmcnt<0>();
     __syncthreads();
     if (step + STAGES - 1 < count) issue(block + STAGES - 1, stage > 0 ? stage - 1 : STAGES - 1);
@@ -446,6 +446,8 @@ static ProductKernel8 product_kernel8(int64_t rows, int64_t experts, int64_t inp
   if (each > 16 && tiles > (inputs % 8 ? 640 : 1792) && inputs <= kMostTileInputs8) {
     // Larger tiles read less, smaller ones fill the chip.  4096 x 4096, tiles of 32, 64, 128, 256 rows: 256 rows 21, 24, 29, 55 us; 1024 rows 44, 30, 34, 59;
     // 2048 rows 78, 57, 43, 62; 64 experts of 1024 x 4096, 20 rows each 72, 67, 72, 83, 64 rows each 105, 95, 97, 92, 128 rows each 162, 128, 131, 108.
+    // Experts of 256 +- 16 rows, half of which need a second tile of 256: 1024, 2048 and 4096 inputs 182, 250 and 438 by 256, 208, 312 and 561 by 128 (exactly
+    // 256 rows each: 134, 206, 358 and 192, 308, 550).
     const auto count = [&](int64_t high, int64_t wide) { return hit * ((each + high - 1) / high) * ((outputs + wide - 1) / wide); };
     if (each > 64 && count(256, 256) >= 192) return kTile8_256;
     if (each > 64 && count(128, 128) > 256) return kTile8_128;

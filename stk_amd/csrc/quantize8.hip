@@ -5,7 +5,7 @@
 // scales beside the codes, for nothing.  A block with an infinity or a NaN becomes NaN as a whole.
 //
 // All of it is bound by bytes: what is read once is written in every form that the products of a training step want of it.  16384 x 4096 bfloat16 along and down:
-// 53 us for 268 MB, 5.1 TB/s; 64 weights of 1024 x 4096 and their transposes 218 us for 1.07 GB; rows alone 22 us for 8192 x 4096.
+// 53 us for 268 MB, 5.1 TB/s; 64 weights of 1024 x 4096 and their transposes 218 - 226 us for 1.07 GB; rows alone 22 us for 8192 x 4096.
 #include "common.h"
 #include "fp8.h"
 #include "values.h"

@@ -95,16 +95,16 @@ class _GroupTopExperts(torch.autograd.Function):
 def group_top_experts(scores, top_k, groups=1, top_groups=1, scoring="sigmoid", bias=None, group_best=2, normalize=True, scale=1.0):
     """A router's choice among groups of experts given scores [tokens, experts] on the GPU: (experts, weights), both [tokens, top_k].
 
-    With p the scores' softmax over all experts or their sigmoid (scoring), and c = p + bias (one value for each expert, to balance them; None: 0): the experts
-    are `groups` groups of equal size, neighbours; a group counts as the sum of its group_best (1 or 2) largest c; the top_groups groups that count most are
-    kept, ties to the lower group.  Where all groups are kept group_best has no say.
+    With p the scores' softmax over all experts or their sigmoid (scoring), and c = p + bias (one value for each expert, to balance them, in float32 or rounded to
+    it; None: 0): the experts are `groups` groups of equal size, neighbours; a group counts as the sum of its group_best (1 or 2) largest c; the top_groups
+    groups that count most are kept, ties to the lower group.  Where all groups are kept group_best has no say.
     experts  int32, the top_k experts of these groups with the largest c (without a bias: the largest scores) in descending order, ties to the lower number: what
              route takes
     weights  fp32, scale times p - without the bias - at these places, with normalize divided by its sum over them: what padded_scatter takes;
              differentiable with respect to the scores
 
     scores float16, bfloat16 or float32, at most 1024 experts, 64 groups, the top 32.  Which experts are chosen does not depend on how p is rounded: what fp32 does
-    not tell apart is compared in 64 bits.  A score of -infinity masks an expert: it is chosen only where the kept groups have too few
+    not tell apart is compared in 64 bits, and what these do not is a tie.  A score of -infinity masks an expert: it is chosen only where the kept groups have too few
     others, and its weight is 0 (as every weight of a normalised row is where the chosen p are all 0 in 64 bits: a sigmoid below -745).  In a row
     with a NaN (softmax: or +infinity) the experts are valid and distinct, and weights that it enters are NaN."""
     if scoring not in ("softmax", "sigmoid"):
